@@ -296,6 +296,43 @@ int tf_qmm_prefill_act(const void* x, int64_t ldx, int m, const void* tiled, int
  * part: [sk, total] fp32; out: [total] bf16 or fp32. */
 int tf_reduce_slices(const float* part, int sk, int64_t total, void* out, int out_f32, void* stream);
 
+/* ---- microscaled 4-bit floating point ------------------------------------------------------------------------------
+ * Blocks of 32 neighbours along K: e2m1 codes (a sign and 0, 0.5, 1, 1.5, 2, 3, 4, 6; eight a 32-bit word, the first in the low
+ * bits) and one scale byte, the biased exponent of a power of two (255: NaN).  Stored layout, of checkpoints: words [n, k / 8] and
+ * scales [n, k / 32].  Quantising: scale code = max(exponent of the block's largest magnitude - 2, 0), values rounded to nearest
+ * even and saturated at 6; a block that holds an infinity or a NaN gets scale 255 and zero codes, and every sum it enters is
+ * NaN.  K is a positive multiple of 32 everywhere.  No counterpart in the reference, whose weights are affine integers.
+ *
+ * dtype / out_type: 0 bf16, 1 fp16, 2 fp32.  x: [rows, k], rows ldx elements apart on 16-byte boundaries. */
+int tf_mx_quantize(const void* x, int64_t ldx, int dtype, int rows, int k, void* words, void* scales, void* stream);
+int tf_mx_dequantize(const void* words, const void* scales, int rows, int k, int out_type, void* out, void* stream);
+/* Stored weights to the kernels' layout (super-blocks of 128 rows, each K in stages as the tensor cores read them) and back.
+ * tf_mx_pack: `experts` weights of n rows, one after another on both sides; with up_words and up_scales the n rows are n / 2 of
+ * the first projection (gate) and n / 2 of the second (up), interleaved in tiles of 16.  tiled: experts * tf_mx_tiled_bytes. */
+int64_t tf_mx_tiled_bytes(int n, int k);
+int tf_mx_pack(const void* words, const void* scales, const void* up_words, const void* up_scales, int experts, int n, int k, void* tiled,
+               void* stream);
+int tf_mx_unpack(const void* tiled, int n, int k, void* words, void* scales, void* stream);
+/* out[m, n] = x @ w.T with the rows of x quantised as above, products exact, sums fp32: K slices of tf_mx_split(n, k), each one
+ * chain of 64-input steps, added in order, so a row's bits never depend on m.  epi and limit as in tf_qmm_act, but activations
+ * are computed from the fp32 sums and rounded once.  pdl as in tf_qmm.
+ *   work     tf_mx_matmul_bytes(m, n, k) bytes (0 for decode and verify windows: the kernel quantises the rows itself), 16-byte
+ *            aligned, contents free; calls that may overlap need different work */
+int tf_mx_split(int n, int k);
+int64_t tf_mx_matmul_bytes(int m, int n, int k);
+int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
+                 void* work, int64_t work_bytes, int pdl, void* stream);
+/* The grouped form over a plan (tf_moe_plan, items of `tile` pairs: a multiple of 8 up to 128): as tf_moe_experts, with K in one
+ * slice.  Input: bf16 rows x with work of tf_mx_experts_bytes(k, tile, max_items) bytes, or with x NULL work that an earlier call
+ * filled as out_operands.  Output: out as in tf_moe_experts, or out_operands, where the results (activations: epi 1 or 2) are
+ * quantised from their fp32 values for the next projection: max_items * tf_mx_operand_bytes(tile, columns) bytes.  A pair's bits
+ * do not depend on the other pairs, nor on the tile. */
+int64_t tf_mx_operand_bytes(int rows, int k);
+int64_t tf_mx_experts_bytes(int k, int tile, int max_items);
+int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
+                  const int* counts, const int* members, int pairs, int max_items, int tile, void* out, int64_t ldo, int out_f32,
+                  void* out_operands, int epi, float limit, void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,18 @@ SIGNATURES = {
     "tf_sum_ranks": (_i32, (_vp, _i32, _i64, _i32, _vp, _i32, _vp)),
     "tf_qmm_prefill": (_i32, (_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _vp)),
     "tf_qmm_prefill_act": (_i32, (_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _i32, ctypes.c_float, _vp)),
+    "tf_mx_quantize": (_i32, (_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp)),
+    "tf_mx_dequantize": (_i32, (_vp, _vp, _i32, _i32, _i32, _vp, _vp)),
+    "tf_mx_tiled_bytes": (_i64, (_i32, _i32)),
+    "tf_mx_pack": (_i32, (_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp)),
+    "tf_mx_unpack": (_i32, (_vp, _i32, _i32, _vp, _vp, _vp)),
+    "tf_mx_split": (_i32, (_i32, _i32)),
+    "tf_mx_matmul_bytes": (_i64, (_i32, _i32, _i32)),
+    "tf_mx_matmul": (_i32, (_vp, _i64, _i32, _vp, _i32, _i32, _vp, _i64, _i32, _i32, ctypes.c_float, _vp, _i64, _i32, _vp)),
+    "tf_mx_operand_bytes": (_i64, (_i32, _i32)),
+    "tf_mx_experts_bytes": (_i64, (_i32, _i32, _i32)),
+    "tf_mx_experts": (_i32, (_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _i32,
+                             ctypes.c_float, _vp, _i64, _vp)),
     "tf_reduce_slices": (_i32, (_vp, _i32, _i64, _vp, _i32, _vp)),
 }
 

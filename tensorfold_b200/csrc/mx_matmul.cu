@@ -1,0 +1,805 @@
+// Products of microscaled 4-bit rows with microscaled 4-bit weights on the block-scaled tensor-core path:
+//
+//     out[m, n] = sum over blocks b of 2^(sx[m, b] - 127) 2^(sw[n, b] - 127) sum_{i in b} qx[m, i] qw[n, i]
+//
+// Products of e2m1 values and powers of two are exact; sums are fp32 in tensor memory.  K runs in `sk` slices, a function of the
+// weight's shape only; a slice is one chain of MMAs of 64 inputs, slices are added in order, so a row's bits depend neither on the
+// number of rows nor on which of the forms below runs it.
+//
+// "Swap-AB": the weights are the MMA's A operand (M = 128 output columns a block), the rows its B operand (N = 8 to 256).  Both lie
+// in memory as the MMA reads them (mx_layout.h), so a stage of 256 inputs is one bulk copy of 17 KB of weights beside the rows' copies; nothing
+// passes through registers.  Scales go from the stage to tensor memory (tcgen05.cp, the same thread that issues the MMAs), to
+// columns that belong to the stage's slot: they are free when the slot is.
+//
+// Forms (template): FUSED (up to 16 rows): bf16 rows are quantised by the block itself into shared memory while its weights
+// arrive, one launch in all; the block is bound by its weights' bytes.  Otherwise rows come quantised, as operands, in the ring.
+// `cluster` blocks (one a K slice) share a tile where there are few tiles: each sends its part to the block that owns the rows,
+// through distributed shared memory.  With a plan a tile is an item (expert, first, count) x 128 columns.
+//
+// Roles: warp 0 loads weights, warp 1 owns tensor memory and issues the MMAs, warp 2 loads rows, warps 4-11 drain (FUSED: 4-7
+// drain, 8-11 quantise, and where every tile has the same rows 4-7 help before they drain).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/tensorfold_b200.h"
+#include "mx_layout.h"
+#include "mx_quant.cuh"
+#include "tf_ptx.cuh"
+
+namespace tf {
+
+int fail_moe(int code, const char* msg);
+int cuda_fail_moe(cudaError_t e, const char* what);
+int* device_error_word();
+cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
+                           const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream);
+
+namespace {
+
+constexpr int MX_THREADS = 384;
+constexpr int MX_RING_MAX = 12;
+constexpr int MX_BAR_BYTES = 1024;
+constexpr int MX_SMEM_MAX = 232448 - 1024 /* alignment slack */ - MX_BAR_BYTES;
+constexpr int MX_FUSED_ROWS = 16;
+constexpr int MX_QUANT_COLS = 128;                 // columns of the buffer in which a drain group collects rows to quantise
+constexpr int MX_QUANT_ROWS = 16;
+constexpr int MX_QUANT_BYTES = MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;
+constexpr int MX_CLUSTER_MAX = 8;
+
+enum MxEpilogue : int { MX_STORE = 0, MX_RELU2 = 1, MX_SWIGLU = 2 };
+
+struct MxParams {
+  const uint8_t* w;
+  int64_t sb_bytes, expert_stride;
+  int N, M, K, steps, stages;
+  int sk, cluster;
+  int ring;                     // slots
+  int bufs;                     // FUSED: operands held in shared memory (2 with a plan, room permitting)
+  int operand_stages;           // FUSED: stages of the longest slice
+  // rows: operands (items `item_stride` bytes apart), or bf16 rows (FUSED)
+  const uint8_t* b;
+  int b_rows;
+  int64_t item_stride;
+  const __nv_bfloat16* x;
+  int64_t ldx;
+  int slots;                    // FUSED with a plan: rows of x are pair / slots (0: the pair itself)
+  int tile;                     // rows of a tile
+  void* out;
+  int64_t ldo;
+  int out_f32, epi;
+  float limit;
+  // result quantised into operands instead (one an item, q_rows rows of q_blocks blocks)
+  uint8_t* q;
+  int q_rows, q_steps;
+  int64_t q_item_stride;
+  const int *items, *counts, *members;
+  int experts, pairs, max_items;
+  int* err;
+};
+
+// Shared-memory matrix descriptors.  K-major, 8-row atoms one after another; swizzle 128 B (a stage's codes), 32 B (the last
+// stage's steps), or none (scales: 16-byte lines, 8 to an atom of 128 bytes).
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t atom_bytes, uint32_t swizzle) {
+  const uint32_t lo = ((addr >> 4) & 0x3FFFu) | (1u << 16);
+  const uint32_t hi = (atom_bytes >> 4) | (1u << 14) | (swizzle << 29);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+constexpr uint32_t SWIZZLE_NONE = 0, SWIZZLE_128 = 2, SWIZZLE_32 = 6;
+
+// e2m1 x e2m1 with power-of-two scales per 32 inputs, K = 64, M = 128.  `half`: which two of a line's four scales.
+__device__ __forceinline__ uint32_t instruction(int n, uint32_t half) {
+  return (half * 2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (1u << 27) | (half * 2u << 29);
+}
+
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+// 32 lines of 16 bytes to four columns, the same in each of the four lane groups.
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc(smem, 128, SWIZZLE_NONE)) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void let_copies_land() {
+  for (int i = 0; i < 64; ++i) __nanosleep(20000);
+}
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+
+// silu(gate) * up in fp32, clipped first where limit > 0.
+__device__ __forceinline__ float swiglu(float g, float u, float limit) {
+  if (limit > 0.f) {
+    g = fminf(g, limit);
+    u = fminf(fmaxf(u, -limit), limit);
+  }
+  return g / (1.f + expf(-g)) * u;
+}
+
+template <int NT, bool FUSED>
+struct MxShape {
+  static constexpr int SBS = (NT + MX_SB - 1) / MX_SB;
+  static constexpr int B_BYTES = NT * 128 + SBS * MX_SCALES;
+  static constexpr int SLOT = MX_UNIT + (FUSED ? 0 : B_BYTES);
+  static constexpr int ACCS = NT > 128 ? 1 : 2;                    // accumulators in turn
+  static constexpr int SF_COLS = 8 + 8 * SBS;                      // scale columns of a slot
+  static constexpr int TMEM = FUSED ? 256 : 512;
+  static constexpr int GROUPS = NT > 16 ? 2 : 1;                   // drain groups of four warps, NT / GROUPS columns each
+  static constexpr int COLS = NT / GROUPS;
+  static constexpr int RING = (TMEM - ACCS * NT) / SF_COLS < MX_RING_MAX ? (TMEM - ACCS * NT) / SF_COLS : MX_RING_MAX;
+};
+
+template <int NT, bool FUSED>
+__global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
+  using S = MxShape<NT, FUSED>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);              // [MX_RING_MAX] the slot's copies have landed
+  uint64_t* empty = full + MX_RING_MAX;                            // [MX_RING_MAX] the MMAs that read the slot are done
+  uint64_t* acc_full = empty + MX_RING_MAX;                        // [2]
+  uint64_t* acc_empty = acc_full + 2;                              // [2]
+  uint64_t* op_full = acc_empty + 2;                               // [2] FUSED: an operand is quantised
+  uint64_t* op_empty = op_full + 2;                                // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(op_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t ring0 = smem_addr(smem) + MX_BAR_BYTES;           // slots, FUSED operands, then the exchange buffers
+  const uint32_t operand0 = ring0 + p.ring * S::SLOT;
+  const uint32_t operand_bytes = FUSED ? p.operand_stages * S::B_BYTES : 0;
+  const uint32_t extra_off = MX_BAR_BYTES + p.ring * S::SLOT + p.bufs * operand_bytes;
+  const uint32_t abort_word = smem_addr(const_cast<int*>(abort_flag));
+
+  const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
+  const bool grouped = p.items != nullptr;
+  const int c = p.cluster, rank = c > 1 ? static_cast<int>(blockIdx.x % c) : 0;
+  const int full_stages = p.steps >> 2, tail = p.steps & 3;
+
+  auto give_up = [&](int code) {
+    if (lane == 0) {
+      *abort_flag = code;
+      atomicCAS(p.err, 0, code);
+    }
+  };
+
+  if (tid == 0) {
+    for (int i = 0; i < MX_RING_MAX; ++i) mbar_init(full + i, FUSED ? 1 : 2), mbar_init(empty + i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, 4 * S::GROUPS);
+      mbar_init(op_full + i, grouped ? 4 : 8), mbar_init(op_empty + i, 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (c > 1) cluster_barrier();                                    // the other blocks run before anything is sent to them
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+  pdl_launch_dependents();
+  if (grouped) pdl_wait();                                         // the plan may be the previous kernel's output
+
+  // Tiles: (row tile or item) x 128 columns, columns fastest.  A cluster takes every gridDim / c-th tile; FUSED with a plan a run
+  // of neighbours, so that its rows are quantised once an item.
+  const int ncb = (p.N + MX_SB - 1) / MX_SB;
+  const int row_tiles = grouped ? min(p.counts[0], p.max_items) : (p.M + p.tile - 1) / p.tile;
+  const int tiles = ncb * row_tiles, mine = blockIdx.x / c, clusters = gridDim.x / c;
+  const bool runs = FUSED && grouped;
+  const int first_tile = runs ? static_cast<int>(static_cast<int64_t>(tiles) * mine / clusters) : mine;
+  const int tile_step = runs ? 1 : clusters;
+  const int my_tiles = runs ? static_cast<int>(static_cast<int64_t>(tiles) * (mine + 1) / clusters) - first_tile
+                            : (mine < tiles ? (tiles - mine + clusters - 1) / clusters : 0);
+  const int slice0 = c > 1 ? rank : 0, slice1 = c > 1 ? rank + 1 : p.sk;
+
+  struct Tile {
+    int y, cb, m0, rows, n;                                        // item or row tile, column block, first row (or member), rows, MMA N
+    int64_t w;                                                     // offset of the weights
+  };
+  auto tile_at = [&](int it) {
+    const int t = first_tile + it * tile_step;
+    Tile ti;
+    ti.y = t / ncb, ti.cb = t - ti.y * ncb;
+    ti.w = ti.cb * p.sb_bytes;
+    if (grouped) {
+      const int* item = p.items + 3 * ti.y;
+      const int expert = __ldg(item);
+      // an item that names an expert outside the table runs against expert 0 with no rows and is reported
+      const bool known = expert >= 0 && expert < p.experts;
+      if (!known && threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BAD_ITEM);
+      ti.w += (known ? expert : 0) * p.expert_stride;
+      ti.m0 = __ldg(item + 1);
+      ti.rows = known ? min(p.tile, __ldg(item + 2)) : 0;
+      if (ti.m0 < 0 || ti.rows < 0 || ti.m0 > p.pairs - ti.rows) ti.rows = 0;
+    } else {
+      ti.m0 = ti.y * p.tile;
+      ti.rows = min(p.tile, p.M - ti.m0);
+    }
+    ti.n = max(8, (ti.rows + 7) & ~7);
+    return ti;
+  };
+  auto slice_at = [&](int s) { return static_cast<int>(static_cast<int64_t>(p.stages) * s / p.sk); };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ weights
+    bool ok = true;
+    int slot = 0;
+    uint32_t phase = 1;
+    for (int it = 0; it < my_tiles && ok; ++it) {
+      const Tile ti = tile_at(it);
+#pragma unroll 1
+      for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
+        ok = mbar32_wait(smem_addr(empty + slot), phase, abort_word);
+        if (!ok) break;
+        const uint32_t bytes = u < full_stages ? MX_UNIT : tail * 4096 + mx_tail_scales(tail);
+        if (elect_lane()) {
+          mbar32_expect_tx(smem_addr(full + slot), bytes);
+          bulk_load32(ring0 + slot * S::SLOT, p.w + ti.w + static_cast<int64_t>(u) * MX_UNIT, bytes, smem_addr(full + slot));
+        }
+        __syncwarp();
+        if (++slot == p.ring) slot = 0, phase ^= 1u;
+      }
+    }
+    if (!ok) give_up(ERR_WAIT_EMPTY), let_copies_land();
+  } else if (warp == 2 && !FUSED) {
+    // ------------------------------------------------------------------ quantised rows
+    pdl_wait();
+    bool ok = true;
+    int slot = 0;
+    uint32_t phase = 1;
+    const int64_t stage_bytes = mx_stage_bytes(p.b_rows);
+    for (int it = 0; it < my_tiles && ok; ++it) {
+      const Tile ti = tile_at(it);
+      const uint8_t* op = p.b + (grouped ? ti.y * p.item_stride : 0);
+      const int r0 = grouped ? 0 : ti.m0, sbs = mx_scale_blocks(ti.n);
+#pragma unroll 1
+      for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
+        ok = mbar32_wait(smem_addr(empty + slot), phase, abort_word);
+        if (!ok) break;
+        const bool whole = u < full_stages;
+        const uint32_t bar = smem_addr(full + slot), dst = ring0 + slot * S::SLOT + MX_UNIT;
+        const uint32_t scales = whole ? MX_SCALES : mx_tail_scales(tail);     // per 128 rows
+        const uint8_t* src = op + u * stage_bytes;
+        if (elect_lane()) {
+          mbar32_expect_tx(bar, ti.n * (whole ? 128 : 32 * tail) + sbs * scales);
+          if (whole) {
+            bulk_load32(dst, src + static_cast<int64_t>(r0) * 128, ti.n * 128, bar);
+            src += static_cast<int64_t>(p.b_rows) * 128;
+          } else {
+            for (int j = 0; j < tail; ++j) {
+              bulk_load32(dst + j * NT * 32, src + static_cast<int64_t>(r0) * 32, ti.n * 32, bar);
+              src += static_cast<int64_t>(p.b_rows) * 32;
+            }
+          }
+          bulk_load32(dst + NT * 128, src + (r0 / MX_SB) * scales, sbs * scales, bar);
+        }
+        __syncwarp();
+        if (++slot == p.ring) slot = 0, phase ^= 1u;
+      }
+    }
+    if (!ok) give_up(ERR_WAIT_EMPTY), let_copies_land();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issue
+    const uint32_t sf0 = tmem + S::ACCS * NT;
+    bool ok = true;
+    int slot = 0, use = 0, op = -1, last_y = -1;
+    uint32_t phase = 0;
+    for (int it = 0; it < my_tiles && ok; ++it) {
+      const Tile ti = tile_at(it);
+      bool new_op = false, last_of_op = false;
+      if (FUSED) {
+        new_op = grouped ? ti.y != last_y : it == 0;
+        last_y = ti.y;
+        if (new_op) {
+          ++op;
+          ok = mbar32_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word);
+          if (!ok) break;
+        }
+        last_of_op = grouped && (it + 1 == my_tiles || (first_tile + it + 1) / ncb != ti.y);
+      }
+      const uint32_t id0 = instruction(ti.n, 0), id1 = instruction(ti.n, 1);
+      for (int s = slice0; s < slice1 && ok; ++s, ++use) {
+        const int acc = use % S::ACCS, start = slice_at(s), end = slice_at(s + 1);
+        if (use >= S::ACCS) ok = mbar32_wait(smem_addr(acc_empty + acc), (use / S::ACCS - 1) & 1, abort_word);
+        const uint32_t d = tmem + acc * NT;
+#pragma unroll 1
+        for (int u = start; u < end && ok; ++u) {
+          ok = mbar32_wait(smem_addr(full + slot), phase, abort_word);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const bool whole = u < full_stages;
+          const int steps = whole ? 4 : tail;
+          const uint32_t a = ring0 + slot * S::SLOT;
+          const uint32_t b = FUSED ? operand0 + (op % p.bufs) * operand_bytes + (u - start) * S::B_BYTES : a + MX_UNIT;
+          const uint32_t a_scales = a + (whole ? MX_SB * 128 : tail * 4096), b_scales = b + NT * 128;
+          const uint32_t sb_bytes = whole || FUSED ? MX_SCALES : mx_tail_scales(tail);
+          const uint32_t sa = sf0 + slot * S::SF_COLS, sb = sa + 8;
+          if (elect_lane()) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (2 * h >= steps) break;
+              copy_scales(sa + 4 * h, a_scales + 512 * h);
+#pragma unroll
+              for (int q = 0; q < S::SBS; ++q) copy_scales(sb + 4 * S::SBS * h + 4 * q, b_scales + q * sb_bytes + 512 * h);
+            }
+            const uint64_t ad = whole ? desc(a, 1024, SWIZZLE_128) : desc(a, 256, SWIZZLE_32);
+            const uint64_t bd = whole ? desc(b, 1024, SWIZZLE_128) : desc(b, 256, SWIZZLE_32);
+            const uint32_t a_step = whole ? 2 : 4096 >> 4, b_step = whole ? 2 : NT * 32 >> 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (j >= steps) break;
+              mma_mxf4(d, ad + j * a_step, bd + j * b_step, j & 1 ? id1 : id0, sa + 4 * (j >> 1), sb + 4 * S::SBS * (j >> 1),
+                       u > start || j > 0);
+            }
+            commit(smem_addr(empty + slot));
+            if (u + 1 == end) {
+              commit(smem_addr(acc_full + acc));
+              if (FUSED && last_of_op) commit(smem_addr(op_empty + op % p.bufs));
+            }
+          }
+          __syncwarp();
+          if (++slot == p.ring) slot = 0, phase ^= 1u;
+        }
+      }
+    }
+    if (!ok) give_up(ERR_WAIT_FULL);
+  }
+
+  if (FUSED && (grouped ? warp >= 8 : warp >= 4)) {
+    // ------------------------------------------------------------------ bf16 rows -> operand in shared memory
+    // Four lanes a block as everywhere; a thread has four 16-byte loads in flight.
+    if (!grouped) pdl_wait();
+    const int qt = grouped ? tid - 256 : tid - 128, qthreads = grouped ? 128 : 256;
+    bool ok = true;
+    int op = -1, last_y = -1;
+    const int u0 = slice_at(slice0), u1 = slice_at(slice1);
+    const int p0 = u0 * 32, pieces = min(p.steps * 8, u1 * 32) - p0;   // 16-byte pieces of a row in this slice (K padded to 64)
+    for (int it = 0; it < my_tiles && ok; ++it) {
+      const Tile ti = tile_at(it);
+      if (grouped ? ti.y == last_y : it > 0) continue;
+      last_y = ti.y;
+      ++op;
+      if (op >= p.bufs) {
+        ok = mbar32_wait(smem_addr(op_empty + op % p.bufs), (op / p.bufs - 1) & 1, abort_word);
+        if (!ok) break;
+      }
+      uint8_t* base = smem + (operand0 - smem_addr(smem)) + (op % p.bufs) * operand_bytes;
+      const int total = ti.rows * pieces;                            // a multiple of 8
+      for (int i0 = 0; i0 < total; i0 += 4 * qthreads) {
+        uint4 v4[4];
+        int rr[4], pp[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + j * qthreads + qt;
+          rr[j] = i / pieces, pp[j] = i - rr[j] * pieces;
+          v4[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (i < total && (p0 + pp[j]) * 8 < p.K) {
+            int64_t row = rr[j];
+            bool live = true;
+            if (grouped) {
+              const int pair = p.members[ti.m0 + rr[j]];
+              live = pair >= 0 && pair < p.pairs;
+              row = p.slots > 0 ? pair / p.slots : pair;
+            }
+            if (live) v4[j] = *(reinterpret_cast<const uint4*>(p.x + row * p.ldx) + p0 + pp[j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v[8];
+          widen8(v4[j], v);
+          uint32_t scale;
+          const uint32_t codes = quantize_block(v, scale);
+          if (i0 + j * qthreads + qt < total) {
+            const int b = pp[j] >> 2, u = b >> 3, r = rr[j];
+            uint8_t* stage = base + u * S::B_BYTES;
+            const uint32_t at = u0 + u < full_stages ? (r >> 3) * 1024 + (r & 7) * 128 + (((b & 7) ^ (r & 7)) << 4)
+                                                     : ((b & 7) >> 1) * (NT * 32) + (r >> 3) * 256 + (r & 7) * 32 + (((b & 1) ^ ((r >> 2) & 1)) << 4);
+            *reinterpret_cast<uint32_t*>(stage + at + 4 * (pp[j] & 3)) = codes;
+            if ((pp[j] & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + r * 16 + (b & 3)] = static_cast<uint8_t>(scale);
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(op_full + op % p.bufs);
+    }
+    if (!ok) give_up(ERR_WAIT_EMPTY);
+  }
+
+  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 unless they quantise)
+  const bool drains = warp >= 4 && group < S::GROUPS;
+  const int lg = warp & 3, col0 = group * S::COLS;
+  // acc values of one row of the tile, a lane a column: stored, or two rows (n, n + 1) of SwiGLU, gate in lanes 0-15
+  const int ncols = p.epi == MX_SWIGLU ? p.N / 2 : p.N;
+  auto store = [&](const Tile& ti, float v, int n, int col) {
+    if (n < ti.rows && col < ncols) {
+      const int64_t row = grouped && p.members != nullptr ? p.members[ti.m0 + n] : ti.m0 + n;
+      if (grouped && (row < 0 || row >= p.pairs)) return;
+      if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + col] = v;
+      else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + col] = __float2bfloat16_rn(v);
+    }
+  };
+  auto finish2 = [&](const Tile& ti, float v0, float v1, int n) {
+    if (p.epi == MX_SWIGLU) {
+      const bool low = lane < 16;
+      const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v1 : v0, 16);
+      const float a = swiglu(low ? v0 : got, low ? got : v1, p.limit);
+      store(ti, a, n + (low ? 0 : 1), ti.cb * 64 + lg * 16 + (lane & 15));
+    } else {
+      if (p.epi == MX_RELU2) v0 = fmaxf(v0, 0.f), v1 = fmaxf(v1, 0.f), v0 *= v0, v1 *= v1;
+      store(ti, v0, n, ti.cb * MX_SB + lg * 32 + lane);
+      store(ti, v1, n + 1, ti.cb * MX_SB + lg * 32 + lane);
+    }
+  };
+
+  if (drains) {
+    // ------------------------------------------------------------------ drain
+    pdl_wait();                                                      // nothing is written before the previous kernel is done
+    bool ok = true;
+    int use = 0;
+    const uint32_t my_tmem = tmem + (static_cast<uint32_t>(lg * 32) << 16) + col0;
+    for (int it = 0; it < my_tiles && ok; ++it) {
+      const Tile ti = tile_at(it);
+      float acc[S::COLS];
+      for (int s = slice0; s < slice1 && ok; ++s, ++use) {
+        const int ab = use % S::ACCS;
+        ok = mbar32_wait(smem_addr(acc_full + ab), (use / S::ACCS) & 1, abort_word);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t src = my_tmem + ab * NT;
+        if (s == slice0) {
+#pragma unroll
+          for (int i = 0; i < S::COLS; i += 16)
+            if (col0 + i < ti.n) tmem_load16(src + i, acc + i);
+          tmem_loaded();
+        } else {
+#pragma unroll
+          for (int i = 0; i < S::COLS; i += 16) {
+            if (col0 + i < ti.n) {
+              float v[16];
+              tmem_load16(src + i, v);
+              tmem_loaded();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[i + j] = acc[i + j] + v[j];
+            }
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + ab);
+      }
+      if (!ok) break;
+      if (c > 1) {
+        // part [slice][row of the owner][128 columns] in the shared memory of the block that owns the row
+        const int share = (ti.n + c - 1) / c;
+        const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 4;
+#pragma unroll
+        for (int i = 0; i < S::COLS; ++i) {
+          const int n = col0 + i;
+          if (n < ti.n) {
+            const int owner = n / share;
+            store_remote(part + (rank * share + n - owner * share) * (MX_SB * 4), owner, acc[i]);
+          }
+        }
+      } else if (p.q != nullptr) {
+        // rows of activations, sixteen at a time through shared memory, where four lanes see a block
+        const int width = p.epi == MX_SWIGLU ? 64 : 128;
+        float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES);
+        uint8_t* op = p.q + ti.y * p.q_item_stride;
+        const int gt = (lg << 5) | lane;
+#pragma unroll
+        for (int i = 0; i < S::COLS; i += MX_QUANT_ROWS) {
+          if (col0 + i >= ti.rows) break;
+          named_barrier(1 + group, 128);                             // the last sixteen rows have been read
+#pragma unroll
+          for (int j = 0; j < MX_QUANT_ROWS; j += 2) {
+            float v0 = acc[i + j], v1 = acc[i + j + 1];
+            if (p.epi == MX_SWIGLU) {
+              const bool low = lane < 16;
+              const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v1 : v0, 16);
+              rows[(j + (low ? 0 : 1)) * (MX_QUANT_COLS + 4) + lg * 16 + (lane & 15)] = swiglu(low ? v0 : got, low ? got : v1, p.limit);
+            } else {
+              if (p.epi == MX_RELU2) v0 = fmaxf(v0, 0.f), v1 = fmaxf(v1, 0.f), v0 *= v0, v1 *= v1;
+              rows[j * (MX_QUANT_COLS + 4) + lg * 32 + lane] = v0;
+              rows[(j + 1) * (MX_QUANT_COLS + 4) + lg * 32 + lane] = v1;
+            }
+          }
+          named_barrier(1 + group, 128);
+          for (int t = gt; t < MX_QUANT_ROWS * width / 8; t += 128) {
+            const int r = t / (width / 8), piece = t - r * (width / 8), n = col0 + i + r;
+            const float4* from = reinterpret_cast<const float4*>(rows + r * (MX_QUANT_COLS + 4) + piece * 8);
+            const float4 lo = from[0], hi = from[1];
+            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            uint32_t scale;
+            const uint32_t codes = quantize_block(v, scale);
+            const int b = ti.cb * (width / 32) + (piece >> 2);
+            if (n < ti.rows && b < 2 * p.q_steps) {
+              *reinterpret_cast<uint32_t*>(op + mx_code_offset(p.q_rows, p.q_steps, n, b) + 4 * (piece & 3)) = codes;
+              if ((piece & 3) == 0) op[mx_scale_offset(p.q_rows, p.q_steps, n, b)] = static_cast<uint8_t>(scale);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::COLS; i += 2)
+          if (col0 + i < ti.rows) finish2(ti, acc[i], acc[i + 1], col0 + i);
+      }
+    }
+    if (!ok) give_up(ERR_WAIT_FULL);
+  }
+
+  if (c > 1) {
+    // The host launches one tile a cluster: every block's part has been sent when this barrier opens (parts of blocks that
+    // gave up are missing, which the error word says).
+    __syncwarp();
+    cluster_barrier();
+    if (drains && my_tiles > 0 && *abort_flag == 0) {
+      const Tile ti = tile_at(0);
+      const int share = (ti.n + c - 1) / c, n0 = rank * share;
+      const float* part = reinterpret_cast<const float*>(smem + extra_off) + lg * 32 + lane;
+      for (int i = 2 * group; i < share; i += 2 * S::GROUPS) {
+        float v0 = 0.f, v1 = 0.f;
+        for (int s = 0; s < c; ++s) {
+          const float a = part[(s * share + i) * MX_SB], b = i + 1 < share ? part[(s * share + i + 1) * MX_SB] : 0.f;
+          v0 = s == 0 ? a : v0 + a, v1 = s == 0 ? b : v1 + b;
+        }
+        Tile own = ti;
+        own.rows = min(ti.rows, n0 + share);                         // row i + 1 may be the next block's
+        finish2(own, v0, v1, n0 + i);
+      }
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+
+int g_mx_sms[64] = {};
+
+int device_sms() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  return g_mx_sms[dev];
+}
+
+// K slices of an (n, k) weight: enough (128-column block, slice) units for one block an SM, no slice below two stages.
+int slices_for(int n, int k) {
+  const int blocks = (n + MX_SB - 1) / MX_SB, stages = mx_stages(mx_steps(k));
+  return std::max(1, std::min({MX_CLUSTER_MAX, 148 / std::min(blocks, 148), stages / 2}));
+}
+
+template <int NT, bool FUSED>
+cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
+  using S = MxShape<NT, FUSED>;
+  int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
+  if (p.cluster > 1) extra = (NT + p.cluster) * MX_SB * 4;
+  const int operand = FUSED ? p.operand_stages * S::B_BYTES : 0;
+  if (FUSED && p.bufs == 2 && MX_SMEM_MAX - extra - 2 * operand < 4 * S::SLOT) p.bufs = 1;
+  const int room = MX_SMEM_MAX - extra - p.bufs * operand;
+  p.ring = std::min(S::RING, room / S::SLOT);
+  if (p.ring < 2) return cudaErrorInvalidConfiguration;              // (the callers' rules keep shapes that would not fit out)
+  const int64_t most = std::max(1, sms / p.cluster);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.cluster > 1 ? tiles : std::min(tiles, most)) * p.cluster));
+  cfg.blockDim = dim3(MX_THREADS);
+  cfg.dynamicSmemBytes = 1024 + MX_BAR_BYTES + p.ring * S::SLOT + p.bufs * operand + extra;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  int count = 0;
+  if (p.cluster > 1) {
+    attrs[count].id = cudaLaunchAttributeClusterDimension;
+    attrs[count].val.clusterDim.x = p.cluster, attrs[count].val.clusterDim.y = 1, attrs[count].val.clusterDim.z = 1;
+    ++count;
+  }
+  if (pdl) {
+    attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[count].val.programmaticStreamSerializationAllowed = 1;
+    ++count;
+  }
+  cfg.attrs = attrs;
+  cfg.numAttrs = count;
+  return cudaLaunchKernelEx(&cfg, mx_kernel<NT, FUSED>, p);
+}
+
+template <int NT, bool FUSED>
+cudaError_t configure() {
+  return cudaFuncSetAttribute(mx_kernel<NT, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+}
+
+// The tile of a call of m rows whose rows come as operands.
+cudaError_t launch_rows(MxParams& p, int nt, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
+  p.tile = std::min(p.tile, nt);
+  switch (nt) {
+    case 16: return launch<16, false>(p, tiles, quant_out, sms, pdl, stream);
+    case 64: return launch<64, false>(p, tiles, quant_out, sms, pdl, stream);
+    case 128: return launch<128, false>(p, tiles, quant_out, sms, pdl, stream);
+    default: return launch<256, false>(p, tiles, quant_out, sms, pdl, stream);
+  }
+}
+
+int rows_padded(int m) { return m > MX_SB ? (m + MX_SB - 1) / MX_SB * MX_SB : (m + 7) / 8 * 8; }
+
+// Whether a block can hold its K slice of sixteen quantised rows beside a ring of four slots.
+bool fused_fits(int k, int sk) {
+  const int stages = mx_stages(mx_steps(k)), longest = (stages + sk - 1) / sk;
+  return longest * MxShape<16, true>::B_BYTES + 4 * MX_UNIT + (MX_FUSED_ROWS + MX_CLUSTER_MAX) * MX_SB * 4 <= MX_SMEM_MAX;
+}
+
+bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+}  // namespace
+
+cudaError_t mx_configure(int device, int sms) {
+  cudaError_t e = configure<16, true>();
+  if (e == cudaSuccess) e = configure<16, false>();
+  if (e == cudaSuccess) e = configure<64, false>();
+  if (e == cudaSuccess) e = configure<128, false>();
+  if (e == cudaSuccess) e = configure<256, false>();
+  if (e == cudaSuccess && device >= 0 && device < 64) g_mx_sms[device] = sms;
+  return e;
+}
+
+}  // namespace tf
+
+using namespace tf;
+
+extern "C" {
+
+int tf_mx_split(int n, int k) { return n < 1 || k < MX_BLOCK || k % MX_BLOCK ? TF_ERR_ARG : slices_for(n, k); }
+
+int64_t tf_mx_matmul_bytes(int m, int n, int k) {
+  if (m < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  if (m <= MX_FUSED_ROWS && fused_fits(k, slices_for(n, k))) return 0;
+  return mx_operand_bytes(rows_padded(m), mx_steps(k));
+}
+
+int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
+                 void* work, int64_t work_bytes, int pdl, void* stream) {
+  if (m < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: K must be a positive multiple of 32, n and m positive");
+  if (epi < 0 || epi > 2 || (epi == 2 && n % 32) || (epi != 0 && out_f32)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: bad epilogue");
+  if (!x || !tiled || !out || ldo < (epi == 2 ? n / 2 : n) || ldx < k) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: null pointer or short rows");
+  if (misaligned(x, 16) || (m > 1 && ldx % 8)) return fail_moe(TF_ERR_ALIGN, "tf_mx_matmul: x rows must start on 16-byte boundaries");
+  if (misaligned(tiled, 16) || misaligned(work, 16)) return fail_moe(TF_ERR_ALIGN, "tf_mx_matmul: tiled weights and work must be 16-byte aligned");
+  if (misaligned(out, out_f32 ? 4 : 2)) return fail_moe(TF_ERR_ALIGN, "tf_mx_matmul: out is not aligned to its type");
+  const int64_t need = tf_mx_matmul_bytes(m, n, k);
+  if (need > 0 && (!work || work_bytes < need)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: work is smaller than tf_mx_matmul_bytes");
+  int* err = device_error_word();
+  const int sms = device_sms();
+  if (err == nullptr || sms < 1) return fail_moe(TF_ERR_STATE, "tf_mx_matmul: tf_init has not been called for the current device");
+  MxParams p = {};
+  p.w = static_cast<const uint8_t*>(tiled);
+  p.N = n, p.M = m, p.K = k;
+  p.steps = mx_steps(k), p.stages = mx_stages(p.steps);
+  p.sb_bytes = mx_operand_bytes(MX_SB, p.steps);
+  p.sk = slices_for(n, k);
+  p.out = out, p.ldo = ldo, p.out_f32 = out_f32, p.epi = epi, p.limit = limit;
+  p.err = err;
+  p.bufs = 1;
+  const int64_t ncb = (n + MX_SB - 1) / MX_SB;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (need == 0) {
+    p.x = static_cast<const __nv_bfloat16*>(x), p.ldx = ldx;
+    p.tile = MX_FUSED_ROWS;
+    p.cluster = p.sk;
+    p.operand_stages = (p.stages + p.sk - 1) / p.sk;
+    e = launch<16, true>(p, ncb, false, sms, pdl != 0, s);
+  } else {
+    const int rows = rows_padded(m);
+    e = mx_rows_launch(x, ldx, m, k, rows, 0, 0, nullptr, nullptr, nullptr, 0, 0, 0, work, pdl != 0, s);
+    if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
+    p.b = static_cast<const uint8_t*>(work), p.b_rows = rows;
+    const int nt = m <= 16 ? 16 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+    p.tile = nt;
+    const int64_t row_tiles = (m + nt - 1) / nt;
+    if (ncb * row_tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: too many tiles");
+    p.cluster = nt <= 128 ? p.sk : 1;
+    // the rows' kernel lets this one set up and fetch weights while it runs; the weights were settled before it started
+    e = launch_rows(p, nt, ncb * row_tiles, false, sms, true, s);
+  }
+  return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_matmul");
+}
+
+int64_t tf_mx_operand_bytes(int rows, int k) {
+  if (rows < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  return mx_operand_bytes(rows_padded(rows), mx_steps(k));
+}
+
+int64_t tf_mx_experts_bytes(int k, int tile, int max_items) {
+  if (tile < 8 || tile > MX_SB || max_items < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  return tile <= MX_FUSED_ROWS && fused_fits(k, 1) ? 0 : max_items * mx_operand_bytes(rows_padded(tile), mx_steps(k));
+}
+
+int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
+                  const int* counts, const int* members, int pairs, int max_items, int tile, void* out, int64_t ldo, int out_f32,
+                  void* out_operands, int epi, float limit, void* work, int64_t work_bytes, void* stream) {
+  if (experts < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || pairs < 1 || max_items < 1 || max_items > (1 << 20) || slots < 0)
+    return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad sizes (K a positive multiple of 32)");
+  if (tile < 8 || tile > MX_SB || tile % 8) return fail_moe(TF_ERR_ARG, "tf_mx_experts: items of 8 to 128 pairs, in whole eights");
+  if (epi < 0 || epi > 2 || (epi == 2 && n % 32)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad epilogue");
+  if (!tiled || !items || !counts || !members || (out == nullptr) == (out_operands == nullptr))
+    return fail_moe(TF_ERR_ARG, "tf_mx_experts: null pointer, or not one of out and out_operands");
+  const int ncols = epi == 2 ? n / 2 : n;
+  if (out && (ldo < ncols || (epi != 0 && out_f32))) return fail_moe(TF_ERR_ARG, "tf_mx_experts: short rows, or activations in fp32");
+  if (out_operands && ncols % MX_BLOCK) return fail_moe(TF_ERR_ARG, "tf_mx_experts: quantised results have a multiple of 32 columns");
+  if (x && (ldx < k || misaligned(x, 16) || ldx % 8)) return fail_moe(TF_ERR_ALIGN, "tf_mx_experts: x rows must start on 16-byte boundaries");
+  if (misaligned(tiled, 16) || expert_stride % 16 || misaligned(work, 16) || misaligned(out_operands, 16) || misaligned(out, out_f32 ? 4 : 2))
+    return fail_moe(TF_ERR_ALIGN, "tf_mx_experts: weights, work and operands must start on 16-byte boundaries");
+  const int rows = rows_padded(tile);
+  const int64_t operand = mx_operand_bytes(rows, mx_steps(k)), need = x ? tf_mx_experts_bytes(k, tile, max_items) : max_items * operand;
+  if (need > 0 && (!work || work_bytes < need)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: work is too small");
+  int* err = device_error_word();
+  const int sms = device_sms();
+  if (err == nullptr || sms < 1) return fail_moe(TF_ERR_STATE, "tf_mx_experts: tf_init has not been called for the current device");
+  MxParams p = {};
+  p.w = static_cast<const uint8_t*>(tiled);
+  p.N = n, p.M = pairs, p.K = k;
+  p.steps = mx_steps(k), p.stages = mx_stages(p.steps);
+  p.sb_bytes = mx_operand_bytes(MX_SB, p.steps), p.expert_stride = expert_stride;
+  p.sk = 1, p.cluster = 1;
+  p.out = out, p.ldo = ldo, p.out_f32 = out_f32, p.epi = epi, p.limit = limit;
+  if (out_operands) {
+    p.q = static_cast<uint8_t*>(out_operands), p.q_rows = rows, p.q_steps = mx_steps(ncols);
+    p.q_item_stride = mx_operand_bytes(rows, p.q_steps);
+  }
+  p.items = items, p.counts = counts, p.members = members, p.experts = experts, p.pairs = pairs, p.max_items = max_items;
+  p.err = err;
+  p.tile = tile;
+  const int64_t tiles = static_cast<int64_t>((n + MX_SB - 1) / MX_SB) * max_items;       // upper bound: the plan says how many
+  if (tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: too many tiles");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (x && need == 0) {
+    p.x = static_cast<const __nv_bfloat16*>(x), p.ldx = ldx, p.slots = slots;
+    p.bufs = 2, p.operand_stages = p.stages;
+    e = launch<16, true>(p, tiles, out_operands != nullptr, sms, false, s);
+  } else {
+    if (x) {
+      e = mx_rows_launch(x, ldx, 0, k, rows, tile, operand, items, counts, members, slots, pairs, max_items, work, false, s);
+      if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_experts: rows");
+    }
+    p.b = static_cast<const uint8_t*>(work), p.b_rows = rows, p.item_stride = operand;
+    p.bufs = 1;
+    e = launch_rows(p, tile <= 16 ? 16 : tile <= 64 ? 64 : 128, tiles, out_operands != nullptr, sms, x != nullptr, s);
+  }
+  return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_experts");
+}
+
+}  // extern "C"

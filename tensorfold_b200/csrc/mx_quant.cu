@@ -1,0 +1,277 @@
+// Microscaled 4-bit floating point: quantise and read back (stored layout), weights to and from the operand layout, rows to the
+// operand layout.  All of them move bytes; the arithmetic is in mx_quant.cuh.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/tensorfold_b200.h"
+#include "mx_layout.h"
+#include "mx_quant.cuh"
+#include "tf_ptx.cuh"
+
+namespace tf {
+
+int fail_moe(int code, const char* msg);
+int cuda_fail_moe(cudaError_t e, const char* what);
+
+namespace {
+
+// Eight values of one of the stored types: 0 bf16, 1 fp16, 2 fp32.
+__device__ __forceinline__ void load8(const void* row, int64_t at, int dtype, float (&v)[8]) {
+  if (dtype == 0) {
+    widen8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(row) + at), v);
+  } else if (dtype == 1) {
+    const uint4 p = *reinterpret_cast<const uint4*>(static_cast<const __half*>(row) + at);
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  } else {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
+    const float4 a = p[0], b = p[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+}
+
+// Rows to stored words and scales.  A lane takes eight values, four lanes a block, so loads and stores of a warp are runs.
+__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int64_t ldx, int dtype, int64_t pieces, int per_row,
+                                                       uint32_t* __restrict__ words, uint8_t* __restrict__ scales) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  // whole warps walk together: a piece past the end computes on zeros and stores nothing
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31); first < pieces; first += step) {
+    const int64_t i = first + (threadIdx.x & 31);
+    float v[8] = {};
+    const int64_t r = i / per_row;
+    if (i < pieces) load8(static_cast<const char*>(x) + r * ldx * (dtype == 2 ? 4 : 2), (i - r * per_row) * 8, dtype, v);
+    uint32_t scale;
+    const uint32_t codes = quantize_block(v, scale);
+    if (i < pieces) {
+      words[i] = codes;
+      if ((i & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(scale);
+    }
+  }
+}
+
+// Stored words and scales to values.  Every value is exact in bf16 and fp32 but where 2^127 or more overflows bf16's largest.
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ words, const uint8_t* __restrict__ scales, int64_t pieces,
+                                                         int out_type, void* __restrict__ out) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < pieces; i += step) {
+    const uint32_t w = words[i], code = scales[i >> 2];
+    const float scale = __uint_as_float(code == 255u ? 0x7FC00000u : code == 0u ? 0x00400000u : code << 23);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t q = w >> (4 * j);
+      // e2m1 to fp32: two exponent bits and one of fraction; the only subnormal is 0.5
+      const uint32_t m = q & 7u;
+      const float a = m < 2u ? (m ? 0.5f : 0.f) : __uint_as_float((m << 22) + (126u << 23));
+      v[j] = ((q & 8u) ? -a : a) * scale;
+    }
+    if (out_type == 2) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + i * 8);
+      o[0] = make_float4(v[0], v[1], v[2], v[3]), o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (out_type == 0) {
+          const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          p[j] = *reinterpret_cast<const uint32_t*>(&t);
+        } else {
+          const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          p[j] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+      }
+      reinterpret_cast<uint4*>(out)[i] = make_uint4(p[0], p[1], p[2], p[3]);
+    }
+  }
+}
+
+// Stored weights to super-blocks and back.  A thread takes 16 bytes of codes (one block); eight neighbours write the 128 bytes of
+// one swizzle line.  `up` interleaves a second projection in tiles of 16 rows.  Rows and inputs past the end become zeros.
+__global__ void __launch_bounds__(256) pack_kernel(const uint4* __restrict__ words, const uint8_t* __restrict__ scales,
+                                                   const uint4* __restrict__ up_words, const uint8_t* __restrict__ up_scales, int n, int blocks,
+                                                   int steps, int64_t sb_bytes, uint8_t* __restrict__ tiled) {
+  const int padded = 2 * steps, nsb = (n + MX_SB - 1) / MX_SB;
+  const int64_t total = static_cast<int64_t>(nsb) * MX_SB * padded, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t expert = blockIdx.y;
+  const bool pair = up_words != nullptr;
+  const int each = pair ? n / 2 : n;
+  words += expert * each * blocks, scales += expert * each * blocks;
+  if (pair) up_words += expert * each * blocks, up_scales += expert * each * blocks;
+  tiled += expert * nsb * sb_bytes;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int row = static_cast<int>(i / padded), b = static_cast<int>(i - static_cast<int64_t>(row) * padded);
+    uint4 codes = make_uint4(0u, 0u, 0u, 0u);
+    uint8_t scale = 0;
+    if (row < n && b < blocks) {
+      const bool second = pair && mx_pair_second(row);
+      const int64_t at = static_cast<int64_t>(pair ? mx_pair_row(row) : row) * blocks + b;
+      codes = (second ? up_words : words)[at];
+      scale = (second ? up_scales : scales)[at];
+    }
+    uint8_t* sb = tiled + (row / MX_SB) * sb_bytes;
+    *reinterpret_cast<uint4*>(sb + mx_code_offset(MX_SB, steps, row % MX_SB, b)) = codes;
+    sb[mx_scale_offset(MX_SB, steps, row % MX_SB, b)] = scale;
+    // a last stage with an odd number of steps has scales for one step more, which no MMA reads: they are left zero all the same
+    if (b == padded - 1 && (steps & 1)) {
+      sb[mx_scale_offset(MX_SB, steps, row % MX_SB, b) + 1] = 0;
+      sb[mx_scale_offset(MX_SB, steps, row % MX_SB, b) + 2] = 0;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__ tiled, int n, int blocks, int steps, int64_t sb_bytes,
+                                                     uint4* __restrict__ words, uint8_t* __restrict__ scales) {
+  const int64_t total = static_cast<int64_t>(n) * blocks, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int row = static_cast<int>(i / blocks), b = static_cast<int>(i - static_cast<int64_t>(row) * blocks);
+    const uint8_t* sb = tiled + (row / MX_SB) * sb_bytes;
+    words[i] = *reinterpret_cast<const uint4*>(sb + mx_code_offset(MX_SB, steps, row % MX_SB, b));
+    scales[i] = sb[mx_scale_offset(MX_SB, steps, row % MX_SB, b)];
+  }
+}
+
+// bf16 rows to the operand layout, a warp a segment of 1024 inputs of one row (four loads in flight a lane).  With a plan, row r
+// of item y is row members[first + r] / slots of x (members[first + r] itself with slots 0) and goes to row r of operand y.
+constexpr int ROWS_SEGMENT = 1024;
+__global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int m, int k, int steps, int rows,
+                                                   int segments, int tile, int64_t item_bytes, const int* __restrict__ items,
+                                                   const int* __restrict__ counts, const int* __restrict__ members, int slots, int pairs,
+                                                   uint8_t* __restrict__ out) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  int row = static_cast<int>(w / segments);
+  const int seg = static_cast<int>(w - static_cast<int64_t>(row) * segments);
+  int64_t src = row;
+  if (items != nullptr) {
+    const int y = row / tile;
+    row -= y * tile;
+    if (y >= counts[0] || row >= items[3 * y + 2]) return;
+    const int pos = items[3 * y + 1] + row;
+    if (pos < 0 || pos >= pairs) return;
+    const int pair = members[pos];
+    if (pair < 0 || pair >= pairs) return;
+    src = slots > 0 ? pair / slots : pair;
+    out += y * item_bytes;
+  } else if (row >= m) {
+    return;
+  }
+  const uint4* from = reinterpret_cast<const uint4*>(x + src * ldx);
+  uint4 p[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int piece = seg * (ROWS_SEGMENT / 8) + 32 * j + lane;
+    p[j] = piece * 8 < k ? from[piece] : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int piece = seg * (ROWS_SEGMENT / 8) + 32 * j + lane, b = piece >> 2;
+    float v[8];
+    widen8(p[j], v);
+    uint32_t scale;
+    const uint32_t codes = quantize_block(v, scale);
+    if (b < 2 * steps) {                                     // K ends inside a step: its second block is zeros
+      *reinterpret_cast<uint32_t*>(out + mx_code_offset(rows, steps, row, b) + 4 * (piece & 3)) = codes;
+      if ((piece & 3) == 0) out[mx_scale_offset(rows, steps, row, b)] = static_cast<uint8_t>(scale);
+    }
+  }
+}
+
+int blocks_for(int64_t threads) {
+  const int64_t b = (threads + 255) / 256;
+  return static_cast<int>(b < 1 ? 1 : b > 148 * 64 ? 148 * 64 : b);
+}
+
+bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+}  // namespace
+
+// Rows quantised into operands: the first half of the products.  items null: one operand of `rows` rows.
+cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
+                           const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream) {
+  const int steps = mx_steps(k), segments = (steps * MX_STEP + ROWS_SEGMENT - 1) / ROWS_SEGMENT;
+  const int64_t warps = (items ? static_cast<int64_t>(max_items) * tile : m) * segments;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((warps + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, rows_kernel, static_cast<const __nv_bfloat16*>(x), ldx, m, k, steps, rows, segments, tile, item_bytes, items,
+                            counts, members, slots, pairs, static_cast<uint8_t*>(out));
+}
+
+}  // namespace tf
+
+using namespace tf;
+
+extern "C" {
+
+int64_t tf_mx_tiled_bytes(int n, int k) {
+  if (n < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  return static_cast<int64_t>((n + MX_SB - 1) / MX_SB) * mx_operand_bytes(MX_SB, mx_steps(k));
+}
+
+int tf_mx_quantize(const void* x, int64_t ldx, int dtype, int rows, int k, void* words, void* scales, void* stream) {
+  if (dtype < 0 || dtype > 2 || rows < 1 || k < MX_BLOCK || k % MX_BLOCK || ldx < k || !x || !words || !scales)
+    return fail_moe(TF_ERR_ARG, "tf_mx_quantize: rows of a positive multiple of 32 values, none null");
+  if (misaligned(x, 16) || (rows > 1 && ldx % (dtype == 2 ? 4 : 8)) || misaligned(words, 4))
+    return fail_moe(TF_ERR_ALIGN, "tf_mx_quantize: rows must start on 16-byte boundaries");
+  const int64_t pieces = static_cast<int64_t>(rows) * (k / 8);
+  quantize_kernel<<<blocks_for(pieces), 256, 0, static_cast<cudaStream_t>(stream)>>>(x, ldx, dtype, pieces, k / 8, static_cast<uint32_t*>(words),
+                                                                                     static_cast<uint8_t*>(scales));
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_quantize");
+}
+
+int tf_mx_dequantize(const void* words, const void* scales, int rows, int k, int out_type, void* out, void* stream) {
+  if (out_type < 0 || out_type > 2 || rows < 1 || k < MX_BLOCK || k % MX_BLOCK || !words || !scales || !out)
+    return fail_moe(TF_ERR_ARG, "tf_mx_dequantize: rows of a positive multiple of 32 values, none null");
+  if (misaligned(words, 4) || misaligned(out, 16)) return fail_moe(TF_ERR_ALIGN, "tf_mx_dequantize: out must start on a 16-byte boundary");
+  const int64_t pieces = static_cast<int64_t>(rows) * (k / 8);
+  dequantize_kernel<<<blocks_for(pieces), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(words), static_cast<const uint8_t*>(scales), pieces, out_type, out);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_dequantize");
+}
+
+int tf_mx_pack(const void* words, const void* scales, const void* up_words, const void* up_scales, int experts, int n, int k, void* tiled,
+               void* stream) {
+  const bool pair = up_words != nullptr;
+  if (experts < 1 || experts > 65535 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || !words || !scales || !tiled || pair != (up_scales != nullptr))
+    return fail_moe(TF_ERR_ARG, "tf_mx_pack: rows of a positive multiple of 32 values, none null");
+  if (pair && n % 32) return fail_moe(TF_ERR_ARG, "tf_mx_pack: a pair interleaves whole tiles of 16 rows");
+  if (misaligned(words, 16) || misaligned(up_words, 16) || misaligned(tiled, 16))
+    return fail_moe(TF_ERR_ALIGN, "tf_mx_pack: words and units must start on 16-byte boundaries");
+  const int steps = mx_steps(k);
+  const int64_t total = static_cast<int64_t>((n + MX_SB - 1) / MX_SB) * MX_SB * 2 * steps;
+  const dim3 grid(blocks_for(total), experts);
+  pack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint4*>(words), static_cast<const uint8_t*>(scales), static_cast<const uint4*>(up_words),
+      static_cast<const uint8_t*>(up_scales), n, k / MX_BLOCK, steps, mx_operand_bytes(MX_SB, steps), static_cast<uint8_t*>(tiled));
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_pack");
+}
+
+int tf_mx_unpack(const void* tiled, int n, int k, void* words, void* scales, void* stream) {
+  if (n < 1 || k < MX_BLOCK || k % MX_BLOCK || !words || !scales || !tiled) return fail_moe(TF_ERR_ARG, "tf_mx_unpack: bad shape or null pointer");
+  if (misaligned(words, 16) || misaligned(tiled, 16))
+    return fail_moe(TF_ERR_ALIGN, "tf_mx_unpack: words and units must start on 16-byte boundaries");
+  const int steps = mx_steps(k);
+  unpack_kernel<<<blocks_for(static_cast<int64_t>(n) * (k / MX_BLOCK)), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(tiled), n, k / MX_BLOCK, steps, mx_operand_bytes(MX_SB, steps), static_cast<uint4*>(words),
+      static_cast<uint8_t*>(scales));
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_unpack");
+}
+
+}  // extern "C"

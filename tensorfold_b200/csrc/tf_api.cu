@@ -59,6 +59,7 @@ std::mutex g_init_mutex;
 }  // namespace
 
 cudaError_t prefill_configure(int device);      // qmm_prefill.cu
+cudaError_t mx_configure(int device, int sms);  // mx_matmul.cu
 void peer_reduce_plain(int on);       // peer_reduce.cu
 cudaError_t moe_static_init(int device);   // moe.cu: the built-in plan scratch's address on that device
 int encode_rows(CUtensorMap* map, const void* x, int64_t ldx, int rows, int k, int box_rows);
@@ -312,6 +313,7 @@ int tf_init(int device) {
   if (e == cudaSuccess) e = qmm_window_configure_b6();
   int sms = 0;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess) e = mx_configure(device, sms);
   if (e == cudaSuccess) {
     for (int b = 0; b < 6; ++b)
       for (int g = 0; g < 3; ++g)

@@ -47,6 +47,7 @@ constexpr int MX_QUANT_COLS = 128;                 // columns of the buffer in w
 constexpr int MX_QUANT_ROWS = 16;
 constexpr int MX_QUANT_BYTES = MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;
 constexpr int MX_CLUSTER_MAX = 8;
+constexpr int MX_TILE_MAX = 192;                   // rows of a tile: two accumulators and five slots' scales fill tensor memory
 
 enum MxEpilogue : int { MX_STORE = 0, MX_RELU2 = 1, MX_SWIGLU = 2 };
 
@@ -127,6 +128,13 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, float* v) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "f"(v[0]),
+      "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]),
+      "f"(v[14]), "f"(v[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float v) {
   uint32_t remote;
@@ -140,7 +148,7 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
     g = fminf(g, limit);
     u = fminf(fmaxf(u, -limit), limit);
   }
-  return g / (1.f + expf(-g)) * u;
+  return __fdividef(g, 1.f + expf(-g)) * u;
 }
 
 template <int NT, bool FUSED>
@@ -148,12 +156,11 @@ struct MxShape {
   static constexpr int SBS = (NT + MX_SB - 1) / MX_SB;
   static constexpr int B_BYTES = NT * 128 + SBS * MX_SCALES;
   static constexpr int SLOT = MX_UNIT + (FUSED ? 0 : B_BYTES);
-  static constexpr int ACCS = NT > 128 ? 1 : 2;                    // accumulators in turn
   static constexpr int SF_COLS = 8 + 8 * SBS;                      // scale columns of a slot
   static constexpr int TMEM = FUSED ? 256 : 512;
-  static constexpr int GROUPS = NT > 16 ? 2 : 1;                   // drain groups of four warps, NT / GROUPS columns each
-  static constexpr int COLS = NT / GROUPS;
-  static constexpr int RING = (TMEM - ACCS * NT) / SF_COLS < MX_RING_MAX ? (TMEM - ACCS * NT) / SF_COLS : MX_RING_MAX;
+  static constexpr int GROUPS = NT > 16 ? 2 : 1;                   // drain groups of four warps; they take sixteen rows in turn
+  static constexpr int CHUNKS = (NT / 16 + GROUPS - 1) / GROUPS;   // runs of sixteen rows a group drains
+  static constexpr int RING = (TMEM - 2 * NT) / SF_COLS < MX_RING_MAX ? (TMEM - 2 * NT) / SF_COLS : MX_RING_MAX;
 };
 
 template <int NT, bool FUSED>
@@ -278,8 +285,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     const int64_t stage_bytes = mx_stage_bytes(p.b_rows);
     for (int it = 0; it < my_tiles && ok; ++it) {
       const Tile ti = tile_at(it);
-      const uint8_t* op = p.b + (grouped ? ti.y * p.item_stride : 0);
-      const int r0 = grouped ? 0 : ti.m0, sbs = mx_scale_blocks(ti.n);
+      const uint8_t* op = p.b + ti.y * p.item_stride;
+      const int sbs = mx_scale_blocks(ti.n);
 #pragma unroll 1
       for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
         ok = mbar32_wait(smem_addr(empty + slot), phase, abort_word);
@@ -291,15 +298,15 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         if (elect_lane()) {
           mbar32_expect_tx(bar, ti.n * (whole ? 128 : 32 * tail) + sbs * scales);
           if (whole) {
-            bulk_load32(dst, src + static_cast<int64_t>(r0) * 128, ti.n * 128, bar);
+            bulk_load32(dst, src, ti.n * 128, bar);
             src += static_cast<int64_t>(p.b_rows) * 128;
           } else {
             for (int j = 0; j < tail; ++j) {
-              bulk_load32(dst + j * NT * 32, src + static_cast<int64_t>(r0) * 32, ti.n * 32, bar);
+              bulk_load32(dst + j * NT * 32, src, ti.n * 32, bar);
               src += static_cast<int64_t>(p.b_rows) * 32;
             }
           }
-          bulk_load32(dst + NT * 128, src + (r0 / MX_SB) * scales, sbs * scales, bar);
+          bulk_load32(dst + NT * 128, src, sbs * scales, bar);
         }
         __syncwarp();
         if (++slot == p.ring) slot = 0, phase ^= 1u;
@@ -308,7 +315,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     if (!ok) give_up(ERR_WAIT_EMPTY), let_copies_land();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
-    const uint32_t sf0 = tmem + S::ACCS * NT;
+    const uint32_t sf0 = tmem + 2 * NT;
     bool ok = true;
     int slot = 0, use = 0, op = -1, last_y = -1;
     uint32_t phase = 0;
@@ -327,8 +334,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       }
       const uint32_t id0 = instruction(ti.n, 0), id1 = instruction(ti.n, 1);
       for (int s = slice0; s < slice1 && ok; ++s, ++use) {
-        const int acc = use % S::ACCS, start = slice_at(s), end = slice_at(s + 1);
-        if (use >= S::ACCS) ok = mbar32_wait(smem_addr(acc_empty + acc), (use / S::ACCS - 1) & 1, abort_word);
+        const int acc = use & 1, start = slice_at(s), end = slice_at(s + 1);
+        if (use >= 2) ok = mbar32_wait(smem_addr(acc_empty + acc), ((use >> 1) - 1) & 1, abort_word);
         const uint32_t d = tmem + acc * NT;
 #pragma unroll 1
         for (int u = start; u < end && ok; ++u) {
@@ -392,39 +399,36 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         if (!ok) break;
       }
       uint8_t* base = smem + (operand0 - smem_addr(smem)) + (op % p.bufs) * operand_bytes;
-      const int total = ti.rows * pieces;                            // a multiple of 8
-      for (int i0 = 0; i0 < total; i0 += 4 * qthreads) {
+      // a warp takes segments of 1024 inputs of a row, four 16-byte loads in flight a lane
+      const int segments = (pieces + 127) >> 7;
+      for (int w = qt >> 5; w < ti.rows * segments; w += qthreads >> 5) {
+        const int r = w / segments, q0 = (w - r * segments) * 128 + lane;
+        int64_t row = r;
+        if (grouped) {
+          const int pair = p.members[ti.m0 + r];
+          if (pair < 0 || pair >= p.pairs) continue;
+          row = p.slots > 0 ? pair / p.slots : pair;
+        }
+        const uint4* from = reinterpret_cast<const uint4*>(p.x + row * p.ldx) + p0;
         uint4 v4[4];
-        int rr[4], pp[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int i = i0 + j * qthreads + qt;
-          rr[j] = i / pieces, pp[j] = i - rr[j] * pieces;
-          v4[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (i < total && (p0 + pp[j]) * 8 < p.K) {
-            int64_t row = rr[j];
-            bool live = true;
-            if (grouped) {
-              const int pair = p.members[ti.m0 + rr[j]];
-              live = pair >= 0 && pair < p.pairs;
-              row = p.slots > 0 ? pair / p.slots : pair;
-            }
-            if (live) v4[j] = *(reinterpret_cast<const uint4*>(p.x + row * p.ldx) + p0 + pp[j]);
-          }
+          const int q = q0 + 32 * j;
+          v4[j] = q < pieces && (p0 + q) * 8 < p.K ? from[q] : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          const int q = q0 + 32 * j, b = q >> 2, u = b >> 3;
           float v[8];
           widen8(v4[j], v);
           uint32_t scale;
           const uint32_t codes = quantize_block(v, scale);
-          if (i0 + j * qthreads + qt < total) {
-            const int b = pp[j] >> 2, u = b >> 3, r = rr[j];
+          if (q < pieces) {
             uint8_t* stage = base + u * S::B_BYTES;
             const uint32_t at = u0 + u < full_stages ? (r >> 3) * 1024 + (r & 7) * 128 + (((b & 7) ^ (r & 7)) << 4)
                                                      : ((b & 7) >> 1) * (NT * 32) + (r >> 3) * 256 + (r & 7) * 32 + (((b & 1) ^ ((r >> 2) & 1)) << 4);
-            *reinterpret_cast<uint32_t*>(stage + at + 4 * (pp[j] & 3)) = codes;
-            if ((pp[j] & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + r * 16 + (b & 3)] = static_cast<uint8_t>(scale);
+            *reinterpret_cast<uint32_t*>(stage + at + 4 * (q & 3)) = codes;
+            if ((q & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + r * 16 + (b & 3)] = static_cast<uint8_t>(scale);
           }
         }
       }
@@ -437,122 +441,161 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
 
   const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 unless they quantise)
   const bool drains = warp >= 4 && group < S::GROUPS;
-  const int lg = warp & 3, col0 = group * S::COLS;
-  // acc values of one row of the tile, a lane a column: stored, or two rows (n, n + 1) of SwiGLU, gate in lanes 0-15
+  const int lg = warp & 3;
   const int ncols = p.epi == MX_SWIGLU ? p.N / 2 : p.N;
-  auto store = [&](const Tile& ti, float v, int n, int col) {
-    if (n < ti.rows && col < ncols) {
-      const int64_t row = grouped && p.members != nullptr ? p.members[ti.m0 + n] : ti.m0 + n;
-      if (grouped && (row < 0 || row >= p.pairs)) return;
-      if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + col] = v;
-      else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + col] = __float2bfloat16_rn(v);
+  const bool wide = !p.out_f32 && (ncols & 7) == 0 && (p.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  auto row_of = [&](const Tile& ti, int n) -> int64_t {              // the output row of row n of the tile; below 0: none
+    if (n >= ti.rows) return -1;
+    if (!grouped) return ti.m0 + n;
+    const int pair = p.members[ti.m0 + n];
+    return pair < p.pairs ? pair : -1;
+  };
+  // v[j] = row n + j of the tile in output column `col`, a lane a column
+  auto store8 = [&](const Tile& ti, const float* v, int n, int col) {
+    if (wide) {
+      const float t[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+      const uint4 o = transpose8(t, lane);                           // columns col - l8 .. col - l8 + 7 of row n + l8
+      const int64_t row = row_of(ti, n + (lane & 7));
+      if (row >= 0 && col < ncols) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + (col - (lane & 7))) = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t row = row_of(ti, n + j);
+        if (row < 0 || col >= ncols) continue;
+        if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + col] = v[j];
+        else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + col] = __float2bfloat16_rn(v[j]);
+      }
     }
   };
-  auto finish2 = [&](const Tile& ti, float v0, float v1, int n) {
+  // Activations of sixteen rows.  SwiGLU: gate in lanes 0-15, up in lanes 16-31 of the same outputs; the lower lanes come out with
+  // rows 0-7 in v[0..7], the upper ones with rows 8-15.
+  auto activate = [&](float* v) {
     if (p.epi == MX_SWIGLU) {
       const bool low = lane < 16;
-      const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v1 : v0, 16);
-      const float a = swiglu(low ? v0 : got, low ? got : v1, p.limit);
-      store(ti, a, n + (low ? 0 : 1), ti.cb * 64 + lg * 16 + (lane & 15));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v[8 + j] : v[j], 16);
+        v[j] = swiglu(low ? v[j] : got, low ? got : v[8 + j], p.limit);
+      }
+    } else if (p.epi == MX_RELU2) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float u = fmaxf(v[j], 0.f);
+        v[j] = u * u;
+      }
+    }
+  };
+  auto finish16 = [&](const Tile& ti, float* v, int n) {
+    activate(v);
+    if (p.epi == MX_SWIGLU) {
+      store8(ti, v, n + (lane < 16 ? 0 : 8), ti.cb * 64 + lg * 16 + (lane & 15));
     } else {
-      if (p.epi == MX_RELU2) v0 = fmaxf(v0, 0.f), v1 = fmaxf(v1, 0.f), v0 *= v0, v1 *= v1;
-      store(ti, v0, n, ti.cb * MX_SB + lg * 32 + lane);
-      store(ti, v1, n + 1, ti.cb * MX_SB + lg * 32 + lane);
+      const int col = ti.cb * MX_SB + lg * 32 + lane;
+      store8(ti, v, n, col);
+      if (n + 8 < ti.rows) store8(ti, v + 8, n + 8, col);
+    }
+  };
+  // The same, quantised: through shared memory, where four lanes see a block.
+  auto quantize16 = [&](const Tile& ti, float* v, int n) {
+    constexpr int LINE = MX_QUANT_COLS + 4;
+    const int width = p.epi == MX_SWIGLU ? 64 : 128;
+    float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES);
+    uint8_t* op = p.q + ti.y * p.q_item_stride;
+    activate(v);
+    named_barrier(1 + group, 128);                                   // the last sixteen rows have been read
+    if (p.epi == MX_SWIGLU) {
+      float* to = rows + (lane < 16 ? 0 : 8) * LINE + lg * 16 + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j * LINE] = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) rows[j * LINE + lg * 32 + lane] = v[j];
+    }
+    named_barrier(1 + group, 128);
+    for (int t = lg * 32 + lane; t < MX_QUANT_ROWS * width / 8; t += 128) {
+      const int r = t / (width / 8), piece = t - r * (width / 8);
+      const float4* from = reinterpret_cast<const float4*>(rows + r * LINE + piece * 8);
+      const float4 lo = from[0], hi = from[1];
+      float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      uint32_t scale;
+      const uint32_t codes = quantize_block(w, scale);
+      const int b = ti.cb * (width / 32) + (piece >> 2);
+      if (n + r < ti.rows && b < 2 * p.q_steps) {
+        *reinterpret_cast<uint32_t*>(op + mx_code_offset(p.q_rows, p.q_steps, n + r, b) + 4 * (piece & 3)) = codes;
+        if ((piece & 3) == 0) op[mx_scale_offset(p.q_rows, p.q_steps, n + r, b)] = static_cast<uint8_t>(scale);
+      }
     }
   };
 
   if (drains) {
     // ------------------------------------------------------------------ drain
+    // Sixteen rows at a time straight from tensor memory.  The loop is not unrolled and its body is kept small: unrolled over
+    // a tile (5900 instructions) the warps mostly waited for instructions, and a tile of 256 rows took 42 us.
     pdl_wait();                                                      // nothing is written before the previous kernel is done
     bool ok = true;
     int use = 0;
-    const uint32_t my_tmem = tmem + (static_cast<uint32_t>(lg * 32) << 16) + col0;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(lg * 32) << 16) + 16 * group;
     for (int it = 0; it < my_tiles && ok; ++it) {
       const Tile ti = tile_at(it);
-      float acc[S::COLS];
-      for (int s = slice0; s < slice1 && ok; ++s, ++use) {
-        const int ab = use % S::ACCS;
-        ok = mbar32_wait(smem_addr(acc_full + ab), (use / S::ACCS) & 1, abort_word);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t src = my_tmem + ab * NT;
-        if (s == slice0) {
+      if (slice1 - slice0 > 1) {
+        // slices are added in registers, and the sum goes back to where the last one came from
+        float acc[S::CHUNKS][16];
+        for (int s = slice0; s < slice1; ++s, ++use) {
+          ok = mbar32_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t src = lanes + (use & 1) * NT;
 #pragma unroll
-          for (int i = 0; i < S::COLS; i += 16)
-            if (col0 + i < ti.n) tmem_load16(src + i, acc + i);
-          tmem_loaded();
-        } else {
+          for (int i = 0; i < S::CHUNKS; ++i) {
+            if (16 * (S::GROUPS * i + group) >= ti.rows) break;
+            float v[16];
+            tmem_load16(src + 16 * S::GROUPS * i, v);
+            tmem_loaded();
 #pragma unroll
-          for (int i = 0; i < S::COLS; i += 16) {
-            if (col0 + i < ti.n) {
-              float v[16];
-              tmem_load16(src + i, v);
-              tmem_loaded();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) acc[i + j] = acc[i + j] + v[j];
-            }
+            for (int j = 0; j < 16; ++j) acc[i][j] = s == slice0 ? v[j] : acc[i][j] + v[j];
+            if (s + 1 == slice1) tmem_store16(src + 16 * S::GROUPS * i, acc[i]);
           }
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + ab);
-      }
-      if (!ok) break;
-      if (c > 1) {
-        // part [slice][row of the owner][128 columns] in the shared memory of the block that owns the row
-        const int share = (ti.n + c - 1) / c;
-        const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 4;
-#pragma unroll
-        for (int i = 0; i < S::COLS; ++i) {
-          const int n = col0 + i;
-          if (n < ti.n) {
-            const int owner = n / share;
-            store_remote(part + (rank * share + n - owner * share) * (MX_SB * 4), owner, acc[i]);
+          if (s + 1 == slice1) {
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            break;                                                   // (the loop below ends this use of the accumulator)
           }
-        }
-      } else if (p.q != nullptr) {
-        // rows of activations, sixteen at a time through shared memory, where four lanes see a block
-        const int width = p.epi == MX_SWIGLU ? 64 : 128;
-        float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES);
-        uint8_t* op = p.q + ti.y * p.q_item_stride;
-        const int gt = (lg << 5) | lane;
-#pragma unroll
-        for (int i = 0; i < S::COLS; i += MX_QUANT_ROWS) {
-          if (col0 + i >= ti.rows) break;
-          named_barrier(1 + group, 128);                             // the last sixteen rows have been read
-#pragma unroll
-          for (int j = 0; j < MX_QUANT_ROWS; j += 2) {
-            float v0 = acc[i + j], v1 = acc[i + j + 1];
-            if (p.epi == MX_SWIGLU) {
-              const bool low = lane < 16;
-              const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v1 : v0, 16);
-              rows[(j + (low ? 0 : 1)) * (MX_QUANT_COLS + 4) + lg * 16 + (lane & 15)] = swiglu(low ? v0 : got, low ? got : v1, p.limit);
-            } else {
-              if (p.epi == MX_RELU2) v0 = fmaxf(v0, 0.f), v1 = fmaxf(v1, 0.f), v0 *= v0, v1 *= v1;
-              rows[j * (MX_QUANT_COLS + 4) + lg * 32 + lane] = v0;
-              rows[(j + 1) * (MX_QUANT_COLS + 4) + lg * 32 + lane] = v1;
-            }
-          }
-          named_barrier(1 + group, 128);
-          for (int t = gt; t < MX_QUANT_ROWS * width / 8; t += 128) {
-            const int r = t / (width / 8), piece = t - r * (width / 8), n = col0 + i + r;
-            const float4* from = reinterpret_cast<const float4*>(rows + r * (MX_QUANT_COLS + 4) + piece * 8);
-            const float4 lo = from[0], hi = from[1];
-            float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-            uint32_t scale;
-            const uint32_t codes = quantize_block(v, scale);
-            const int b = ti.cb * (width / 32) + (piece >> 2);
-            if (n < ti.rows && b < 2 * p.q_steps) {
-              *reinterpret_cast<uint32_t*>(op + mx_code_offset(p.q_rows, p.q_steps, n, b) + 4 * (piece & 3)) = codes;
-              if ((piece & 3) == 0) op[mx_scale_offset(p.q_rows, p.q_steps, n, b)] = static_cast<uint8_t>(scale);
-            }
-          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + (use & 1));
         }
       } else {
-#pragma unroll
-        for (int i = 0; i < S::COLS; i += 2)
-          if (col0 + i < ti.rows) finish2(ti, acc[i], acc[i + 1], col0 + i);
+        ok = mbar32_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
+      if (!ok) break;
+      const uint32_t src = lanes + (use & 1) * NT;
+#pragma unroll 1
+      for (int i = 0; i < S::CHUNKS; ++i) {
+        const int n = 16 * (S::GROUPS * i + group);
+        if (n >= ti.rows) break;
+        float v[16];
+        tmem_load16(src + 16 * S::GROUPS * i, v);
+        tmem_loaded();
+        if (c > 1) {
+          // part [slice][row of the owner][128 columns] in the shared memory of the block that owns the row
+          const int share = (ti.n + c - 1) / c;
+          const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 4;
+          int owner = n / share, at = n - owner * share;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (n + j < ti.rows) store_remote(part + (rank * share + at) * (MX_SB * 4), owner, v[j]);
+            if (++at == share) at = 0, ++owner;
+          }
+        } else if (p.q != nullptr) {
+          quantize16(ti, v, n);
+        } else {
+          finish16(ti, v, n);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + (use & 1));
+      ++use;
     }
     if (!ok) give_up(ERR_WAIT_FULL);
   }
@@ -563,18 +606,23 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     __syncwarp();
     cluster_barrier();
     if (drains && my_tiles > 0 && *abort_flag == 0) {
-      const Tile ti = tile_at(0);
+      Tile ti = tile_at(0);
       const int share = (ti.n + c - 1) / c, n0 = rank * share;
+      ti.rows = min(ti.rows, n0 + share);
       const float* part = reinterpret_cast<const float*>(smem + extra_off) + lg * 32 + lane;
-      for (int i = 2 * group; i < share; i += 2 * S::GROUPS) {
-        float v0 = 0.f, v1 = 0.f;
+#pragma unroll 1
+      for (int i = 16 * group; n0 + i < ti.rows; i += 16 * S::GROUPS) {
+        float v[16] = {};
+#pragma unroll 1
         for (int s = 0; s < c; ++s) {
-          const float a = part[(s * share + i) * MX_SB], b = i + 1 < share ? part[(s * share + i + 1) * MX_SB] : 0.f;
-          v0 = s == 0 ? a : v0 + a, v1 = s == 0 ? b : v1 + b;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (n0 + i + j >= ti.rows) break;
+            const float a = part[(s * share + i + j) * MX_SB];
+            v[j] = s == 0 ? a : v[j] + a;
+          }
         }
-        Tile own = ti;
-        own.rows = min(ti.rows, n0 + share);                         // row i + 1 may be the next block's
-        finish2(own, v0, v1, n0 + i);
+        finish16(ti, v, n0 + i);
       }
     }
   }
@@ -643,18 +691,40 @@ cudaError_t configure() {
   return cudaFuncSetAttribute(mx_kernel<NT, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
 }
 
-// The tile of a call of m rows whose rows come as operands.
-cudaError_t launch_rows(MxParams& p, int nt, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
-  p.tile = std::min(p.tile, nt);
-  switch (nt) {
-    case 16: return launch<16, false>(p, tiles, quant_out, sms, pdl, stream);
-    case 64: return launch<64, false>(p, tiles, quant_out, sms, pdl, stream);
-    case 128: return launch<128, false>(p, tiles, quant_out, sms, pdl, stream);
-    default: return launch<256, false>(p, tiles, quant_out, sms, pdl, stream);
-  }
+// Rows come as operands: the kernel whose tiles hold `tile` rows.
+cudaError_t launch_rows(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
+  if (p.tile <= 16) return launch<16, false>(p, tiles, quant_out, sms, pdl, stream);
+  if (p.tile <= 64) return launch<64, false>(p, tiles, quant_out, sms, pdl, stream);
+  if (p.tile <= 128) return launch<128, false>(p, tiles, quant_out, sms, pdl, stream);
+  return launch<192, false>(p, tiles, quant_out, sms, pdl, stream);
 }
 
-int rows_padded(int m) { return m > MX_SB ? (m + MX_SB - 1) / MX_SB * MX_SB : (m + 7) / 8 * 8; }
+int round8(int m) { return (m + 7) / 8 * 8; }
+
+// Rows of a tile of an m-row call, and blocks that share a tile (all K slices or one): the fewest cycles by a plain model.  A stage
+// takes 2 cycles a row of math, but no less than its copies (17 KB and 136 bytes a row, at COPY bytes a cycle); a tile has a start
+// and an end besides.
+struct Tiling {
+  int tile, cluster;
+};
+Tiling tiling_for(int m, int n, int stages, int sk) {
+  constexpr int SMS = 148, COPY = 48, ENDS = 1500;
+  const int64_t ncb = (n + MX_SB - 1) / MX_SB;
+  Tiling best = {8, 1};
+  double cost = 1e30;
+  for (int t = 8; t <= MX_TILE_MAX; t += 8) {
+    const int64_t tiles = ncb * ((m + t - 1) / t);
+    for (int c = 1; c <= sk; c += sk > 1 ? sk - 1 : 1) {
+      if (c > 1 && t > MX_SB) continue;                              // (no room for the exchange beside the ring)
+      const int64_t waves = (tiles * c + SMS - 1) / SMS;
+      const double stage = std::max(2.0 * t, (MX_UNIT + 136.0 * t) / COPY);
+      const double here = waves * (stages / static_cast<double>(c) * stage + ENDS + (c > 1 ? ENDS : 0));
+      if (here <= cost) cost = here, best = {t, c};
+    }
+    if (t >= m) break;
+  }
+  return best;
+}
 
 // Whether a block can hold its K slice of sixteen quantised rows beside a ring of four slots.
 bool fused_fits(int k, int sk) {
@@ -671,7 +741,7 @@ cudaError_t mx_configure(int device, int sms) {
   if (e == cudaSuccess) e = configure<16, false>();
   if (e == cudaSuccess) e = configure<64, false>();
   if (e == cudaSuccess) e = configure<128, false>();
-  if (e == cudaSuccess) e = configure<256, false>();
+  if (e == cudaSuccess) e = configure<192, false>();
   if (e == cudaSuccess && device >= 0 && device < 64) g_mx_sms[device] = sms;
   return e;
 }
@@ -687,7 +757,8 @@ int tf_mx_split(int n, int k) { return n < 1 || k < MX_BLOCK || k % MX_BLOCK ? T
 int64_t tf_mx_matmul_bytes(int m, int n, int k) {
   if (m < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
   if (m <= MX_FUSED_ROWS && fused_fits(k, slices_for(n, k))) return 0;
-  return mx_operand_bytes(rows_padded(m), mx_steps(k));
+  const int steps = mx_steps(k), tile = tiling_for(m, n, mx_stages(steps), slices_for(n, k)).tile;
+  return (m + tile - 1) / tile * mx_operand_bytes(tile, steps);
 }
 
 int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
@@ -722,29 +793,27 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     p.operand_stages = (p.stages + p.sk - 1) / p.sk;
     e = launch<16, true>(p, ncb, false, sms, pdl != 0, s);
   } else {
-    const int rows = rows_padded(m);
-    e = mx_rows_launch(x, ldx, m, k, rows, 0, 0, nullptr, nullptr, nullptr, 0, 0, 0, work, pdl != 0, s);
-    if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
-    p.b = static_cast<const uint8_t*>(work), p.b_rows = rows;
-    const int nt = m <= 16 ? 16 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
-    p.tile = nt;
-    const int64_t row_tiles = (m + nt - 1) / nt;
+    const Tiling t = tiling_for(m, n, p.stages, p.sk);
+    p.tile = p.b_rows = t.tile, p.cluster = t.cluster;
+    p.b = static_cast<const uint8_t*>(work), p.item_stride = mx_operand_bytes(t.tile, p.steps);
+    const int64_t row_tiles = (m + t.tile - 1) / t.tile;
     if (ncb * row_tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: too many tiles");
-    p.cluster = nt <= 128 ? p.sk : 1;
+    e = mx_rows_launch(x, ldx, m, k, t.tile, t.tile, p.item_stride, nullptr, nullptr, nullptr, 0, 0, 0, work, pdl != 0, s);
+    if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
     // the rows' kernel lets this one set up and fetch weights while it runs; the weights were settled before it started
-    e = launch_rows(p, nt, ncb * row_tiles, false, sms, true, s);
+    e = launch_rows(p, ncb * row_tiles, false, sms, true, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_matmul");
 }
 
 int64_t tf_mx_operand_bytes(int rows, int k) {
   if (rows < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
-  return mx_operand_bytes(rows_padded(rows), mx_steps(k));
+  return mx_operand_bytes(round8(rows), mx_steps(k));
 }
 
 int64_t tf_mx_experts_bytes(int k, int tile, int max_items) {
   if (tile < 8 || tile > MX_SB || max_items < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
-  return tile <= MX_FUSED_ROWS && fused_fits(k, 1) ? 0 : max_items * mx_operand_bytes(rows_padded(tile), mx_steps(k));
+  return tile <= MX_FUSED_ROWS && fused_fits(k, 1) ? 0 : max_items * mx_operand_bytes(round8(tile), mx_steps(k));
 }
 
 int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
@@ -762,7 +831,7 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
   if (x && (ldx < k || misaligned(x, 16) || ldx % 8)) return fail_moe(TF_ERR_ALIGN, "tf_mx_experts: x rows must start on 16-byte boundaries");
   if (misaligned(tiled, 16) || expert_stride % 16 || misaligned(work, 16) || misaligned(out_operands, 16) || misaligned(out, out_f32 ? 4 : 2))
     return fail_moe(TF_ERR_ALIGN, "tf_mx_experts: weights, work and operands must start on 16-byte boundaries");
-  const int rows = rows_padded(tile);
+  const int rows = round8(tile);
   const int64_t operand = mx_operand_bytes(rows, mx_steps(k)), need = x ? tf_mx_experts_bytes(k, tile, max_items) : max_items * operand;
   if (need > 0 && (!work || work_bytes < need)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: work is too small");
   int* err = device_error_word();
@@ -797,7 +866,7 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
     }
     p.b = static_cast<const uint8_t*>(work), p.b_rows = rows, p.item_stride = operand;
     p.bufs = 1;
-    e = launch_rows(p, tile <= 16 ? 16 : tile <= 64 ? 64 : 128, tiles, out_operands != nullptr, sms, x != nullptr, s);
+    e = launch_rows(p, tiles, out_operands != nullptr, sms, x != nullptr, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_experts");
 }

@@ -135,8 +135,9 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__
   }
 }
 
-// bf16 rows to the operand layout, a warp a segment of 1024 inputs of one row (four loads in flight a lane).  With a plan, row r
-// of item y is row members[first + r] / slots of x (members[first + r] itself with slots 0) and goes to row r of operand y.
+// bf16 rows to the operand layout, an operand a tile of rows, a warp a segment of 1024 inputs of one row (four loads in flight a
+// lane).  With a plan, row r of item y is row members[first + r] / slots of x (members[first + r] itself with slots 0) and goes to
+// row r of operand y.
 constexpr int ROWS_SEGMENT = 1024;
 __global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int m, int k, int steps, int rows,
                                                    int segments, int tile, int64_t item_bytes, const int* __restrict__ items,
@@ -149,17 +150,17 @@ __global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restri
   int row = static_cast<int>(w / segments);
   const int seg = static_cast<int>(w - static_cast<int64_t>(row) * segments);
   int64_t src = row;
+  const int y = row / tile;
+  row -= y * tile;
+  out += y * item_bytes;
   if (items != nullptr) {
-    const int y = row / tile;
-    row -= y * tile;
     if (y >= counts[0] || row >= items[3 * y + 2]) return;
     const int pos = items[3 * y + 1] + row;
     if (pos < 0 || pos >= pairs) return;
     const int pair = members[pos];
     if (pair < 0 || pair >= pairs) return;
     src = slots > 0 ? pair / slots : pair;
-    out += y * item_bytes;
-  } else if (row >= m) {
+  } else if (src >= m) {
     return;
   }
   const uint4* from = reinterpret_cast<const uint4*>(x + src * ldx);
@@ -192,7 +193,8 @@ bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 
 }  // namespace
 
-// Rows quantised into operands: the first half of the products.  items null: one operand of `rows` rows.
+// Rows quantised into operands of `rows` rows, `tile` of them used, item_bytes apart: the first half of the products.  items null:
+// the m rows in order.
 cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
                            const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream) {
   const int steps = mx_steps(k), segments = (steps * MX_STEP + ROWS_SEGMENT - 1) / ROWS_SEGMENT;

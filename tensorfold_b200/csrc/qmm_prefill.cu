@@ -193,38 +193,6 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[2][8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// Eight lanes each hold eight rows of one column; afterwards each holds eight columns of one row, as bf16: lane l of the
-// group gets row l.  Rows are rounded and paired first, so three exchanges of two words do it.
-__device__ __forceinline__ uint4 transpose8(const float (&v)[8], int lane) {
-  uint32_t p[4];                                             // rows 2 i, 2 i + 1 of this lane's column
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    p[i] = *reinterpret_cast<const uint32_t*>(&t);
-  }
-  // neighbouring columns: an even lane keeps rows 2 i of both, an odd lane rows 2 i + 1
-  const bool odd = lane & 1;
-#pragma unroll
-  for (int i = 0; i < 4; i += 2) {
-    const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, __byte_perm(p[i], p[i + 1], odd ? 0x5410 : 0x7632), 1);
-    p[i] = odd ? __byte_perm(got, p[i], 0x7610) : __byte_perm(p[i], got, 0x5410);
-    p[i + 1] = odd ? __byte_perm(got, p[i + 1], 0x7632) : __byte_perm(p[i + 1], got, 0x7610);
-  }
-  // then a 4 x 4 transpose of (column pair, row pair) words over the other two lane bits
-#pragma unroll
-  for (int bit = 1; bit <= 2; bit <<= 1) {
-    const bool upper = lane & (2 * bit);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i & bit) continue;
-      const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, upper ? p[i] : p[i | bit], 2 * bit);
-      if (upper) p[i] = got;
-      else p[i | bit] = got;
-    }
-  }
-  return make_uint4(p[0], p[1], p[2], p[3]);
-}
-
 template <int GS>
 __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_constant__ CUtensorMap tmx, const PrefillParams p) {
   constexpr int S = GS / 16;                                 // k16 steps a group

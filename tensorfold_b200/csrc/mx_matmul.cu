@@ -142,11 +142,11 @@ __device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
-// silu(gate) * up in fp32, clipped first where limit > 0.
+// silu(gate) * up in fp32, clipped first where limit > 0.  Comparisons, not fminf: a NaN goes through.
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
   if (limit > 0.f) {
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = g > limit ? limit : g;
+    u = u > limit ? limit : u < -limit ? -limit : u;
   }
   return __fdividef(g, 1.f + expf(-g)) * u;
 }
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     } else if (p.epi == MX_RELU2) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float u = fmaxf(v[j], 0.f);
+        const float u = v[j] < 0.f ? 0.f : v[j];
         v[j] = u * u;
       }
     }

@@ -9,7 +9,8 @@ import torch
 
 from .. import _lib
 from . import experts as grouped
-from .kernels import qmm
+from . import mx_experts
+from .kernels import mx, qmm
 
 
 def router(x: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None, *, prefill: bool = False) -> torch.Tensor:
@@ -79,27 +80,34 @@ def select(logits: torch.Tensor, buf: MoEBuffers, top_k: int, experts: int) -> N
 @dataclass
 class SharedExpert:
     """A shared expert of its own width, run as dense projections: ``up`` is a ``qmm.pack_pair`` weight (gate and up
-    interleaved), ``down`` a ``qmm.pack`` weight.  (The reference appends the shared expert to the routed table, which
-    needs equal widths: families/qwen3_5_moe/cuda/weights.py:41-45.)"""
+    interleaved), ``down`` a ``qmm.pack`` weight, or both their ``mx`` counterparts.  (The reference appends the shared expert
+    to the routed table, which needs equal widths: families/qwen3_5_moe/cuda/weights.py:41-45.)"""
 
-    up: qmm.Q4
-    down: qmm.Q4
+    up: qmm.Q4 | mx.MX4
+    down: qmm.Q4 | mx.MX4
     limit: float = 0.0
 
 
-def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts, buf: MoEBuffers, top_k: int,
+def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts | mx_experts.Experts, buf: MoEBuffers, top_k: int,
         experts: int, shared: SharedExpert | None = None) -> MoEBuffers:
-    """Route x [R, D] and run its experts into buf.y [R, k + 1, D] (bf16 in prefill); slot k is the shared expert."""
+    """Route x [R, D] and run its experts into buf.y [R, k + 1, D] (bf16 in prefill); slot k is the shared expert.  The experts
+    are affine (``experts.make``) or microscaled (``mx_experts.make``)."""
 
     rows = x.shape[0]
 
     def routed() -> None:
         router(x, router_rows, buf.logits[:rows], prefill=buf.plan.prefill)
         select(buf.logits[:rows], buf, top_k, experts)
-        grouped.layer(x, ex, buf.plan, buf.act.view(-1, ex.width), buf.y.view(-1, ex.dims), rows)
+        if isinstance(ex, mx_experts.Experts):
+            mx_experts.layer(x, ex, buf.plan, buf.y.view(-1, ex.dims), rows)
+        else:
+            grouped.layer(x, ex, buf.plan, buf.act.view(-1, ex.width), buf.y.view(-1, ex.dims), rows)
 
     def dense() -> None:
-        if buf.plan.prefill:                                    # prefill arithmetic for the dense shared expert too
+        if isinstance(shared.up, mx.MX4):
+            act = mx.matmul_act(x, shared.up, act="swiglu", limit=shared.limit)
+            mx.matmul(act, shared.down, f32=buf.y.dtype == torch.float32, out=buf.y[:rows, top_k])
+        elif buf.plan.prefill:                                    # prefill arithmetic for the dense shared expert too
             act = qmm.matmul_act(x, shared.up, act="swiglu", limit=shared.limit, prefill=True)
             qmm.prefill_matmul(act, shared.down, f32=buf.y.dtype == torch.float32, out=buf.y[:rows, top_k])
         else:
@@ -139,7 +147,7 @@ class Routed:
     (shared expert appended), or E entries plus a dense ``shared`` expert of another width."""
 
     router: torch.Tensor
-    experts: grouped.Experts
+    experts: grouped.Experts | mx_experts.Experts
     top_k: int
     shared: SharedExpert | None = None
 

@@ -102,8 +102,8 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
       : "memory");
 }
 // 32 lines of 16 bytes to four columns, the same in each of the four lane groups.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc(smem, 128, SWIZZLE_NONE)) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t from) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(from) : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -112,6 +112,24 @@ __device__ __forceinline__ bool elect_lane() {
   uint32_t one;
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
   return one != 0;
+}
+// Bounded wait by a whole warp.  The polling loop stays out of line: the roles share the instruction caches.
+__device__ __noinline__ bool poll(uint32_t bar, uint32_t parity, uint32_t abort_word) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < WAIT_POLLS; ++i) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity), "r"(20000u)
+                 : "memory");
+    if (done) return true;
+    if ((i & 255u) == 255u && lds32(abort_word)) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t abort_word) {
+  if (__all_sync(0xFFFFFFFFu, mbar32_try_wait(bar, parity))) return true;
+  return __all_sync(0xFFFFFFFFu, poll(bar, parity, abort_word));
 }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -136,11 +154,14 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const float* v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, float v) {
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, const float* v) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
 }
+
+// Fours of rows each of the c blocks of a cluster owns when they add their slices.
+__host__ __device__ __forceinline__ int quads_of(int rows, int c) { return ((rows + 3) / 4 + c - 1) / c; }
 
 // silu(gate) * up in fp32, clipped first where limit > 0.  Comparisons, not fminf: a NaN goes through.
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
@@ -264,7 +285,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       const Tile ti = tile_at(it);
 #pragma unroll 1
       for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
-        ok = mbar32_wait(smem_addr(empty + slot), phase, abort_word);
+        ok = warp_wait(smem_addr(empty + slot), phase, abort_word);
         if (!ok) break;
         const uint32_t bytes = u < full_stages ? MX_UNIT : tail * 4096 + mx_tail_scales(tail);
         if (elect_lane()) {
@@ -289,7 +310,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       const int sbs = mx_scale_blocks(ti.n);
 #pragma unroll 1
       for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
-        ok = mbar32_wait(smem_addr(empty + slot), phase, abort_word);
+        ok = warp_wait(smem_addr(empty + slot), phase, abort_word);
         if (!ok) break;
         const bool whole = u < full_stages;
         const uint32_t bar = smem_addr(full + slot), dst = ring0 + slot * S::SLOT + MX_UNIT;
@@ -315,66 +336,86 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     if (!ok) give_up(ERR_WAIT_EMPTY), let_copies_land();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
+    // The loop over whole stages is kept to adds on descriptors that are the same in every lane: with descriptors built in
+    // place and the last stage's form beside it in one body, a stage cost 700 cycles of issue at 16 rows.
+    const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty), acc_full32 = smem_addr(acc_full);
     const uint32_t sf0 = tmem + 2 * NT;
+    const uint64_t a0 = desc(ring0, 1024, SWIZZLE_128), as0 = desc(ring0 + MX_SB * 128, 128, SWIZZLE_NONE);
+    const uint64_t b0 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 1024, SWIZZLE_128);
+    const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + NT * 128, 128, SWIZZLE_NONE);
     bool ok = true;
     int slot = 0, use = 0, op = -1, last_y = -1;
     uint32_t phase = 0;
     for (int it = 0; it < my_tiles && ok; ++it) {
       const Tile ti = tile_at(it);
-      bool new_op = false, last_of_op = false;
+      bool last_of_op = false;
       if (FUSED) {
-        new_op = grouped ? ti.y != last_y : it == 0;
+        const bool new_op = grouped ? ti.y != last_y : it == 0;
         last_y = ti.y;
         if (new_op) {
           ++op;
-          ok = mbar32_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word);
+          ok = warp_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word);
           if (!ok) break;
         }
         last_of_op = grouped && (it + 1 == my_tiles || (first_tile + it + 1) / ncb != ti.y);
       }
-      const uint32_t id0 = instruction(ti.n, 0), id1 = instruction(ti.n, 1);
+      const uint32_t n8 = __shfl_sync(0xFFFFFFFFu, static_cast<uint32_t>(ti.n), 0);
+      const uint32_t id0 = instruction(n8, 0), id1 = instruction(n8, 1);
       for (int s = slice0; s < slice1 && ok; ++s, ++use) {
-        const int acc = use & 1, start = slice_at(s), end = slice_at(s + 1);
-        if (use >= 2) ok = mbar32_wait(smem_addr(acc_empty + acc), ((use >> 1) - 1) & 1, abort_word);
-        const uint32_t d = tmem + acc * NT;
+        const int start = slice_at(s), end = slice_at(s + 1), last_whole = min(end, full_stages);
+        if (use >= 2) ok = warp_wait(smem_addr(acc_empty + (use & 1)), ((use >> 1) - 1) & 1, abort_word);
+        const uint32_t d = tmem + (use & 1) * NT;
+        uint32_t more = 0;                                           // 0: the first step of the slice overwrites the accumulator
+        uint32_t fused_at = FUSED ? (op % p.bufs) * (operand_bytes >> 4) : 0;
 #pragma unroll 1
-        for (int u = start; u < end && ok; ++u) {
-          ok = mbar32_wait(smem_addr(full + slot), phase, abort_word);
-          if (!ok) break;
+        for (int u = start; u < last_whole && ok; ++u) {
+          ok = warp_wait(full32 + 8 * slot, phase, abort_word);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const bool whole = u < full_stages;
-          const int steps = whole ? 4 : tail;
-          const uint32_t a = ring0 + slot * S::SLOT;
-          const uint32_t b = FUSED ? operand0 + (op % p.bufs) * operand_bytes + (u - start) * S::B_BYTES : a + MX_UNIT;
-          const uint32_t a_scales = a + (whole ? MX_SB * 128 : tail * 4096), b_scales = b + NT * 128;
-          const uint32_t sb_bytes = whole || FUSED ? MX_SCALES : mx_tail_scales(tail);
-          const uint32_t sa = sf0 + slot * S::SF_COLS, sb = sa + 8;
-          if (elect_lane()) {
+          const uint32_t at = slot * (S::SLOT >> 4), bt = FUSED ? fused_at : at, sa = sf0 + slot * S::SF_COLS, sb = sa + 8;
+          if (ok && elect_lane()) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (2 * h >= steps) break;
-              copy_scales(sa + 4 * h, a_scales + 512 * h);
+              copy_scales(sa + 4 * h, as0 + at + 32 * h);
 #pragma unroll
-              for (int q = 0; q < S::SBS; ++q) copy_scales(sb + 4 * S::SBS * h + 4 * q, b_scales + q * sb_bytes + 512 * h);
+              for (int q = 0; q < S::SBS; ++q) copy_scales(sb + 4 * S::SBS * h + 4 * q, bs0 + bt + (MX_SCALES >> 4) * q + 32 * h);
             }
-            const uint64_t ad = whole ? desc(a, 1024, SWIZZLE_128) : desc(a, 256, SWIZZLE_32);
-            const uint64_t bd = whole ? desc(b, 1024, SWIZZLE_128) : desc(b, 256, SWIZZLE_32);
-            const uint32_t a_step = whole ? 2 : 4096 >> 4, b_step = whole ? 2 : NT * 32 >> 4;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (j >= steps) break;
-              mma_mxf4(d, ad + j * a_step, bd + j * b_step, j & 1 ? id1 : id0, sa + 4 * (j >> 1), sb + 4 * S::SBS * (j >> 1),
-                       u > start || j > 0);
+            mma_mxf4(d, a0 + at, b0 + bt, id0, sa, sb, more);
+            mma_mxf4(d, a0 + at + 2, b0 + bt + 2, id1, sa, sb, 1u);
+            mma_mxf4(d, a0 + at + 4, b0 + bt + 4, id0, sa + 4, sb + 4 * S::SBS, 1u);
+            mma_mxf4(d, a0 + at + 6, b0 + bt + 6, id1, sa + 4, sb + 4 * S::SBS, 1u);
+            commit(empty32 + 8 * slot);
+          }
+          __syncwarp();
+          more = 1;
+          if (FUSED) fused_at += S::B_BYTES >> 4;
+          if (++slot == p.ring) slot = 0, phase ^= 1u;
+        }
+        if (end > full_stages && ok) {                               // the last stage: `tail` steps, each a region of its own
+          ok = warp_wait(full32 + 8 * slot, phase, abort_word);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t a = ring0 + slot * S::SLOT, b = FUSED ? operand0 + fused_at * 16 : a + MX_UNIT;
+          const uint32_t sb_bytes = FUSED ? MX_SCALES : mx_tail_scales(tail), sa = sf0 + slot * S::SF_COLS, sb = sa + 8;
+          if (ok && elect_lane()) {
+#pragma unroll 1
+            for (int h = 0; 2 * h < tail; ++h) {
+              copy_scales(sa + 4 * h, desc(a + tail * 4096 + 512 * h, 128, SWIZZLE_NONE));
+              for (int q = 0; q < S::SBS; ++q)
+                copy_scales(sb + 4 * S::SBS * h + 4 * q, desc(b + NT * 128 + q * sb_bytes + 512 * h, 128, SWIZZLE_NONE));
             }
-            commit(smem_addr(empty + slot));
-            if (u + 1 == end) {
-              commit(smem_addr(acc_full + acc));
-              if (FUSED && last_of_op) commit(smem_addr(op_empty + op % p.bufs));
-            }
+#pragma unroll 1
+            for (int j = 0; j < tail; ++j)
+              mma_mxf4(d, desc(a + j * 4096, 256, SWIZZLE_32), desc(b + j * NT * 32, 256, SWIZZLE_32), j & 1 ? id1 : id0, sa + 4 * (j >> 1),
+                       sb + 4 * S::SBS * (j >> 1), more | (j > 0));
+            commit(empty32 + 8 * slot);
           }
           __syncwarp();
           if (++slot == p.ring) slot = 0, phase ^= 1u;
         }
+        if (ok && elect_lane()) {
+          commit(acc_full32 + 8 * (use & 1));
+          if (FUSED && last_of_op && s + 1 == slice1) commit(smem_addr(op_empty + op % p.bufs));
+        }
+        __syncwarp();
       }
     }
     if (!ok) give_up(ERR_WAIT_FULL);
@@ -395,40 +436,53 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       last_y = ti.y;
       ++op;
       if (op >= p.bufs) {
-        ok = mbar32_wait(smem_addr(op_empty + op % p.bufs), (op / p.bufs - 1) & 1, abort_word);
+        ok = warp_wait(smem_addr(op_empty + op % p.bufs), (op / p.bufs - 1) & 1, abort_word);
         if (!ok) break;
       }
       uint8_t* base = smem + (operand0 - smem_addr(smem)) + (op % p.bufs) * operand_bytes;
-      // a warp takes segments of 1024 inputs of a row, four 16-byte loads in flight a lane
-      const int segments = (pieces + 127) >> 7;
-      for (int w = qt >> 5; w < ti.rows * segments; w += qthreads >> 5) {
+      // a warp takes segments of 1024 inputs of a row, four 16-byte loads a lane; the next segment's are in flight meanwhile
+      const int segments = (pieces + 127) >> 7, total = ti.rows * segments, stride = qthreads >> 5;
+      auto fetch = [&](int w, uint4 (&v4)[4]) {
         const int r = w / segments, q0 = (w - r * segments) * 128 + lane;
         int64_t row = r;
+        bool live = true;
         if (grouped) {
           const int pair = p.members[ti.m0 + r];
-          if (pair < 0 || pair >= p.pairs) continue;
+          live = pair >= 0 && pair < p.pairs;
           row = p.slots > 0 ? pair / p.slots : pair;
         }
         const uint4* from = reinterpret_cast<const uint4*>(p.x + row * p.ldx) + p0;
-        uint4 v4[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int q = q0 + 32 * j;
-          v4[j] = q < pieces && (p0 + q) * 8 < p.K ? from[q] : make_uint4(0u, 0u, 0u, 0u);
+          v4[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (live && q < pieces && (p0 + q) * 8 < p.K) v4[j] = from[q];
+        }
+      };
+      uint4 next[4];
+      if ((qt >> 5) < total) fetch(qt >> 5, next);
+      for (int w = qt >> 5; w < total; w += stride) {
+        const int r = w / segments, q0 = (w - r * segments) * 128 + lane;
+        uint4 v4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v4[j] = next[j];
+        if (w + stride < total) fetch(w + stride, next);
+        uint32_t codes[4], scale[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v[8];
+          widen8(v4[j], v);
+          codes[j] = quantize_block(v, scale[j]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int q = q0 + 32 * j, b = q >> 2, u = b >> 3;
-          float v[8];
-          widen8(v4[j], v);
-          uint32_t scale;
-          const uint32_t codes = quantize_block(v, scale);
           if (q < pieces) {
             uint8_t* stage = base + u * S::B_BYTES;
             const uint32_t at = u0 + u < full_stages ? (r >> 3) * 1024 + (r & 7) * 128 + (((b & 7) ^ (r & 7)) << 4)
                                                      : ((b & 7) >> 1) * (NT * 32) + (r >> 3) * 256 + (r & 7) * 32 + (((b & 1) ^ ((r >> 2) & 1)) << 4);
-            *reinterpret_cast<uint32_t*>(stage + at + 4 * (q & 3)) = codes;
-            if ((q & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + r * 16 + (b & 3)] = static_cast<uint8_t>(scale);
+            *reinterpret_cast<uint32_t*>(stage + at + 4 * (q & 3)) = codes[j];
+            if ((q & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + r * 16 + (b & 3)] = static_cast<uint8_t>(scale[j]);
           }
         }
       }
@@ -541,7 +595,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         // slices are added in registers, and the sum goes back to where the last one came from
         float acc[S::CHUNKS][16];
         for (int s = slice0; s < slice1; ++s, ++use) {
-          ok = mbar32_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
+          ok = warp_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t src = lanes + (use & 1) * NT;
@@ -564,7 +618,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
           if (lane == 0) mbar_arrive(acc_empty + (use & 1));
         }
       } else {
-        ok = mbar32_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
+        ok = warp_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       if (!ok) break;
@@ -577,14 +631,13 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         tmem_load16(src + 16 * S::GROUPS * i, v);
         tmem_loaded();
         if (c > 1) {
-          // part [slice][row of the owner][128 columns] in the shared memory of the block that owns the row
-          const int share = (ti.n + c - 1) / c;
-          const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 4;
-          int owner = n / share, at = n - owner * share;
+          // part [slice][four rows of the owner][128 columns][4] in the shared memory of the block that owns the rows
+          const int share = quads_of(ti.rows, c);
+          const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 16;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (n + j < ti.rows) store_remote(part + (rank * share + at) * (MX_SB * 4), owner, v[j]);
-            if (++at == share) at = 0, ++owner;
+          for (int j = 0; j < 4; ++j) {
+            const int quad = (n >> 2) + j, owner = quad / share;
+            if (4 * quad < ti.rows) store_remote(part + (rank * share + quad - owner * share) * (MX_SB * 16), owner, v + 4 * j);
           }
         } else if (p.q != nullptr) {
           quantize16(ti, v, n);
@@ -607,22 +660,26 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     cluster_barrier();
     if (drains && my_tiles > 0 && *abort_flag == 0) {
       Tile ti = tile_at(0);
-      const int share = (ti.n + c - 1) / c, n0 = rank * share;
-      ti.rows = min(ti.rows, n0 + share);
-      const float* part = reinterpret_cast<const float*>(smem + extra_off) + lg * 32 + lane;
+      const int share = quads_of(ti.rows, c), n0 = 4 * rank * share;
+      ti.rows = min(ti.rows, n0 + 4 * share);
+      const float4* part = reinterpret_cast<const float4*>(smem + extra_off) + lg * 32 + lane;
 #pragma unroll 1
-      for (int i = 16 * group; n0 + i < ti.rows; i += 16 * S::GROUPS) {
-        float v[16] = {};
-#pragma unroll 1
-        for (int s = 0; s < c; ++s) {
+      for (int i = 4 * group; n0 + 4 * i < ti.rows; i += 4 * S::GROUPS) {
+        float v[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (n0 + i + j >= ti.rows) break;
-            const float a = part[(s * share + i + j) * MX_SB];
-            v[j] = s == 0 ? a : v[j] + a;
+        for (int j = 0; j < 4; ++j) {                                // (quads past the share read other parts and are not stored)
+          const float4 a = part[min(i + j, share - 1) * MX_SB];
+          v[4 * j] = a.x, v[4 * j + 1] = a.y, v[4 * j + 2] = a.z, v[4 * j + 3] = a.w;
+        }
+#pragma unroll 1
+        for (int s = 1; s < c; ++s) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 a = part[(s * share + min(i + j, share - 1)) * MX_SB];
+            v[4 * j] += a.x, v[4 * j + 1] += a.y, v[4 * j + 2] += a.z, v[4 * j + 3] += a.w;
           }
         }
-        finish16(ti, v, n0 + i);
+        finish16(ti, v, n0 + 4 * i);
       }
     }
   }
@@ -657,7 +714,7 @@ template <int NT, bool FUSED>
 cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
   using S = MxShape<NT, FUSED>;
   int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
-  if (p.cluster > 1) extra = (NT + p.cluster) * MX_SB * 4;
+  if (p.cluster > 1) extra = p.cluster * quads_of(std::min(p.tile, p.M), p.cluster) * MX_SB * 16;
   const int operand = FUSED ? p.operand_stages * S::B_BYTES : 0;
   if (FUSED && p.bufs == 2 && MX_SMEM_MAX - extra - 2 * operand < 4 * S::SLOT) p.bufs = 1;
   const int room = MX_SMEM_MAX - extra - p.bufs * operand;
@@ -729,7 +786,16 @@ Tiling tiling_for(int m, int n, int stages, int sk) {
 // Whether a block can hold its K slice of sixteen quantised rows beside a ring of four slots.
 bool fused_fits(int k, int sk) {
   const int stages = mx_stages(mx_steps(k)), longest = (stages + sk - 1) / sk;
-  return longest * MxShape<16, true>::B_BYTES + 4 * MX_UNIT + (MX_FUSED_ROWS + MX_CLUSTER_MAX) * MX_SB * 4 <= MX_SMEM_MAX;
+  return longest * MxShape<16, true>::B_BYTES + 4 * MX_UNIT + MX_CLUSTER_MAX * 4 * MX_SB * 4 <= MX_SMEM_MAX;
+}
+
+// Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its eight warps have
+// few segments of 1024 inputs each.
+constexpr int FUSED_SEGMENTS = 24;
+bool fused_pays(int m, int k, int sk) {
+  if (m > MX_FUSED_ROWS || !fused_fits(k, sk)) return false;
+  const int longest = (mx_stages(mx_steps(k)) + sk - 1) / sk;
+  return m * ((longest + 3) / 4) <= FUSED_SEGMENTS;
 }
 
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
@@ -756,7 +822,7 @@ int tf_mx_split(int n, int k) { return n < 1 || k < MX_BLOCK || k % MX_BLOCK ? T
 
 int64_t tf_mx_matmul_bytes(int m, int n, int k) {
   if (m < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
-  if (m <= MX_FUSED_ROWS && fused_fits(k, slices_for(n, k))) return 0;
+  if (fused_pays(m, k, slices_for(n, k))) return 0;
   const int steps = mx_steps(k), tile = tiling_for(m, n, mx_stages(steps), slices_for(n, k)).tile;
   return (m + tile - 1) / tile * mx_operand_bytes(tile, steps);
 }

@@ -30,16 +30,15 @@ __device__ __forceinline__ uint32_t quantize_block(float (&v)[8], uint32_t& scal
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
   top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  // no branch: several blocks in one thread would run one after another
+  const bool bad = top >= 0x7F800000u;
   const int e = static_cast<int>(top >> 23);
-  if (e == 255) {
-    scale = 255u;
-    return 0u;
-  }
-  scale = static_cast<uint32_t>(max(e - 2, 0));
-  const float inverse = __uint_as_float((254u - scale) << 23);
+  scale = bad ? 255u : static_cast<uint32_t>(max(e - 2, 0));
+  const float inverse = __uint_as_float((254u - min(scale, 254u)) << 23);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] *= inverse;
-  return e2m1x8(v);
+  const uint32_t codes = e2m1x8(v);
+  return bad ? 0u : codes;
 }
 
 __device__ __forceinline__ void widen8(uint4 p, float (&v)[8]) {

@@ -131,6 +131,16 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_
   if (__all_sync(0xFFFFFFFFu, mbar32_try_wait(bar, parity))) return true;
   return __all_sync(0xFFFFFFFFu, poll(bar, parity, abort_word));
 }
+// The copy and MMA roles are one thread each: a vote, an election and a reconvergence for each stage would cost more than its work.
+__device__ __forceinline__ bool lane_wait(uint32_t bar, uint32_t parity, uint32_t abort_word) {
+  return mbar32_try_wait(bar, parity) || poll(bar, parity, abort_word);
+}
+// One test that does not wait.  Asked for a stage before the one ahead of it is issued, its hundred cycles are hidden.
+__device__ __forceinline__ uint32_t lane_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok;
+}
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -276,103 +286,122 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
   };
   auto slice_at = [&](int s) { return static_cast<int>(static_cast<int64_t>(p.stages) * s / p.sk); };
 
+  // Stages of the block in order: a ring slot, and the parity of its barriers.
+  struct Ring {
+    int slot;
+    uint32_t phase;
+    __device__ __forceinline__ void next(int ring) {
+      if (++slot == ring) slot = 0, phase ^= 1u;
+    }
+  };
+  auto lost = [&](int code) {                                      // one thread gave up
+    *abort_flag = code;
+    atomicCAS(p.err, 0, code);
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------------ weights
-    bool ok = true;
-    int slot = 0;
-    uint32_t phase = 1;
-    for (int it = 0; it < my_tiles && ok; ++it) {
-      const Tile ti = tile_at(it);
+    if (elect_lane()) {
+      const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty);
+      const uint32_t last_bytes = tail * 4096 + mx_tail_scales(tail);
+      bool ok = true;
+      Ring r = {0, 1u};
+      uint32_t ready = 1u;                                         // (a fresh slot's test passes)
+      for (int it = 0; it < my_tiles && ok; ++it) {
+        const Tile ti = tile_at(it);
+        const int u0 = slice_at(slice0), u1 = slice_at(slice1);
+        const uint8_t* src = p.w + ti.w + static_cast<int64_t>(u0) * MX_UNIT;
 #pragma unroll 1
-      for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
-        ok = warp_wait(smem_addr(empty + slot), phase, abort_word);
-        if (!ok) break;
-        const uint32_t bytes = u < full_stages ? MX_UNIT : tail * 4096 + mx_tail_scales(tail);
-        if (elect_lane()) {
-          mbar32_expect_tx(smem_addr(full + slot), bytes);
-          bulk_load32(ring0 + slot * S::SLOT, p.w + ti.w + static_cast<int64_t>(u) * MX_UNIT, bytes, smem_addr(full + slot));
+        for (int u = u0; u < u1; ++u, src += MX_UNIT) {
+          if (!ready && !(ok = lane_wait(empty32 + 8 * r.slot, r.phase, abort_word))) break;
+          const uint32_t bar = full32 + 8 * r.slot, dst = ring0 + r.slot * S::SLOT;
+          r.next(p.ring);
+          ready = lane_test(empty32 + 8 * r.slot, r.phase);
+          const uint32_t bytes = u < full_stages ? MX_UNIT : last_bytes;
+          mbar32_expect_tx(bar, bytes);
+          bulk_load32(dst, src, bytes, bar);
         }
-        __syncwarp();
-        if (++slot == p.ring) slot = 0, phase ^= 1u;
       }
+      if (!ok) lost(ERR_WAIT_EMPTY), let_copies_land();
     }
-    if (!ok) give_up(ERR_WAIT_EMPTY), let_copies_land();
+    __syncwarp();
   } else if (warp == 2 && !FUSED) {
     // ------------------------------------------------------------------ quantised rows
     pdl_wait();
-    bool ok = true;
-    int slot = 0;
-    uint32_t phase = 1;
-    const int64_t stage_bytes = mx_stage_bytes(p.b_rows);
-    for (int it = 0; it < my_tiles && ok; ++it) {
-      const Tile ti = tile_at(it);
-      const uint8_t* op = p.b + ti.y * p.item_stride;
-      const int sbs = mx_scale_blocks(ti.n);
+    if (elect_lane()) {
+      const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty);
+      const int64_t stage_bytes = mx_stage_bytes(p.b_rows);
+      bool ok = true;
+      Ring r = {0, 1u};
+      uint32_t ready = 1u;
+      for (int it = 0; it < my_tiles && ok; ++it) {
+        const Tile ti = tile_at(it);
+        const int sbs = mx_scale_blocks(ti.n), u0 = slice_at(slice0), u1 = slice_at(slice1);
+        const uint8_t* src = p.b + ti.y * p.item_stride + u0 * stage_bytes;
 #pragma unroll 1
-      for (int u = slice_at(slice0), end = slice_at(slice1); u < end; ++u) {
-        ok = warp_wait(smem_addr(empty + slot), phase, abort_word);
-        if (!ok) break;
-        const bool whole = u < full_stages;
-        const uint32_t bar = smem_addr(full + slot), dst = ring0 + slot * S::SLOT + MX_UNIT;
-        const uint32_t scales = whole ? MX_SCALES : mx_tail_scales(tail);     // per 128 rows
-        const uint8_t* src = op + u * stage_bytes;
-        if (elect_lane()) {
-          mbar32_expect_tx(bar, ti.n * (whole ? 128 : 32 * tail) + sbs * scales);
-          if (whole) {
+        for (int u = u0; u < u1; ++u, src += stage_bytes) {
+          if (!ready && !(ok = lane_wait(empty32 + 8 * r.slot, r.phase, abort_word))) break;
+          const uint32_t bar = full32 + 8 * r.slot, dst = ring0 + r.slot * S::SLOT + MX_UNIT;
+          r.next(p.ring);
+          ready = lane_test(empty32 + 8 * r.slot, r.phase);
+          if (u < full_stages) {
+            mbar32_expect_tx(bar, ti.n * 128 + sbs * MX_SCALES);
             bulk_load32(dst, src, ti.n * 128, bar);
-            src += static_cast<int64_t>(p.b_rows) * 128;
+            bulk_load32(dst + NT * 128, src + p.b_rows * 128, sbs * MX_SCALES, bar);
           } else {
-            for (int j = 0; j < tail; ++j) {
-              bulk_load32(dst + j * NT * 32, src, ti.n * 32, bar);
-              src += static_cast<int64_t>(p.b_rows) * 32;
-            }
+            const uint32_t scales = sbs * mx_tail_scales(tail);
+            mbar32_expect_tx(bar, ti.n * 32 * tail + scales);
+            for (int j = 0; j < tail; ++j) bulk_load32(dst + j * NT * 32, src + j * p.b_rows * 32, ti.n * 32, bar);
+            bulk_load32(dst + NT * 128, src + tail * p.b_rows * 32, scales, bar);
           }
-          bulk_load32(dst + NT * 128, src, sbs * scales, bar);
         }
-        __syncwarp();
-        if (++slot == p.ring) slot = 0, phase ^= 1u;
       }
+      if (!ok) lost(ERR_WAIT_EMPTY), let_copies_land();
     }
-    if (!ok) give_up(ERR_WAIT_EMPTY), let_copies_land();
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
-    // The loop over whole stages is kept to adds on descriptors that are the same in every lane: with descriptors built in
-    // place and the last stage's form beside it in one body, a stage cost 700 cycles of issue at 16 rows.
-    const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty), acc_full32 = smem_addr(acc_full);
-    const uint32_t sf0 = tmem + 2 * NT;
-    const uint64_t a0 = desc(ring0, 1024, SWIZZLE_128), as0 = desc(ring0 + MX_SB * 128, 128, SWIZZLE_NONE);
-    const uint64_t b0 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 1024, SWIZZLE_128);
-    const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + NT * 128, 128, SWIZZLE_NONE);
-    bool ok = true;
-    int slot = 0, use = 0, op = -1, last_y = -1;
-    uint32_t phase = 0;
-    for (int it = 0; it < my_tiles && ok; ++it) {
-      const Tile ti = tile_at(it);
-      bool last_of_op = false;
-      if (FUSED) {
-        const bool new_op = grouped ? ti.y != last_y : it == 0;
-        last_y = ti.y;
-        if (new_op) {
-          ++op;
-          ok = warp_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word);
-          if (!ok) break;
+    // Measured on one block: an MMA of N columns takes N / 2 cycles but no less than 40 to issue, a scale copy 10 beside MMAs and
+    // 37 alone, a commit 34 alone, a wait that passes 110.  The pipe takes few instructions ahead of it, so what a stage costs this
+    // thread beyond them shows: descriptors are kept to adds, the next stage's barrier is tested before this stage's MMAs, and
+    // the last stage, whose steps are regions of their own, has code of its own.
+    if (elect_lane()) {
+      const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty), acc_full32 = smem_addr(acc_full), acc_empty32 = smem_addr(acc_empty);
+      const uint32_t sf0 = tmem + 2 * NT;
+      const uint64_t a0 = desc(ring0, 1024, SWIZZLE_128), as0 = desc(ring0 + MX_SB * 128, 128, SWIZZLE_NONE);
+      const uint64_t b0 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 1024, SWIZZLE_128);
+      const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + NT * 128, 128, SWIZZLE_NONE);
+      bool ok = true;
+      Ring r = {0, 0u};
+      int use = 0, op = -1, last_y = -1;
+      uint32_t ready = 0;
+      for (int it = 0; it < my_tiles && ok; ++it) {
+        const Tile ti = tile_at(it);
+        bool last_of_op = false;
+        if (FUSED) {
+          const bool new_op = grouped ? ti.y != last_y : it == 0;
+          last_y = ti.y;
+          if (new_op) {
+            ++op;
+            if (!(ok = lane_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word))) break;
+          }
+          last_of_op = grouped && (it + 1 == my_tiles || (first_tile + it + 1) / ncb != ti.y);
         }
-        last_of_op = grouped && (it + 1 == my_tiles || (first_tile + it + 1) / ncb != ti.y);
-      }
-      const uint32_t n8 = __shfl_sync(0xFFFFFFFFu, static_cast<uint32_t>(ti.n), 0);
-      const uint32_t id0 = instruction(n8, 0), id1 = instruction(n8, 1);
-      for (int s = slice0; s < slice1 && ok; ++s, ++use) {
-        const int start = slice_at(s), end = slice_at(s + 1), last_whole = min(end, full_stages);
-        if (use >= 2) ok = warp_wait(smem_addr(acc_empty + (use & 1)), ((use >> 1) - 1) & 1, abort_word);
-        const uint32_t d = tmem + (use & 1) * NT;
-        uint32_t more = 0;                                           // 0: the first step of the slice overwrites the accumulator
-        uint32_t fused_at = FUSED ? (op % p.bufs) * (operand_bytes >> 4) : 0;
-#pragma unroll 1
-        for (int u = start; u < last_whole && ok; ++u) {
-          ok = warp_wait(full32 + 8 * slot, phase, abort_word);
+        const uint32_t id0 = instruction(ti.n, 0), id1 = instruction(ti.n, 1);
+        for (int s = slice0; s < slice1 && ok; ++s, ++use) {
+          const int start = slice_at(s), end = slice_at(s + 1), last_whole = min(end, full_stages);
+          if (use >= 2 && !(ok = lane_wait(acc_empty32 + 8 * (use & 1), ((use >> 1) - 1) & 1, abort_word))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t at = slot * (S::SLOT >> 4), bt = FUSED ? fused_at : at, sa = sf0 + slot * S::SF_COLS, sb = sa + 8;
-          if (ok && elect_lane()) {
+          const uint32_t d = tmem + (use & 1) * NT;
+          uint32_t more = 0;                                         // 0: the first step of the slice overwrites the accumulator
+          uint32_t fused_at = FUSED ? (op % p.bufs) * (operand_bytes >> 4) : 0;
+#pragma unroll 1
+          for (int u = start; u < last_whole; ++u) {
+            if (!ready && !(ok = lane_wait(full32 + 8 * r.slot, r.phase, abort_word))) break;
+            const uint32_t at = r.slot * (S::SLOT >> 4), bt = FUSED ? fused_at : at, sa = sf0 + r.slot * S::SF_COLS, sb = sa + 8;
+            const uint32_t done = empty32 + 8 * r.slot;
+            r.next(p.ring);
+            ready = lane_test(full32 + 8 * r.slot, r.phase);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               copy_scales(sa + 4 * h, as0 + at + 32 * h);
@@ -383,19 +412,15 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
             mma_mxf4(d, a0 + at + 2, b0 + bt + 2, id1, sa, sb, 1u);
             mma_mxf4(d, a0 + at + 4, b0 + bt + 4, id0, sa + 4, sb + 4 * S::SBS, 1u);
             mma_mxf4(d, a0 + at + 6, b0 + bt + 6, id1, sa + 4, sb + 4 * S::SBS, 1u);
-            commit(empty32 + 8 * slot);
+            commit(done);
+            more = 1;
+            if (FUSED) fused_at += S::B_BYTES >> 4;
           }
-          __syncwarp();
-          more = 1;
-          if (FUSED) fused_at += S::B_BYTES >> 4;
-          if (++slot == p.ring) slot = 0, phase ^= 1u;
-        }
-        if (end > full_stages && ok) {                               // the last stage: `tail` steps, each a region of its own
-          ok = warp_wait(full32 + 8 * slot, phase, abort_word);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a = ring0 + slot * S::SLOT, b = FUSED ? operand0 + fused_at * 16 : a + MX_UNIT;
-          const uint32_t sb_bytes = FUSED ? MX_SCALES : mx_tail_scales(tail), sa = sf0 + slot * S::SF_COLS, sb = sa + 8;
-          if (ok && elect_lane()) {
+          if (!ok) break;
+          if (end > full_stages) {                                   // the last stage: `tail` steps, each a region of its own
+            if (!ready && !(ok = lane_wait(full32 + 8 * r.slot, r.phase, abort_word))) break;
+            const uint32_t a = ring0 + r.slot * S::SLOT, b = FUSED ? operand0 + fused_at * 16 : a + MX_UNIT;
+            const uint32_t sb_bytes = FUSED ? MX_SCALES : mx_tail_scales(tail), sa = sf0 + r.slot * S::SF_COLS, sb = sa + 8;
 #pragma unroll 1
             for (int h = 0; 2 * h < tail; ++h) {
               copy_scales(sa + 4 * h, desc(a + tail * 4096 + 512 * h, 128, SWIZZLE_NONE));
@@ -406,19 +431,17 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
             for (int j = 0; j < tail; ++j)
               mma_mxf4(d, desc(a + j * 4096, 256, SWIZZLE_32), desc(b + j * NT * 32, 256, SWIZZLE_32), j & 1 ? id1 : id0, sa + 4 * (j >> 1),
                        sb + 4 * S::SBS * (j >> 1), more | (j > 0));
-            commit(empty32 + 8 * slot);
+            commit(empty32 + 8 * r.slot);
+            r.next(p.ring);
+            ready = 0;
           }
-          __syncwarp();
-          if (++slot == p.ring) slot = 0, phase ^= 1u;
-        }
-        if (ok && elect_lane()) {
           commit(acc_full32 + 8 * (use & 1));
           if (FUSED && last_of_op && s + 1 == slice1) commit(smem_addr(op_empty + op % p.bufs));
         }
-        __syncwarp();
       }
+      if (!ok) lost(ERR_WAIT_FULL);
     }
-    if (!ok) give_up(ERR_WAIT_FULL);
+    __syncwarp();
   }
 
   if (FUSED && (grouped ? warp >= 8 : warp >= 4)) {
@@ -623,13 +646,17 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       }
       if (!ok) break;
       const uint32_t src = lanes + (use & 1) * NT;
+      float ahead[16];                                               // the next sixteen rows are on their way meanwhile
+      if (16 * group < ti.rows) tmem_load16(src, ahead);
 #pragma unroll 1
       for (int i = 0; i < S::CHUNKS; ++i) {
         const int n = 16 * (S::GROUPS * i + group);
         if (n >= ti.rows) break;
         float v[16];
-        tmem_load16(src + 16 * S::GROUPS * i, v);
         tmem_loaded();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = ahead[j];
+        if (n + 16 * S::GROUPS < ti.rows) tmem_load16(src + 16 * S::GROUPS * (i + 1), ahead);
         if (c > 1) {
           // part [slice][four rows of the owner][128 columns][4] in the shared memory of the block that owns the rows
           const int share = quads_of(ti.rows, c);

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     ti.n = max(8, (ti.rows + 7) & ~7);
     return ti;
   };
-  auto slice_at = [&](int s) { return static_cast<int>(static_cast<int64_t>(p.stages) * s / p.sk); };
+  auto slice_at = [&](int s) { return p.sk == 1 ? s * p.stages : p.stages * s / p.sk; };
 
   // Stages of the block in order: a ring slot, and the parity of its barriers.
   struct Ring {

@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/tensorfold_b200.h"
 #include "mx_layout.h"
 #include "mx_quant.cuh"
@@ -17,7 +19,7 @@ int cuda_fail_moe(cudaError_t e, const char* what);
 namespace {
 
 // Eight values of one of the stored types: 0 bf16, 1 fp16, 2 fp32.
-__device__ __forceinline__ void load8(const void* row, int64_t at, int dtype, float (&v)[8]) {
+__device__ __forceinline__ void load8(const void* row, int64_t at, const int dtype, float (&v)[8]) {
   if (dtype == 0) {
     widen8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(row) + at), v);
   } else if (dtype == 1) {
@@ -35,57 +37,91 @@ __device__ __forceinline__ void load8(const void* row, int64_t at, int dtype, fl
   }
 }
 
-// Rows to stored words and scales.  A lane takes eight values, four lanes a block, so loads and stores of a warp are runs.
-__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int64_t ldx, int dtype, int64_t pieces, int per_row,
-                                                       uint32_t* __restrict__ words, uint8_t* __restrict__ scales) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  // whole warps walk together: a piece past the end computes on zeros and stores nothing
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31); first < pieces; first += step) {
-    const int64_t i = first + (threadIdx.x & 31);
-    float v[8] = {};
-    const int64_t r = i / per_row;
-    if (i < pieces) load8(static_cast<const char*>(x) + r * ldx * (dtype == 2 ? 4 : 2), (i - r * per_row) * 8, dtype, v);
-    uint32_t scale;
-    const uint32_t codes = quantize_block(v, scale);
-    if (i < pieces) {
-      words[i] = codes;
-      if ((i & 3) == 0) scales[i >> 2] = static_cast<uint8_t>(scale);
+// Rows to stored words and scales.  A lane takes eight values, four lanes a block, so loads and stores of a warp are runs; U
+// pieces a thread are in flight at once.  Rows one after another (FLAT) are one run of pieces; others go by blockIdx.y.
+template <int DTYPE, bool FLAT, int U>
+__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int64_t pieces, uint32_t* __restrict__ words,
+                                                       uint8_t* __restrict__ scales) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    const char* from = static_cast<const char*>(x) + (FLAT ? 0 : row * ldx * (DTYPE == 2 ? 4 : 2));
+    // whole warps walk together: a piece past the end computes on zeros and stores nothing
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + (threadIdx.x & ~31); first < pieces; first += U * step) {
+      float v[U][8];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = first + u * step + (threadIdx.x & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
+        if (i < pieces) load8(from, i * 8, DTYPE, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = first + u * step + (threadIdx.x & 31);
+        uint32_t scale;
+        const uint32_t codes = quantize_block(v[u], scale);
+        if (i < pieces) {
+          const int64_t to = FLAT ? i : row * pieces + i;
+          words[to] = codes;
+          if ((i & 3) == 0) scales[to >> 2] = static_cast<uint8_t>(scale);
+        }
+      }
     }
   }
 }
 
-// Stored words and scales to values.  Every value is exact in bf16 and fp32 but where 2^127 or more overflows bf16's largest.
+// Stored words and scales to values, exact in bf16 and fp32 (2^127 times 2 and more overflows).  An e2m1 magnitude m, three
+// bits, moved to the top of a fraction field reads as value * 2^-126 (two exponent bits and one of fraction, subnormals alike), so
+// two products by powers of two make the value; in bf16 two values go at once.
+template <int OUT, int U>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ words, const uint8_t* __restrict__ scales, int64_t pieces,
-                                                         int out_type, void* __restrict__ out) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < pieces; i += step) {
-    const uint32_t w = words[i], code = scales[i >> 2];
-    const float scale = __uint_as_float(code == 255u ? 0x7FC00000u : code == 0u ? 0x00400000u : code << 23);
-    float v[8];
+                                                         void* __restrict__ out) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; first < pieces; first += U * step) {
+    uint32_t w[U], code[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t q = w >> (4 * j);
-      // e2m1 to fp32: two exponent bits and one of fraction; the only subnormal is 0.5
-      const uint32_t m = q & 7u;
-      const float a = m < 2u ? (m ? 0.5f : 0.f) : __uint_as_float((m << 22) + (126u << 23));
-      v[j] = ((q & 8u) ? -a : a) * scale;
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = first + u * step;
+      w[u] = i < pieces ? words[i] : 0u;
+      code[u] = i < pieces ? scales[i >> 2] : 0u;
     }
-    if (out_type == 2) {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + i * 8);
-      o[0] = make_float4(v[0], v[1], v[2], v[3]), o[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t p[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (out_type == 0) {
-          const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-          p[j] = *reinterpret_cast<const uint32_t*>(&t);
-        } else {
-          const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = first + u * step;
+      if (i >= pieces) break;
+      if (OUT == 0) {
+        const uint32_t s1 = code[u] == 255u ? 0x7FC0u : code[u] == 0u ? 0x0040u : code[u] << 7, s2 = s1 | (s1 << 16), lift2 = 0x7E807E80u;
+        const __nv_bfloat162 lift = *reinterpret_cast<const __nv_bfloat162*>(&lift2), scale = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+        uint32_t p[4];                                               // values j and j + 4
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t q = w[u] >> (4 * j), bits = ((q & 0x00070007u) << 6) | ((q & 0x00080008u) << 12);
+          const __nv_bfloat162 t = __hmul2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), lift), scale);
           p[j] = *reinterpret_cast<const uint32_t*>(&t);
         }
+        static_cast<uint4*>(out)[i] = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
+                                                 __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
+      } else {
+        const float scale = __uint_as_float(code[u] == 255u ? 0x7FC00000u : code[u] == 0u ? 0x00400000u : code[u] << 23);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t q = w[u] >> (4 * j);
+          v[j] = __uint_as_float(((q & 7u) << 22) | ((q & 8u) << 28)) * 0x1p126f * scale;
+        }
+        if (OUT == 2) {
+          float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + i * 8);
+          o[0] = make_float4(v[0], v[1], v[2], v[3]), o[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          uint32_t p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            p[j] = *reinterpret_cast<const uint32_t*>(&t);
+          }
+          static_cast<uint4*>(out)[i] = make_uint4(p[0], p[1], p[2], p[3]);
+        }
       }
-      reinterpret_cast<uint4*>(out)[i] = make_uint4(p[0], p[1], p[2], p[3]);
     }
   }
 }
@@ -189,6 +225,8 @@ int blocks_for(int64_t threads) {
   return static_cast<int>(b < 1 ? 1 : b > 148 * 64 ? 148 * 64 : b);
 }
 
+constexpr int64_t MANY = 148 * 2048 * 4;      // pieces past which a thread takes four at a time
+
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 }  // namespace
@@ -229,8 +267,18 @@ int tf_mx_quantize(const void* x, int64_t ldx, int dtype, int rows, int k, void*
   if (misaligned(x, 16) || (rows > 1 && ldx % (dtype == 2 ? 4 : 8)) || misaligned(words, 4))
     return fail_moe(TF_ERR_ALIGN, "tf_mx_quantize: rows must start on 16-byte boundaries");
   const int64_t pieces = static_cast<int64_t>(rows) * (k / 8);
-  quantize_kernel<<<blocks_for(pieces), 256, 0, static_cast<cudaStream_t>(stream)>>>(x, ldx, dtype, pieces, k / 8, static_cast<uint32_t*>(words),
-                                                                                     static_cast<uint8_t*>(scales));
+  const bool flat = rows == 1 || ldx == k;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint32_t* w = static_cast<uint32_t*>(words);
+  uint8_t* s = static_cast<uint8_t*>(scales);
+#define TF_MX_QUANTIZE(DT)                                                                                                            \
+  if (dtype == DT) {                                                                                                                  \
+    if (!flat) quantize_kernel<DT, false, 1><<<dim3((k / 8 + 255) / 256, std::min(rows, 65535)), 256, 0, st>>>(x, ldx, rows, k / 8, w, s); \
+    else if (pieces < MANY) quantize_kernel<DT, true, 1><<<blocks_for(pieces), 256, 0, st>>>(x, ldx, 1, pieces, w, s);                 \
+    else quantize_kernel<DT, true, 4><<<blocks_for((pieces + 3) / 4), 256, 0, st>>>(x, ldx, 1, pieces, w, s);                          \
+  }
+  TF_MX_QUANTIZE(0) TF_MX_QUANTIZE(1) TF_MX_QUANTIZE(2)
+#undef TF_MX_QUANTIZE
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_quantize");
 }
@@ -240,8 +288,16 @@ int tf_mx_dequantize(const void* words, const void* scales, int rows, int k, int
     return fail_moe(TF_ERR_ARG, "tf_mx_dequantize: rows of a positive multiple of 32 values, none null");
   if (misaligned(words, 4) || misaligned(out, 16)) return fail_moe(TF_ERR_ALIGN, "tf_mx_dequantize: out must start on a 16-byte boundary");
   const int64_t pieces = static_cast<int64_t>(rows) * (k / 8);
-  dequantize_kernel<<<blocks_for(pieces), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint32_t*>(words), static_cast<const uint8_t*>(scales), pieces, out_type, out);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const uint32_t* w = static_cast<const uint32_t*>(words);
+  const uint8_t* s = static_cast<const uint8_t*>(scales);
+#define TF_MX_DEQUANTIZE(OUT)                                                                                             \
+  if (out_type == OUT) {                                                                                                  \
+    if (pieces < MANY) dequantize_kernel<OUT, 1><<<blocks_for(pieces), 256, 0, st>>>(w, s, pieces, out);                   \
+    else dequantize_kernel<OUT, 4><<<blocks_for((pieces + 3) / 4), 256, 0, st>>>(w, s, pieces, out);                       \
+  }
+  TF_MX_DEQUANTIZE(0) TF_MX_DEQUANTIZE(1) TF_MX_DEQUANTIZE(2)
+#undef TF_MX_DEQUANTIZE
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_dequantize");
 }

@@ -4,7 +4,7 @@
 // rows, and the seven calls of a dense layer 190 us against 90.
 //
 // Two kinds of functions: whole wrappers for the calls an engine issues per layer (matmul, matmul_set, prefill_matmul,
-// matmul_act, add_rmsnorm, swiglu), and one thin thunk per C-ABI entry for the rest, which takes tensors where the entry
+// matmul_act, add_rmsnorm, swiglu, the microscaled product and quantisation), and one thin thunk per C-ABI entry for the rest, which takes tensors where the entry
 // takes pointers.  Refused arguments raise ValueError, failed launches RuntimeError.  The library itself stays free of
 // Python and torch: its entry points are resolved with dlsym from the path the Python side loaded.
 #include <ATen/ATen.h>
@@ -31,10 +31,10 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------
 
 #define TF_WRAPPED(X) X(tf_qmm) X(tf_qmm_set) X(tf_qmm_set_scratch_bytes) X(tf_qmm_window) X(tf_qmm_window_part_bytes) X(tf_qmm_prefill) X(tf_qmm_prefill_act) X(tf_qmm_act) \
-  X(tf_add_rmsnorm) X(tf_swiglu)
+  X(tf_add_rmsnorm) X(tf_swiglu) X(tf_mx_quantize) X(tf_mx_dequantize) X(tf_mx_tiled_bytes) X(tf_mx_matmul) X(tf_mx_matmul_bytes)
 #define TF_THUNKS(X) X(tf_pack) X(tf_pack_pair) X(tf_unpack) X(tf_group_sums) X(tf_affine_rows) X(tf_moe_plan) X(tf_moe_experts) \
   X(tf_moe_experts_prefill) X(tf_moe_gather) X(tf_moe_experts_sorted) X(tf_moe_router) X(tf_moe_router_tiles) X(tf_moe_topk) X(tf_moe_topk_local) X(tf_moe_combine) \
-  X(tf_mx_quantize) X(tf_mx_dequantize) X(tf_mx_pack) X(tf_mx_unpack) X(tf_mx_matmul) X(tf_mx_experts)
+  X(tf_mx_pack) X(tf_mx_unpack) X(tf_mx_experts)
 
 #define TF_POINTER(name) decltype(&::name) p_##name = nullptr;
 TF_WRAPPED(TF_POINTER)
@@ -537,6 +537,109 @@ PyObject* swiglu(PyObject* const* a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// microscaled 4-bit floating point
+// ---------------------------------------------------------------------------------------------------------------------
+
+constexpr int64_t MX_BLOCK = 32, MX_COLS = 128;
+
+// dtype numbers of the C entries; below 0: not one of them
+int mx_type(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1; }
+
+bool whole_rows(const at::Tensor& x, int64_t k) {       // rows that the kernels can read in 16-byte pieces
+  return x.stride(1) == 1 && (x.size(0) <= 1 || (x.stride(0) * x.element_size() % 16 == 0 && x.stride(0) >= k)) && aligned(x.data_ptr(), 16);
+}
+
+at::Tensor blocks(at::IntArrayRef sizes, int64_t last, at::ScalarType type, const at::Tensor& like) {
+  at::DimVector shape(sizes.begin(), sizes.end());
+  shape.back() = last;
+  return empty(shape, type, like);
+}
+
+// mx_quantize(x) -> (words, scales)
+PyObject* mx_quantize(PyObject* const* a) {
+  const char* who = "quantize";
+  const at::Tensor& x = tensor(a[0], who);
+  const int type = mx_type(x.scalar_type());
+  if (type < 0) refuse("quantize: x must be bf16, fp16 or fp32");
+  if (x.dim() < 1 || x.size(-1) % MX_BLOCK) refuse("quantize: rows of x must be whole blocks of %d", static_cast<int>(MX_BLOCK));
+  const int64_t k = x.size(-1), m = k ? x.numel() / k : 0;
+  const cudaStream_t stream = stream_of(x);
+  const at::Tensor words = blocks(x.sizes(), k / 8, at::kInt, x), scales = blocks(x.sizes(), k / MX_BLOCK, at::kByte, x);
+  if (x.numel() > 0) {
+    if (m > INT32_MAX || k > INT32_MAX) refuse("quantize: too many rows");
+    at::Tensor rows = x.dim() == 2 ? x : x.reshape({-1, k});
+    if (!whole_rows(rows, k)) rows = rows.clone(at::MemoryFormat::Contiguous);
+    const int64_t ldx = m > 1 ? rows.stride(0) : k;
+    check(unlocked([&] {
+            return p_tf_mx_quantize(rows.data_ptr(), ldx, type, static_cast<int>(m), static_cast<int>(k), words.data_ptr(), scales.data_ptr(), stream);
+          }),
+          who);
+  }
+  return Py_BuildValue("NN", THPVariable_Wrap(words), THPVariable_Wrap(scales));
+}
+
+// mx_dequantize(words, scales, type) -> values; type: the C entries' number
+PyObject* mx_dequantize(PyObject* const* a) {
+  const char* who = "dequantize";
+  const at::Tensor &words = tensor(a[0], who), &scales = tensor(a[1], who);
+  if ((words.scalar_type() != at::kInt && words.scalar_type() != at::kUInt32) || scales.scalar_type() != at::kByte)
+    refuse("dequantize: words must be int32 or uint32, scales uint8");
+  if (words.dim() < 1 || words.dim() != scales.dim() || words.size(-1) != 4 * scales.size(-1) ||
+      !words.sizes().slice(0, words.dim() - 1).equals(scales.sizes().slice(0, words.dim() - 1)))
+    refuse("dequantize: words do not match the scales of blocks of %d", static_cast<int>(MX_BLOCK));
+  if (words.device() != scales.device()) refuse("dequantize: words and scales must share a device");
+  const int type = static_cast<int>(integer(a[2]));
+  const int64_t k = 8 * words.size(-1), m = k ? words.numel() * 8 / k : 0;
+  const cudaStream_t stream = stream_of(words);
+  const at::Tensor out = blocks(words.sizes(), k, type == 0 ? at::kBFloat16 : type == 1 ? at::kHalf : at::kFloat, words);
+  if (out.numel() > 0) {
+    if (m > INT32_MAX || k > INT32_MAX) refuse("dequantize: too many rows");
+    const at::Tensor w = words.contiguous(), s = scales.contiguous();
+    check(unlocked([&] {
+            return p_tf_mx_dequantize(w.data_ptr(), s.data_ptr(), static_cast<int>(m), static_cast<int>(k), type, out.data_ptr(), stream);
+          }),
+          who);
+  }
+  return THPVariable_Wrap(out);
+}
+
+// mx_matmul(x, q, epi, limit, f32, out, pdl)
+PyObject* mx_matmul(PyObject* const* a) {
+  const int epi = static_cast<int>(integer(a[2]));
+  const char* who = epi ? "matmul_act" : "matmul";
+  Owned w(PyObject_GetAttr(a[1], s_weight));
+  const at::Tensor& units = tensor(w.p, "weight");
+  const int n = Weight::field(a[1], s_n), k = Weight::field(a[1], s_k);
+  const at::Tensor& given = tensor(a[0], who);
+  if (given.scalar_type() != at::kBFloat16 || given.dim() != 2 || given.size(1) != k) refuse("%s: x must be (M, %d) bf16", who, k);
+  if (given.size(0) < 1) refuse("%s: x needs at least one row", who);
+  if (given.size(0) > INT32_MAX / 2) refuse("%s: too many rows", who);
+  const cudaStream_t stream = stream_of(given);
+  if (units.device() != given.device()) refuse("%s: x and the weight must share a CUDA device", who);
+  const int64_t bytes = p_tf_mx_tiled_bytes(MX_COLS, k);
+  if (n < 1 || bytes < 0 || units.scalar_type() != at::kByte || units.dim() != 2 || units.size(0) != (n + MX_COLS - 1) / MX_COLS ||
+      units.size(1) != bytes || !units.is_contiguous())
+    refuse("%s: the packed weight does not have the super-blocks of its shape", who);
+  if (epi == 2 && n % 32) refuse("%s: swiglu takes a pack_pair weight", who);
+  const at::Tensor x = whole_rows(given, k) ? given : given.clone(at::MemoryFormat::Contiguous);
+  const bool f32 = truth(a[4]), pdl = truth(a[6]);
+  const float limit = static_cast<float>(number(a[3]));
+  const int m = static_cast<int>(x.size(0)), cols = epi == 2 ? n / 2 : n;
+  const at::Tensor out = out_of(a[5], m, cols, f32 ? at::kFloat : at::kBFloat16, x, who);
+  if (out.device() != x.device() || (m > 1 && out.stride(0) < cols)) refuse("%s: out must have rows of its own on x's device", who);
+  const int64_t need = p_tf_mx_matmul_bytes(m, n, k);
+  at::Tensor work;
+  if (need > 0) work = empty({need}, at::kByte, x);
+  const int64_t ldx = m > 1 ? x.stride(0) : k, ldo = m > 1 ? out.stride(0) : cols;
+  check(unlocked([&] {
+          return p_tf_mx_matmul(x.data_ptr(), ldx, m, units.data_ptr(), n, k, out.data_ptr(), ldo, f32, epi, limit,
+                                work.defined() ? work.data_ptr() : nullptr, need, pdl, stream);
+        }),
+        who);
+  return THPVariable_Wrap(out);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // thunks: name(what, ...) calls the C-ABI entry `name` with tensors (or addresses, or None) for its pointers
 // ---------------------------------------------------------------------------------------------------------------------
 
@@ -601,6 +704,9 @@ TF_WHOLE(prefill_matmul, 4)
 TF_WHOLE(matmul_act, 7)
 TF_WHOLE(add_rmsnorm, 5)
 TF_WHOLE(swiglu, 3)
+TF_WHOLE(mx_quantize, 1)
+TF_WHOLE(mx_dequantize, 3)
+TF_WHOLE(mx_matmul, 7)
 
 #define TF_THUNK(name)                                                                          \
   PyObject* py_##name(PyObject*, PyObject* const* args, Py_ssize_t nargs) {                     \
@@ -651,6 +757,7 @@ PyMethodDef g_methods[] = {
     {"stream_of", py_stream_of, METH_O, nullptr},
     {"forget_scratch", py_forget_scratch, METH_NOARGS, nullptr},
     TF_FAST(matmul) TF_FAST(matmul_set) TF_FAST(prefill_matmul) TF_FAST(matmul_act) TF_FAST(add_rmsnorm) TF_FAST(swiglu)
+    TF_FAST(mx_quantize) TF_FAST(mx_dequantize) TF_FAST(mx_matmul)
     TF_THUNKS(TF_FAST){nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

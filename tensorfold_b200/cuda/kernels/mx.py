@@ -17,7 +17,7 @@ from ... import _lib
 
 BLOCK = 32                                       # inputs that share a scale
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_EPILOGUES = {None: 0, "relu2": 1, "swiglu": 2}
+_EPILOGUES = {"relu2": 1, "swiglu": 2}
 
 
 @dataclass
@@ -49,34 +49,15 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     2^(floor(log2 of its largest magnitude) - 2), values are rounded to nearest even and saturated at 6 times the scale; a block
     that holds an infinity or a NaN gets the scale NaN (255)."""
 
-    if x.dtype not in _TYPES:
-        raise ValueError("quantize: x must be bf16, fp16 or fp32")
-    if x.dim() < 1 or x.shape[-1] % BLOCK:
-        raise ValueError(f"quantize: rows of x must be whole blocks of {BLOCK}")
-    stream = _lib.stream_of(x)
-    k = x.shape[-1]
-    words = torch.empty((*x.shape[:-1], k // 8), dtype=torch.int32, device=x.device)
-    scales = torch.empty((*x.shape[:-1], k // BLOCK), dtype=torch.uint8, device=x.device)
-    if x.numel() == 0:
-        return words, scales
-    rows = x if x.dim() == 2 else x.reshape(-1, k)
-    if rows.stride(1) != 1 or (rows.shape[0] > 1 and (rows.stride(0) * x.element_size() % 16 or rows.stride(0) < k)) or rows.data_ptr() % 16:
-        rows = rows.clone(memory_format=torch.contiguous_format)
-    _lib.native().tf_mx_quantize("quantize", rows, max(rows.stride(0), k), _TYPES[x.dtype], rows.shape[0], k, words, scales, stream)
-    return words, scales
+    return _lib.native().mx_quantize(x)
 
 
 def dequantize(words: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that ``quantize``'s words and scales stand for (exact in fp32, and in bf16 below 2^128)."""
 
-    k = _check_stored(words, scales, "dequantize")
     if dtype not in _TYPES:
         raise ValueError("dequantize: bf16, fp16 or fp32")
-    stream = _lib.stream_of(words)
-    out = torch.empty((*words.shape[:-1], k), dtype=dtype, device=words.device)
-    if out.numel():
-        _lib.native().tf_mx_dequantize("dequantize", words.contiguous(), scales.contiguous(), out.numel() // k, k, _TYPES[dtype], out, stream)
-    return out
+    return _lib.native().mx_dequantize(words, scales, _TYPES[dtype])
 
 
 @lru_cache(maxsize=None)
@@ -143,41 +124,13 @@ def _packed(q: MX4, who: str) -> torch.Tensor:
     return w
 
 
-def _rows(x: torch.Tensor, k: int, who: str) -> torch.Tensor:
-    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != k:
-        raise ValueError(f"{who}: x must be (M, {k}) bf16")
-    if x.shape[0] < 1:
-        raise ValueError(f"{who}: x needs at least one row")
-    if x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < k)) or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _matmul(x, q, act, limit, f32, out, pdl, who):
-    x = _rows(x, q.k, who)
-    stream = _lib.stream_of(x)
-    if q.weight.device != x.device:
-        raise ValueError(f"{who}: x and the weight must share a CUDA device")
-    m, cols = x.shape[0], q.n // 2 if act == "swiglu" else q.n
-    dtype = torch.float32 if f32 else torch.bfloat16
-    if out is None:
-        out = torch.empty((m, cols), dtype=dtype, device=x.device)
-    elif out.shape != (m, cols) or out.dtype != dtype or out.stride(1) != 1 or (m > 1 and out.stride(0) < cols) or out.device != x.device:
-        raise ValueError(f"{who}: out must be (M, n) of the requested dtype with unit-stride rows on x's device")
-    need = _lib.lib().tf_mx_matmul_bytes(m, q.n, q.k)
-    work = torch.empty((need,), dtype=torch.uint8, device=x.device) if need > 0 else None
-    _lib.native().tf_mx_matmul(who, x, max(x.stride(0), q.k), m, _packed(q, who), q.n, q.k, out, max(out.stride(0), cols), f32,
-                               _EPILOGUES[act], limit, work, need, pdl, stream)
-    return out
-
-
 def matmul(x: torch.Tensor, q: MX4, *, f32: bool = False, out: torch.Tensor | None = None, pdl: bool = False) -> torch.Tensor:
     """x (M, k) bf16, quantised as by ``quantize``, times q.T as (M, n) bf16, or unrounded fp32 with ``f32``.
 
     ``pdl`` launches with programmatic stream serialisation so that the weights' first bytes overlap the end of the previous
     kernel in the stream: they must not be what a kernel still in flight writes."""
 
-    return _matmul(x, q, None, 0.0, f32, out, pdl, "matmul")
+    return _lib.native().mx_matmul(x, q, 0, 0.0, f32, out, pdl)
 
 
 def matmul_act(x: torch.Tensor, q: MX4, *, act: str = "swiglu", limit: float = 0.0, out: torch.Tensor | None = None,
@@ -187,6 +140,4 @@ def matmul_act(x: torch.Tensor, q: MX4, *, act: str = "swiglu", limit: float = 0
 
     if act not in ("swiglu", "relu2"):
         raise ValueError("matmul_act: act is 'swiglu' or 'relu2'")
-    if act == "swiglu" and q.n % 32:
-        raise ValueError("matmul_act: swiglu takes a pack_pair weight")
-    return _matmul(x, q, act, limit, False, out, pdl, "matmul_act")
+    return _lib.native().mx_matmul(x, q, _EPILOGUES[act], limit, False, out, pdl)

@@ -55,7 +55,9 @@ struct MxParams {
   const uint8_t* w;
   int64_t sb_bytes, expert_stride;
   int N, M, K, steps, stages;
-  int sk, cluster;
+  int cluster;                  // blocks that share a tile, a K slice each (1: every block runs all slices)
+  int sk;
+  int bounds[MX_CLUSTER_MAX + 1];   // slice s holds stages bounds[s] .. bounds[s + 1]
   int ring;                     // slots
   int bufs;                     // FUSED: operands held in shared memory (2 with a plan, room permitting)
   int operand_stages;           // FUSED: stages of the longest slice
@@ -66,7 +68,7 @@ struct MxParams {
   const __nv_bfloat16* x;
   int64_t ldx;
   int slots;                    // FUSED with a plan: rows of x are pair / slots (0: the pair itself)
-  int tile;                     // rows of a tile
+  int tile, row_tiles;          // rows of a tile; tiles of rows (dense form)
   void* out;
   int64_t ldo;
   int out_f32, epi;
@@ -194,7 +196,16 @@ struct MxShape {
   static constexpr int RING = (TMEM - 2 * NT) / SF_COLS < MX_RING_MAX ? (TMEM - 2 * NT) / SF_COLS : MX_RING_MAX;
 };
 
-template <int NT, bool FUSED>
+// Stages of a block in order: a ring slot, and the parity of its barriers.
+struct Ring {
+  int slot;
+  uint32_t phase;
+  __device__ __forceinline__ void next(int ring) {
+    if (++slot == ring) slot = 0, phase ^= 1u;
+  }
+};
+
+template <int NT, bool FUSED, bool GROUPED>
 __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
   using S = MxShape<NT, FUSED>;
   extern __shared__ uint8_t smem_raw[];
@@ -203,20 +214,26 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
   uint64_t* empty = full + MX_RING_MAX;                            // [MX_RING_MAX] the MMAs that read the slot are done
   uint64_t* acc_full = empty + MX_RING_MAX;                        // [2]
   uint64_t* acc_empty = acc_full + 2;                              // [2]
-  uint64_t* op_full = acc_empty + 2;                               // [2] FUSED: an operand is quantised
+  uint64_t* op_full = acc_empty + 2;                               // [2] FUSED with a plan: an operand is quantised
   uint64_t* op_empty = op_full + 2;                                // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(op_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t ring0 = smem_addr(smem) + MX_BAR_BYTES;           // slots, FUSED operands, then the exchange buffers
   const uint32_t operand0 = ring0 + p.ring * S::SLOT;
   const uint32_t operand_bytes = FUSED ? p.operand_stages * S::B_BYTES : 0;
-  const uint32_t extra_off = MX_BAR_BYTES + p.ring * S::SLOT + p.bufs * operand_bytes;
+  const uint32_t extra_off = MX_BAR_BYTES + p.ring * S::SLOT + (FUSED ? p.bufs * operand_bytes : 0);
   const uint32_t abort_word = smem_addr(const_cast<int*>(abort_flag));
+  const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty), acc_full32 = smem_addr(acc_full), acc_empty32 = smem_addr(acc_empty);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-  const bool grouped = p.items != nullptr;
-  const int c = p.cluster, rank = c > 1 ? static_cast<int>(blockIdx.x % c) : 0;
+  const int c = GROUPED ? 1 : p.cluster;
   const int full_stages = p.steps >> 2, tail = p.steps & 3;
+  uint32_t rank, mine, clusters;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(mine));
+  asm("mov.u32 %0, %%nclusterid.x;" : "=r"(clusters));
+  const int slice0 = c > 1 ? rank : 0, slice1 = c > 1 ? rank + 1 : p.sk;
+  const int u0 = p.bounds[slice0], u1 = p.bounds[slice1];          // this block's stages of a tile
 
   auto give_up = [&](int code) {
     if (lane == 0) {
@@ -224,55 +241,34 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       atomicCAS(p.err, 0, code);
     }
   };
+  auto lost = [&](int code) {                                      // one thread gave up
+    *abort_flag = code;
+    atomicCAS(p.err, 0, code);
+  };
 
-  if (tid == 0) {
-    for (int i = 0; i < MX_RING_MAX; ++i) mbar_init(full + i, FUSED ? 1 : 2), mbar_init(empty + i, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, 4 * S::GROUPS);
-      mbar_init(op_full + i, grouped ? 4 : 8), mbar_init(op_empty + i, 1);
-    }
-    *abort_flag = 0;
-    mbar_fence_init();
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  if (c > 1) cluster_barrier();                                    // the other blocks run before anything is sent to them
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
-  pdl_launch_dependents();
-  if (grouped) pdl_wait();                                         // the plan may be the previous kernel's output
-
-  // Tiles: (row tile or item) x 128 columns, columns fastest.  A cluster takes every gridDim / c-th tile; FUSED with a plan a run
-  // of neighbours, so that its rows are quantised once an item.
+  // Tiles: (row tile or item) x 128 columns, columns fastest.  A cluster takes every clusters-th tile; FUSED with a plan a run of
+  // neighbours, so that its rows are quantised once an item.
+  if (GROUPED) pdl_wait();                                         // the plan may be the previous kernel's output
+  constexpr bool RUNS = FUSED && GROUPED;
   const int ncb = (p.N + MX_SB - 1) / MX_SB;
-  const int row_tiles = grouped ? min(p.counts[0], p.max_items) : (p.M + p.tile - 1) / p.tile;
-  const int tiles = ncb * row_tiles, mine = blockIdx.x / c, clusters = gridDim.x / c;
-  const bool runs = FUSED && grouped;
-  const int first_tile = runs ? static_cast<int>(static_cast<int64_t>(tiles) * mine / clusters) : mine;
-  const int tile_step = runs ? 1 : clusters;
-  const int my_tiles = runs ? static_cast<int>(static_cast<int64_t>(tiles) * (mine + 1) / clusters) - first_tile
-                            : (mine < tiles ? (tiles - mine + clusters - 1) / clusters : 0);
-  const int slice0 = c > 1 ? rank : 0, slice1 = c > 1 ? rank + 1 : p.sk;
+  const int tiles = ncb * (GROUPED ? min(p.counts[0], p.max_items) : p.row_tiles);
+  const int first_tile = RUNS ? static_cast<int>(static_cast<int64_t>(tiles) * mine / clusters) : mine;
+  const int end_tile = RUNS ? static_cast<int>(static_cast<int64_t>(tiles) * (mine + 1) / clusters) : tiles;
+  const int tile_step = RUNS ? 1 : clusters;
 
   struct Tile {
+    int t;                                                         // number of the tile
     int y, cb, m0, rows, n;                                        // item or row tile, column block, first row (or member), rows, MMA N
     int64_t w;                                                     // offset of the weights
   };
-  auto tile_at = [&](int it) {
-    const int t = first_tile + it * tile_step;
-    Tile ti;
-    ti.y = t / ncb, ti.cb = t - ti.y * ncb;
+  auto fill = [&](Tile& ti) {
+    if (ti.t >= end_tile) return;
     ti.w = ti.cb * p.sb_bytes;
-    if (grouped) {
+    if (GROUPED) {
       const int* item = p.items + 3 * ti.y;
       const int expert = __ldg(item);
-      // an item that names an expert outside the table runs against expert 0 with no rows and is reported
+      // an item that names an expert outside the table runs against expert 0 with no rows (the weights' thread reports it)
       const bool known = expert >= 0 && expert < p.experts;
-      if (!known && threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BAD_ITEM);
       ti.w += (known ? expert : 0) * p.expert_stride;
       ti.m0 = __ldg(item + 1);
       ti.rows = known ? min(p.tile, __ldg(item + 2)) : 0;
@@ -282,61 +278,147 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       ti.rows = min(p.tile, p.M - ti.m0);
     }
     ti.n = max(8, (ti.rows + 7) & ~7);
+  };
+  auto first = [&]() {
+    Tile ti = {};
+    ti.t = first_tile;
+    ti.y = FUSED && !GROUPED ? 0 : first_tile / ncb, ti.cb = first_tile - ti.y * ncb;
+    fill(ti);
     return ti;
   };
-  auto slice_at = [&](int s) { return p.sk == 1 ? s * p.stages : p.stages * s / p.sk; };
+  auto next = [&](Tile& ti) {
+    ti.t += tile_step, ti.cb += tile_step;
+    if (!FUSED || GROUPED)
+      while (ti.cb >= ncb) ti.cb -= ncb, ++ti.y;
+    fill(ti);
+  };
 
-  // Stages of the block in order: a ring slot, and the parity of its barriers.
-  struct Ring {
-    int slot;
-    uint32_t phase;
-    __device__ __forceinline__ void next(int ring) {
-      if (++slot == ring) slot = 0, phase ^= 1u;
+  // The weights' thread: the first slots are filled before the block's set-up is complete (nothing has to be free for them).
+  const uint32_t last_bytes = tail * 4096 + mx_tail_scales(tail);
+  Ring wr = {0, 1u};
+  uint32_t w_ready = 1u;
+  Tile wt = {};
+  int wu = u0;
+  bool w_ok = true;
+  auto load_weights = [&](int stages) {
+    while (stages-- > 0 && wt.t < end_tile) {
+      if (!w_ready && !(w_ok = lane_wait(empty32 + 8 * wr.slot, wr.phase, abort_word))) return;
+      const uint32_t bar = full32 + 8 * wr.slot, dst = ring0 + wr.slot * S::SLOT, bytes = wu < full_stages ? MX_UNIT : last_bytes;
+      wr.next(p.ring);
+      w_ready = lane_test(empty32 + 8 * wr.slot, wr.phase);
+      mbar32_expect_tx(bar, bytes);
+      bulk_load32(dst, p.w + wt.w + static_cast<int64_t>(wu) * MX_UNIT, bytes, bar);
+      if (++wu == u1) {
+        wu = u0;
+        next(wt);
+      }
     }
   };
-  auto lost = [&](int code) {                                      // one thread gave up
-    *abort_flag = code;
-    atomicCAS(p.err, 0, code);
+
+  // Rows w, w + stride, ... of `segments` runs of 1024 inputs each, quantised into the operand at `base`; four 16-byte loads a lane, the
+  // next run's in flight meanwhile.  `row_at`: the row of x behind row r of the tile, below 0 for none.
+  auto quantize_rows = [&](uint8_t* base, int rows, int w, int stride, auto&& row_at) {
+    const int p0 = u0 * 32, pieces = min(p.steps * 8, u1 * 32) - p0;   // 16-byte pieces of a row in this slice (K padded to 64)
+    const int segments = (pieces + 127) >> 7;
+    int r = 0, seg = w;
+    auto settle = [&]() {
+      while (seg >= segments) seg -= segments, ++r;
+    };
+    auto fetch = [&](uint4 (&v4)[4]) {
+      const int64_t row = row_at(r);
+      const uint4* from = reinterpret_cast<const uint4*>(p.x + row * p.ldx) + p0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int q = seg * 128 + 32 * j + lane;
+        v4[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (row >= 0 && q < pieces && (p0 + q) * 8 < p.K) v4[j] = from[q];
+      }
+    };
+    settle();
+    uint4 ahead[4];
+    if (r < rows) fetch(ahead);
+    while (r < rows) {
+      const int at_r = r, q0 = seg * 128 + lane;
+      uint4 v4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v4[j] = ahead[j];
+      seg += stride;
+      settle();
+      if (r < rows) fetch(ahead);
+      uint32_t codes[4], scale[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v[8];
+        widen8(v4[j], v);
+        codes[j] = quantize_block(v, scale[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int q = q0 + 32 * j, b = q >> 2, u = b >> 3;
+        if (q < pieces) {
+          uint8_t* stage = base + u * S::B_BYTES;
+          const uint32_t at = u0 + u < full_stages
+                                  ? (at_r >> 3) * 1024 + (at_r & 7) * 128 + (((b & 7) ^ (at_r & 7)) << 4)
+                                  : ((b & 7) >> 1) * (NT * 32) + (at_r >> 3) * 256 + (at_r & 7) * 32 + (((b & 1) ^ ((at_r >> 2) & 1)) << 4);
+          *reinterpret_cast<uint32_t*>(stage + at + 4 * (q & 3)) = codes[j];
+          if ((q & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + at_r * 16 + (b & 3)] = static_cast<uint8_t>(scale[j]);
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   };
 
   if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < MX_RING_MAX; ++i) mbar_init(full + i, FUSED ? 1 : 2), mbar_init(empty + i, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, 4 * S::GROUPS);
+        mbar_init(op_full + i, 4), mbar_init(op_empty + i, 1);
+      }
+      *abort_flag = 0;
+      mbar_fence_init();
+      wt = first();
+      load_weights(p.ring);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (FUSED && !GROUPED && warp >= 4) {
+    // every tile has the same rows: all eight warps quantise them, beside the set-up
+    pdl_wait();
+    quantize_rows(smem + (operand0 - smem_addr(smem)), p.M, warp - 4, 8, [](int r) { return static_cast<int64_t>(r); });
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (c > 1) cluster_barrier();                                    // the other blocks run before anything is sent to them
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+  pdl_launch_dependents();
+
+  if (warp == 0) {
     // ------------------------------------------------------------------ weights
-    if (elect_lane()) {
-      const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty);
-      const uint32_t last_bytes = tail * 4096 + mx_tail_scales(tail);
-      bool ok = true;
-      Ring r = {0, 1u};
-      uint32_t ready = 1u;                                         // (a fresh slot's test passes)
-      for (int it = 0; it < my_tiles && ok; ++it) {
-        const Tile ti = tile_at(it);
-        const int u0 = slice_at(slice0), u1 = slice_at(slice1);
-        const uint8_t* src = p.w + ti.w + static_cast<int64_t>(u0) * MX_UNIT;
-#pragma unroll 1
-        for (int u = u0; u < u1; ++u, src += MX_UNIT) {
-          if (!ready && !(ok = lane_wait(empty32 + 8 * r.slot, r.phase, abort_word))) break;
-          const uint32_t bar = full32 + 8 * r.slot, dst = ring0 + r.slot * S::SLOT;
-          r.next(p.ring);
-          ready = lane_test(empty32 + 8 * r.slot, r.phase);
-          const uint32_t bytes = u < full_stages ? MX_UNIT : last_bytes;
-          mbar32_expect_tx(bar, bytes);
-          bulk_load32(dst, src, bytes, bar);
+    if (lane == 0) {
+      load_weights(INT32_MAX);
+      if (!w_ok) lost(ERR_WAIT_EMPTY), let_copies_land();
+      if (GROUPED) {
+        for (Tile ti = first(); ti.t < end_tile; next(ti)) {
+          const int expert = __ldg(p.items + 3 * ti.y);
+          if (expert < 0 || expert >= p.experts) atomicCAS(p.err, 0, ERR_BAD_ITEM);
         }
       }
-      if (!ok) lost(ERR_WAIT_EMPTY), let_copies_land();
     }
     __syncwarp();
   } else if (warp == 2 && !FUSED) {
     // ------------------------------------------------------------------ quantised rows
     pdl_wait();
     if (elect_lane()) {
-      const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty);
       const int64_t stage_bytes = mx_stage_bytes(p.b_rows);
       bool ok = true;
       Ring r = {0, 1u};
-      uint32_t ready = 1u;
-      for (int it = 0; it < my_tiles && ok; ++it) {
-        const Tile ti = tile_at(it);
-        const int sbs = mx_scale_blocks(ti.n), u0 = slice_at(slice0), u1 = slice_at(slice1);
+      uint32_t ready = 1u;                                         // (a fresh slot's test passes)
+      for (Tile ti = first(); ti.t < end_tile && ok; next(ti)) {
+        const int sbs = mx_scale_blocks(ti.n);
         const uint8_t* src = p.b + ti.y * p.item_stride + u0 * stage_bytes;
 #pragma unroll 1
         for (int u = u0; u < u1; ++u, src += stage_bytes) {
@@ -366,35 +448,31 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     // thread beyond them shows: descriptors are kept to adds, the next stage's barrier is tested before this stage's MMAs, and
     // the last stage, whose steps are regions of their own, has code of its own.
     if (elect_lane()) {
-      const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty), acc_full32 = smem_addr(acc_full), acc_empty32 = smem_addr(acc_empty);
       const uint32_t sf0 = tmem + 2 * NT;
       const uint64_t a0 = desc(ring0, 1024, SWIZZLE_128), as0 = desc(ring0 + MX_SB * 128, 128, SWIZZLE_NONE);
       const uint64_t b0 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 1024, SWIZZLE_128);
       const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + NT * 128, 128, SWIZZLE_NONE);
       bool ok = true;
       Ring r = {0, 0u};
-      int use = 0, op = -1, last_y = -1;
+      int use = 0, op = GROUPED ? -1 : 0, last_y = -1;
       uint32_t ready = 0;
-      for (int it = 0; it < my_tiles && ok; ++it) {
-        const Tile ti = tile_at(it);
-        bool last_of_op = false;
-        if (FUSED) {
-          const bool new_op = grouped ? ti.y != last_y : it == 0;
-          last_y = ti.y;
-          if (new_op) {
-            ++op;
-            if (!(ok = lane_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word))) break;
-          }
-          last_of_op = grouped && (it + 1 == my_tiles || (first_tile + it + 1) / ncb != ti.y);
+      for (Tile ti = first(); ti.t < end_tile && ok;) {
+        const int n = ti.n, y = ti.y;
+        next(ti);
+        if (RUNS && y != last_y) {
+          last_y = y;
+          ++op;
+          if (!(ok = lane_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word))) break;
         }
-        const uint32_t id0 = instruction(ti.n, 0), id1 = instruction(ti.n, 1);
+        const int buf = RUNS ? op % p.bufs : 0;
+        const uint32_t id0 = instruction(n, 0), id1 = instruction(n, 1);
         for (int s = slice0; s < slice1 && ok; ++s, ++use) {
-          const int start = slice_at(s), end = slice_at(s + 1), last_whole = min(end, full_stages);
+          const int start = p.bounds[s], end = p.bounds[s + 1], last_whole = min(end, full_stages);
           if (use >= 2 && !(ok = lane_wait(acc_empty32 + 8 * (use & 1), ((use >> 1) - 1) & 1, abort_word))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t d = tmem + (use & 1) * NT;
           uint32_t more = 0;                                         // 0: the first step of the slice overwrites the accumulator
-          uint32_t fused_at = FUSED ? (op % p.bufs) * (operand_bytes >> 4) : 0;
+          uint32_t fused_at = FUSED ? buf * (operand_bytes >> 4) : 0;
 #pragma unroll 1
           for (int u = start; u < last_whole; ++u) {
             if (!ready && !(ok = lane_wait(full32 + 8 * r.slot, r.phase, abort_word))) break;
@@ -436,284 +514,255 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
             ready = 0;
           }
           commit(acc_full32 + 8 * (use & 1));
-          if (FUSED && last_of_op && s + 1 == slice1) commit(smem_addr(op_empty + op % p.bufs));
         }
+        if (RUNS && ok && (ti.t >= end_tile || ti.y != y)) commit(smem_addr(op_empty + buf));
       }
       if (!ok) lost(ERR_WAIT_FULL);
     }
     __syncwarp();
-  }
-
-  if (FUSED && (grouped ? warp >= 8 : warp >= 4)) {
-    // ------------------------------------------------------------------ bf16 rows -> operand in shared memory
-    // Four lanes a block as everywhere; a thread has four 16-byte loads in flight.
-    if (!grouped) pdl_wait();
-    const int qt = grouped ? tid - 256 : tid - 128, qthreads = grouped ? 128 : 256;
+  } else if (RUNS && warp >= 8) {
+    // ------------------------------------------------------------------ bf16 rows of an item -> operand in shared memory
     bool ok = true;
     int op = -1, last_y = -1;
-    const int u0 = slice_at(slice0), u1 = slice_at(slice1);
-    const int p0 = u0 * 32, pieces = min(p.steps * 8, u1 * 32) - p0;   // 16-byte pieces of a row in this slice (K padded to 64)
-    for (int it = 0; it < my_tiles && ok; ++it) {
-      const Tile ti = tile_at(it);
-      if (grouped ? ti.y == last_y : it > 0) continue;
+    for (Tile ti = first(); ti.t < end_tile; next(ti)) {
+      if (ti.y == last_y) continue;
       last_y = ti.y;
       ++op;
-      if (op >= p.bufs) {
-        ok = warp_wait(smem_addr(op_empty + op % p.bufs), (op / p.bufs - 1) & 1, abort_word);
-        if (!ok) break;
-      }
-      uint8_t* base = smem + (operand0 - smem_addr(smem)) + (op % p.bufs) * operand_bytes;
-      // a warp takes segments of 1024 inputs of a row, four 16-byte loads a lane; the next segment's are in flight meanwhile
-      const int segments = (pieces + 127) >> 7, total = ti.rows * segments, stride = qthreads >> 5;
-      auto fetch = [&](int w, uint4 (&v4)[4]) {
-        const int r = w / segments, q0 = (w - r * segments) * 128 + lane;
-        int64_t row = r;
-        bool live = true;
-        if (grouped) {
-          const int pair = p.members[ti.m0 + r];
-          live = pair >= 0 && pair < p.pairs;
-          row = p.slots > 0 ? pair / p.slots : pair;
-        }
-        const uint4* from = reinterpret_cast<const uint4*>(p.x + row * p.ldx) + p0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int q = q0 + 32 * j;
-          v4[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (live && q < pieces && (p0 + q) * 8 < p.K) v4[j] = from[q];
-        }
-      };
-      uint4 next[4];
-      if ((qt >> 5) < total) fetch(qt >> 5, next);
-      for (int w = qt >> 5; w < total; w += stride) {
-        const int r = w / segments, q0 = (w - r * segments) * 128 + lane;
-        uint4 v4[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v4[j] = next[j];
-        if (w + stride < total) fetch(w + stride, next);
-        uint32_t codes[4], scale[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v[8];
-          widen8(v4[j], v);
-          codes[j] = quantize_block(v, scale[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int q = q0 + 32 * j, b = q >> 2, u = b >> 3;
-          if (q < pieces) {
-            uint8_t* stage = base + u * S::B_BYTES;
-            const uint32_t at = u0 + u < full_stages ? (r >> 3) * 1024 + (r & 7) * 128 + (((b & 7) ^ (r & 7)) << 4)
-                                                     : ((b & 7) >> 1) * (NT * 32) + (r >> 3) * 256 + (r & 7) * 32 + (((b & 1) ^ ((r >> 2) & 1)) << 4);
-            *reinterpret_cast<uint32_t*>(stage + at + 4 * (q & 3)) = codes[j];
-            if ((q & 3) == 0) stage[NT * 128 + ((b & 7) >> 2) * 512 + r * 16 + (b & 3)] = static_cast<uint8_t>(scale[j]);
-          }
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (op >= p.bufs && !(ok = warp_wait(smem_addr(op_empty + op % p.bufs), (op / p.bufs - 1) & 1, abort_word))) break;
+      quantize_rows(smem + (operand0 - smem_addr(smem)) + (op % p.bufs) * operand_bytes, ti.rows, warp - 8, 4, [&](int r) -> int64_t {
+        const int pair = p.members[ti.m0 + r];
+        return pair < 0 || pair >= p.pairs ? -1 : p.slots > 0 ? pair / p.slots : pair;
+      });
       __syncwarp();
       if (lane == 0) mbar_arrive(op_full + op % p.bufs);
     }
     if (!ok) give_up(ERR_WAIT_EMPTY);
   }
 
-  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 unless they quantise)
+  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 where tiles are taller)
   const bool drains = warp >= 4 && group < S::GROUPS;
-  const int lg = warp & 3;
-  const int ncols = p.epi == MX_SWIGLU ? p.N / 2 : p.N;
-  const bool wide = !p.out_f32 && (ncols & 7) == 0 && (p.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-  auto row_of = [&](const Tile& ti, int n) -> int64_t {              // the output row of row n of the tile; below 0: none
-    if (n >= ti.rows) return -1;
-    if (!grouped) return ti.m0 + n;
-    const int pair = p.members[ti.m0 + n];
-    return pair < p.pairs ? pair : -1;
-  };
-  // v[j] = row n + j of the tile in output column `col`, a lane a column
-  auto store8 = [&](const Tile& ti, const float* v, int n, int col) {
-    if (wide) {
-      const float t[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-      const uint4 o = transpose8(t, lane);                           // columns col - l8 .. col - l8 + 7 of row n + l8
-      const int64_t row = row_of(ti, n + (lane & 7));
-      if (row >= 0 && col < ncols) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + (col - (lane & 7))) = o;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t row = row_of(ti, n + j);
-        if (row < 0 || col >= ncols) continue;
-        if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + col] = v[j];
-        else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + col] = __float2bfloat16_rn(v[j]);
-      }
-    }
-  };
-  // Activations of sixteen rows.  SwiGLU: gate in lanes 0-15, up in lanes 16-31 of the same outputs; the lower lanes come out with
-  // rows 0-7 in v[0..7], the upper ones with rows 8-15.
-  auto activate = [&](float* v) {
-    if (p.epi == MX_SWIGLU) {
-      const bool low = lane < 16;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v[8 + j] : v[j], 16);
-        v[j] = swiglu(low ? v[j] : got, low ? got : v[8 + j], p.limit);
-      }
-    } else if (p.epi == MX_RELU2) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float u = v[j] < 0.f ? 0.f : v[j];
-        v[j] = u * u;
-      }
-    }
-  };
-  auto finish16 = [&](const Tile& ti, float* v, int n) {
-    activate(v);
-    if (p.epi == MX_SWIGLU) {
-      store8(ti, v, n + (lane < 16 ? 0 : 8), ti.cb * 64 + lg * 16 + (lane & 15));
-    } else {
-      const int col = ti.cb * MX_SB + lg * 32 + lane;
-      store8(ti, v, n, col);
-      if (n + 8 < ti.rows) store8(ti, v + 8, n + 8, col);
-    }
-  };
-  // The same, quantised: through shared memory, where four lanes see a block.
-  auto quantize16 = [&](const Tile& ti, float* v, int n) {
-    constexpr int LINE = MX_QUANT_COLS + 4;
-    const int width = p.epi == MX_SWIGLU ? 64 : 128;
-    float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES);
-    uint8_t* op = p.q + ti.y * p.q_item_stride;
-    activate(v);
-    named_barrier(1 + group, 128);                                   // the last sixteen rows have been read
-    if (p.epi == MX_SWIGLU) {
-      float* to = rows + (lane < 16 ? 0 : 8) * LINE + lg * 16 + (lane & 15);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) to[j * LINE] = v[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) rows[j * LINE + lg * 32 + lane] = v[j];
-    }
-    named_barrier(1 + group, 128);
-    for (int t = lg * 32 + lane; t < MX_QUANT_ROWS * width / 8; t += 128) {
-      const int r = t / (width / 8), piece = t - r * (width / 8);
-      const float4* from = reinterpret_cast<const float4*>(rows + r * LINE + piece * 8);
-      const float4 lo = from[0], hi = from[1];
-      float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      uint32_t scale;
-      const uint32_t codes = quantize_block(w, scale);
-      const int b = ti.cb * (width / 32) + (piece >> 2);
-      if (n + r < ti.rows && b < 2 * p.q_steps) {
-        *reinterpret_cast<uint32_t*>(op + mx_code_offset(p.q_rows, p.q_steps, n + r, b) + 4 * (piece & 3)) = codes;
-        if ((piece & 3) == 0) op[mx_scale_offset(p.q_rows, p.q_steps, n + r, b)] = static_cast<uint8_t>(scale);
-      }
-    }
-  };
+  if (c > 1 && !drains) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   if (drains) {
     // ------------------------------------------------------------------ drain
+    const int lg = warp & 3;
+    const bool gated = p.epi == MX_SWIGLU;
+    const int ncols = gated ? p.N / 2 : p.N;
+    const bool wide = !p.out_f32 && (ncols & 7) == 0 && (p.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+    auto row_of = [&](const Tile& ti, int n) -> int64_t {            // the output row of row n of the tile; below 0: none
+      if (n >= ti.rows) return -1;
+      if (!GROUPED) return ti.m0 + n;
+      const int pair = p.members[ti.m0 + n];
+      return pair < p.pairs ? pair : -1;
+    };
+    // v[j] = row n + j of the tile in output column `col`, a lane a column
+    auto store8 = [&](const Tile& ti, const float* v, int n, int col) {
+      if (wide) {
+        const float t[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+        const uint4 o = transpose8(t, lane);                         // columns col - l8 .. col - l8 + 7 of row n + l8
+        const int64_t row = row_of(ti, n + (lane & 7));
+        if (row >= 0 && col < ncols) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + (col - (lane & 7))) = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int64_t row = row_of(ti, n + j);
+          if (row < 0 || col >= ncols) continue;
+          if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + col] = v[j];
+          else static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + col] = __float2bfloat16_rn(v[j]);
+        }
+      }
+    };
+    // Activations of sixteen rows.  SwiGLU: gate in lanes 0-15, up in lanes 16-31 of the same outputs; the lower lanes come out
+    // with rows 0-7 in v[0..7], the upper ones with rows 8-15.
+    auto activate = [&](float* v) {
+      if (gated) {
+        const bool low = lane < 16;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v[8 + j] : v[j], 16);
+          v[j] = swiglu(low ? v[j] : got, low ? got : v[8 + j], p.limit);
+        }
+      } else if (p.epi == MX_RELU2) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float u = v[j] < 0.f ? 0.f : v[j];
+          v[j] = u * u;
+        }
+      }
+    };
+    // Sixteen rows of activations to the next projection's operand: through shared memory, where four lanes see a block.
+    auto quantize16 = [&](const Tile& ti, const float* v, int n) {
+      constexpr int LINE = MX_QUANT_COLS + 4;
+      float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES);
+      const int shift = gated ? 3 : 4;                               // pieces of eight columns a row: 8 or 16
+      named_barrier(1 + group, 128);                                 // the last sixteen rows have been read
+      if (gated) {
+        float* to = rows + (lane < 16 ? 0 : 8) * LINE + lg * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j * LINE] = v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) rows[j * LINE + lg * 32 + lane] = v[j];
+      }
+      named_barrier(1 + group, 128);
+      // the tile's blocks lie in one stage of the operand
+      const int block0 = ti.cb << (shift - 2), u = block0 >> 3;
+      uint8_t* op = p.q + ti.y * p.q_item_stride + u * mx_stage_bytes(p.q_rows);
+      const bool whole = u < p.q_steps >> 2;
+      const int q_tail = p.q_steps & 3;
+      uint8_t* scales = op + (whole ? p.q_rows * 128 : p.q_rows * 32 * q_tail);
+      for (int t = lg * 32 + lane; t < MX_QUANT_ROWS << shift; t += 128) {
+        const int r = t >> shift, piece = t & ((1 << shift) - 1), row = n + r;
+        const float4* from = reinterpret_cast<const float4*>(rows + r * LINE + piece * 8);
+        const float4 lo = from[0], hi = from[1];
+        float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        uint32_t scale;
+        const uint32_t codes = quantize_block(w, scale);
+        const int b = (block0 & 7) + (piece >> 2);
+        if (row < ti.rows && 8 * u + b < 2 * p.q_steps) {
+          const int at = whole ? (row >> 3) * 1024 + (row & 7) * 128 + ((b ^ (row & 7)) << 4)
+                               : (b >> 1) * p.q_rows * 32 + (row >> 3) * 256 + (row & 7) * 32 + (((b & 1) ^ ((row >> 2) & 1)) << 4);
+          *reinterpret_cast<uint32_t*>(op + at + 4 * (piece & 3)) = codes;
+          if ((piece & 3) == 0) scales[(b >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(scale);
+        }
+      }
+    };
+
     // Sixteen rows at a time straight from tensor memory.  The loop is not unrolled and its body is kept small: unrolled over
-    // a tile (5900 instructions) the warps mostly waited for instructions, and a tile of 256 rows took 42 us.
-    pdl_wait();                                                      // nothing is written before the previous kernel is done
+    // a tile (5900 instructions) the warps mostly waited for instructions, and a tile of 256 rows took 42 us.  For the same reason
+    // it runs once over no rows before the first accumulator is ready: its instructions are at hand then.
     bool ok = true;
     int use = 0;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(lg * 32) << 16) + 16 * group;
-    for (int it = 0; it < my_tiles && ok; ++it) {
-      const Tile ti = tile_at(it);
-      if (slice1 - slice0 > 1) {
-        // slices are added in registers, and the sum goes back to where the last one came from
-        float acc[S::CHUNKS][16];
-        for (int s = slice0; s < slice1; ++s, ++use) {
-          ok = warp_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
-          if (!ok) break;
+    Tile ti = first();
+    const int here = ti.rows;
+    ti.rows = 0;
+    for (bool rehearsal = true; ti.t < end_tile && ok;) {
+      if (!rehearsal) {
+        if (slice1 - slice0 > 1) {
+          // slices are added in registers, and the sum goes back to where the last one came from
+          float acc[S::CHUNKS][16];
+          for (int s = slice0; s < slice1; ++s, ++use) {
+            ok = warp_wait(acc_full32 + 8 * (use & 1), (use >> 1) & 1, abort_word);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t src = lanes + (use & 1) * NT;
+#pragma unroll
+            for (int i = 0; i < S::CHUNKS; ++i) {
+              if (16 * (S::GROUPS * i + group) >= ti.rows) break;
+              float v[16];
+              tmem_load16(src + 16 * S::GROUPS * i, v);
+              tmem_loaded();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[i][j] = s == slice0 ? v[j] : acc[i][j] + v[j];
+              if (s + 1 == slice1) tmem_store16(src + 16 * S::GROUPS * i, acc[i]);
+            }
+            if (s + 1 == slice1) {
+              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+              break;                                                 // (the loop below ends this use of the accumulator)
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + (use & 1));
+          }
+        } else {
+          ok = warp_wait(acc_full32 + 8 * (use & 1), (use >> 1) & 1, abort_word);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t src = lanes + (use & 1) * NT;
-#pragma unroll
-          for (int i = 0; i < S::CHUNKS; ++i) {
-            if (16 * (S::GROUPS * i + group) >= ti.rows) break;
-            float v[16];
-            tmem_load16(src + 16 * S::GROUPS * i, v);
-            tmem_loaded();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[i][j] = s == slice0 ? v[j] : acc[i][j] + v[j];
-            if (s + 1 == slice1) tmem_store16(src + 16 * S::GROUPS * i, acc[i]);
-          }
-          if (s + 1 == slice1) {
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            break;                                                   // (the loop below ends this use of the accumulator)
-          }
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + (use & 1));
         }
-      } else {
-        ok = warp_wait(smem_addr(acc_full + (use & 1)), (use >> 1) & 1, abort_word);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (!ok) break;
       }
-      if (!ok) break;
       const uint32_t src = lanes + (use & 1) * NT;
-      float ahead[16];                                               // the next sixteen rows are on their way meanwhile
-      if (16 * group < ti.rows) tmem_load16(src, ahead);
+      const int share = quads_of(ti.rows, c);
+      int n0 = 0;                                                    // first row this block finishes
+      if (c > 1) {
+        // Part [slice][four rows of the owner][128 columns][4] goes to the shared memory of the block that owns the rows.  The
+        // host launches one tile a cluster; when the barrier opens every part has been sent (parts of blocks that gave up are missing,
+        // which the error word says).
+        const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 16;
 #pragma unroll 1
-      for (int i = 0; i < S::CHUNKS; ++i) {
-        const int n = 16 * (S::GROUPS * i + group);
-        if (n >= ti.rows) break;
-        float v[16];
-        tmem_loaded();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = ahead[j];
-        if (n + 16 * S::GROUPS < ti.rows) tmem_load16(src + 16 * S::GROUPS * (i + 1), ahead);
-        if (c > 1) {
-          // part [slice][four rows of the owner][128 columns][4] in the shared memory of the block that owns the rows
-          const int share = quads_of(ti.rows, c);
-          const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 16;
+        for (int n = 16 * group; n < ti.rows; n += 16 * S::GROUPS) {
+          float v[16];
+          tmem_load16(src + n - 16 * group, v);
+          tmem_loaded();
+          int owner = (n >> 2) / share, at = (n >> 2) - owner * share;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int quad = (n >> 2) + j, owner = quad / share;
-            if (4 * quad < ti.rows) store_remote(part + (rank * share + quad - owner * share) * (MX_SB * 16), owner, v + 4 * j);
+            if (n + 4 * j < ti.rows) store_remote(part + (rank * share + at) * (MX_SB * 16), owner, v + 4 * j);
+            if (++at == share) at = 0, ++owner;
           }
-        } else if (p.q != nullptr) {
-          quantize16(ti, v, n);
-        } else {
-          finish16(ti, v, n);
         }
+        if (!rehearsal) {
+          __syncwarp();
+          cluster_barrier();
+          if (*abort_flag != 0) break;
+        }
+        n0 = 4 * rank * share;
+      }
+      Tile own = ti;
+      if (c > 1) own.rows = min(ti.rows, n0 + 4 * share);
+      float ahead[16];                                               // the next sixteen rows are on their way meanwhile
+      if (c == 1 && (rehearsal || 16 * group < ti.rows)) tmem_load16(src, ahead);
+#pragma unroll 1
+      for (int n = n0 + 16 * group; n < own.rows || (rehearsal && n < n0 + 16 * S::GROUPS); n += 16 * S::GROUPS) {
+        float v[16];
+        if (c > 1) {
+          const float4* part = reinterpret_cast<const float4*>(smem + extra_off) + lg * 32 + lane;
+          const int i = (n - n0) >> 2;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0.f;
+#pragma unroll 1
+          for (int s = 0; s < c; ++s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {                            // (quads past the share are other parts' and are not stored)
+              const float4 a = part[(s * share + min(i + j, share - 1)) * MX_SB];
+              if (s == 0) {
+                v[4 * j] = a.x, v[4 * j + 1] = a.y, v[4 * j + 2] = a.z, v[4 * j + 3] = a.w;
+              } else {
+                v[4 * j] += a.x, v[4 * j + 1] += a.y, v[4 * j + 2] += a.z, v[4 * j + 3] += a.w;
+              }
+            }
+          }
+        } else {
+          tmem_loaded();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = ahead[j];
+          if (n + 16 * S::GROUPS < own.rows) tmem_load16(src + n + 16 * S::GROUPS - 16 * group, ahead);
+        }
+        activate(v);
+        if (GROUPED && p.q != nullptr) {
+          quantize16(own, v, n);
+        } else if (gated) {
+          store8(own, v, n + (lane < 16 ? 0 : 8), ti.cb * 64 + lg * 16 + (lane & 15));
+        } else {
+          const int col = ti.cb * MX_SB + lg * 32 + lane;
+          store8(own, v, n, col);
+          store8(own, v + 8, n + 8, col);
+        }
+      }
+      if (rehearsal) {
+        rehearsal = false;
+        ti.rows = here;
+        pdl_wait();                                                  // nothing is written before the previous kernel is done
+        continue;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty + (use & 1));
       ++use;
+      if (c > 1) break;                                              // (one tile a cluster)
+      next(ti);
     }
-    if (!ok) give_up(ERR_WAIT_FULL);
-  }
-
-  if (c > 1) {
-    // The host launches one tile a cluster: every block's part has been sent when this barrier opens (parts of blocks that
-    // gave up are missing, which the error word says).
-    __syncwarp();
-    cluster_barrier();
-    if (drains && my_tiles > 0 && *abort_flag == 0) {
-      Tile ti = tile_at(0);
-      const int share = quads_of(ti.rows, c), n0 = 4 * rank * share;
-      ti.rows = min(ti.rows, n0 + 4 * share);
-      const float4* part = reinterpret_cast<const float4*>(smem + extra_off) + lg * 32 + lane;
-#pragma unroll 1
-      for (int i = 4 * group; n0 + 4 * i < ti.rows; i += 4 * S::GROUPS) {
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {                                // (quads past the share read other parts and are not stored)
-          const float4 a = part[min(i + j, share - 1) * MX_SB];
-          v[4 * j] = a.x, v[4 * j + 1] = a.y, v[4 * j + 2] = a.z, v[4 * j + 3] = a.w;
-        }
-#pragma unroll 1
-        for (int s = 1; s < c; ++s) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 a = part[(s * share + min(i + j, share - 1)) * MX_SB];
-            v[4 * j] += a.x, v[4 * j + 1] += a.y, v[4 * j + 2] += a.z, v[4 * j + 3] += a.w;
-          }
-        }
-        finish16(ti, v, n0 + 4 * i);
-      }
+    if (!ok) {
+      give_up(ERR_WAIT_FULL);
+      if (c > 1) cluster_barrier();
     }
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (c > 1 && !drains) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if (warp == 1) {
+    __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
   }
@@ -737,7 +786,7 @@ int slices_for(int n, int k) {
   return std::max(1, std::min({MX_CLUSTER_MAX, 148 / std::min(blocks, 148), stages / 2}));
 }
 
-template <int NT, bool FUSED>
+template <int NT, bool FUSED, bool GROUPED>
 cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
   using S = MxShape<NT, FUSED>;
   int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
@@ -747,6 +796,7 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl
   const int room = MX_SMEM_MAX - extra - p.bufs * operand;
   p.ring = std::min(S::RING, room / S::SLOT);
   if (p.ring < 2) return cudaErrorInvalidConfiguration;              // (the callers' rules keep shapes that would not fit out)
+  for (int i = 0; i <= p.sk; ++i) p.bounds[i] = static_cast<int>(static_cast<int64_t>(p.stages) * i / p.sk);
   const int64_t most = std::max(1, sms / p.cluster);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.cluster > 1 ? tiles : std::min(tiles, most)) * p.cluster));
@@ -767,20 +817,24 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl
   }
   cfg.attrs = attrs;
   cfg.numAttrs = count;
-  return cudaLaunchKernelEx(&cfg, mx_kernel<NT, FUSED>, p);
+  return cudaLaunchKernelEx(&cfg, mx_kernel<NT, FUSED, GROUPED>, p);
 }
 
-template <int NT, bool FUSED>
+template <int NT, bool FUSED, bool GROUPED>
 cudaError_t configure() {
-  return cudaFuncSetAttribute(mx_kernel<NT, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  return cudaFuncSetAttribute(mx_kernel<NT, FUSED, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
 }
 
 // Rows come as operands: the kernel whose tiles hold `tile` rows.
-cudaError_t launch_rows(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
-  if (p.tile <= 16) return launch<16, false>(p, tiles, quant_out, sms, pdl, stream);
-  if (p.tile <= 64) return launch<64, false>(p, tiles, quant_out, sms, pdl, stream);
-  if (p.tile <= 128) return launch<128, false>(p, tiles, quant_out, sms, pdl, stream);
-  return launch<192, false>(p, tiles, quant_out, sms, pdl, stream);
+cudaError_t launch_rows(MxParams& p, int64_t tiles, int sms, bool pdl, cudaStream_t stream) {
+  if (p.tile <= 16) return launch<16, false, false>(p, tiles, false, sms, pdl, stream);
+  if (p.tile <= 64) return launch<64, false, false>(p, tiles, false, sms, pdl, stream);
+  if (p.tile <= 128) return launch<128, false, false>(p, tiles, false, sms, pdl, stream);
+  return launch<192, false, false>(p, tiles, false, sms, pdl, stream);
+}
+cudaError_t launch_items(MxParams& p, int64_t tiles, int sms, bool pdl, cudaStream_t stream) {
+  return p.tile <= 16 ? launch<16, false, true>(p, tiles, p.q != nullptr, sms, pdl, stream)
+                      : launch<128, false, true>(p, tiles, p.q != nullptr, sms, pdl, stream);
 }
 
 int round8(int m) { return (m + 7) / 8 * 8; }
@@ -830,11 +884,14 @@ bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 }  // namespace
 
 cudaError_t mx_configure(int device, int sms) {
-  cudaError_t e = configure<16, true>();
-  if (e == cudaSuccess) e = configure<16, false>();
-  if (e == cudaSuccess) e = configure<64, false>();
-  if (e == cudaSuccess) e = configure<128, false>();
-  if (e == cudaSuccess) e = configure<192, false>();
+  cudaError_t e = configure<16, true, false>();
+  if (e == cudaSuccess) e = configure<16, true, true>();
+  if (e == cudaSuccess) e = configure<16, false, false>();
+  if (e == cudaSuccess) e = configure<16, false, true>();
+  if (e == cudaSuccess) e = configure<64, false, false>();
+  if (e == cudaSuccess) e = configure<128, false, false>();
+  if (e == cudaSuccess) e = configure<128, false, true>();
+  if (e == cudaSuccess) e = configure<192, false, false>();
   if (e == cudaSuccess && device >= 0 && device < 64) g_mx_sms[device] = sms;
   return e;
 }
@@ -884,7 +941,8 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     p.tile = MX_FUSED_ROWS;
     p.cluster = p.sk;
     p.operand_stages = (p.stages + p.sk - 1) / p.sk;
-    e = launch<16, true>(p, ncb, false, sms, pdl != 0, s);
+    p.row_tiles = 1;
+    e = launch<16, true, false>(p, ncb, false, sms, pdl != 0, s);
   } else {
     const Tiling t = tiling_for(m, n, p.stages, p.sk);
     p.tile = p.b_rows = t.tile, p.cluster = t.cluster;
@@ -894,7 +952,8 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     e = mx_rows_launch(x, ldx, m, k, t.tile, t.tile, p.item_stride, nullptr, nullptr, nullptr, 0, 0, 0, work, pdl != 0, s);
     if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
     // the rows' kernel lets this one set up and fetch weights while it runs; the weights were settled before it started
-    e = launch_rows(p, ncb * row_tiles, false, sms, true, s);
+    p.row_tiles = static_cast<int>(row_tiles);
+    e = launch_rows(p, ncb * row_tiles, sms, true, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_matmul");
 }
@@ -951,7 +1010,7 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
   if (x && need == 0) {
     p.x = static_cast<const __nv_bfloat16*>(x), p.ldx = ldx, p.slots = slots;
     p.bufs = 2, p.operand_stages = p.stages;
-    e = launch<16, true>(p, tiles, out_operands != nullptr, sms, false, s);
+    e = launch<16, true, true>(p, tiles, out_operands != nullptr, sms, false, s);
   } else {
     if (x) {
       e = mx_rows_launch(x, ldx, 0, k, rows, tile, operand, items, counts, members, slots, pairs, max_items, work, false, s);
@@ -959,7 +1018,7 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
     }
     p.b = static_cast<const uint8_t*>(work), p.b_rows = rows, p.item_stride = operand;
     p.bufs = 1;
-    e = launch_rows(p, tiles, out_operands != nullptr, sms, x != nullptr, s);
+    e = launch_items(p, tiles, sms, x != nullptr, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_experts");
 }

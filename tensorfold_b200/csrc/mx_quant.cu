@@ -171,24 +171,18 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__
   }
 }
 
-// bf16 rows to the operand layout, an operand a tile of rows, a warp a segment of 1024 inputs of one row (four loads in flight a
-// lane).  With a plan, row r of item y is row members[first + r] / slots of x (members[first + r] itself with slots 0) and goes to
-// row r of operand y.
+// bf16 rows to the operand layout: operand y (blockIdx.y) holds `tile` rows, a warp a row and as many runs of 1024 inputs as gridDim.z
+// leaves it, four 16-byte loads in flight a lane.  With a plan, row r of item y is row members[first + r] / slots of x
+// (members[first + r] itself with slots 0).
 constexpr int ROWS_SEGMENT = 1024;
-__global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int m, int k, int steps, int rows,
-                                                   int segments, int tile, int64_t item_bytes, const int* __restrict__ items,
-                                                   const int* __restrict__ counts, const int* __restrict__ members, int slots, int pairs,
-                                                   uint8_t* __restrict__ out) {
+__global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int m, int k, int steps, int rows, int tile,
+                                                   int64_t item_bytes, const int* __restrict__ items, const int* __restrict__ counts,
+                                                   const int* __restrict__ members, int slots, int pairs, uint8_t* __restrict__ out) {
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  int row = static_cast<int>(w / segments);
-  const int seg = static_cast<int>(w - static_cast<int64_t>(row) * segments);
-  int64_t src = row;
-  const int y = row / tile;
-  row -= y * tile;
-  out += y * item_bytes;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), y = blockIdx.y;
+  int64_t src = static_cast<int64_t>(y) * tile + row;
+  if (row >= tile) return;
   if (items != nullptr) {
     if (y >= counts[0] || row >= items[3 * y + 2]) return;
     const int pos = items[3 * y + 1] + row;
@@ -199,23 +193,33 @@ __global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restri
   } else if (src >= m) {
     return;
   }
+  out += y * item_bytes;
   const uint4* from = reinterpret_cast<const uint4*>(x + src * ldx);
-  uint4 p[4];
+  const int64_t stage_bytes = mx_stage_bytes(rows);
+  const int full = steps >> 2, tail = steps & 3;
+  uint8_t* const line = out + (row >> 3) * 1024 + (row & 7) * 128;                  // of stage 0
+  uint8_t* const scale_line = out + rows * 128 + (row >> 7) * MX_SCALES + (row & 31) * 16 + ((row & 127) >> 5) * 4;
+  for (int at = blockIdx.z * (ROWS_SEGMENT / 8); at < steps * 8; at += gridDim.z * (ROWS_SEGMENT / 8)) {
+    uint4 p[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int piece = seg * (ROWS_SEGMENT / 8) + 32 * j + lane;
-    p[j] = piece * 8 < k ? from[piece] : make_uint4(0u, 0u, 0u, 0u);
-  }
+    for (int j = 0; j < 4; ++j) {
+      const int piece = at + 32 * j + lane;
+      p[j] = piece * 8 < k ? from[piece] : make_uint4(0u, 0u, 0u, 0u);
+    }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int piece = seg * (ROWS_SEGMENT / 8) + 32 * j + lane, b = piece >> 2;
-    float v[8];
-    widen8(p[j], v);
-    uint32_t scale;
-    const uint32_t codes = quantize_block(v, scale);
-    if (b < 2 * steps) {                                     // K ends inside a step: its second block is zeros
-      *reinterpret_cast<uint32_t*>(out + mx_code_offset(rows, steps, row, b) + 4 * (piece & 3)) = codes;
-      if ((piece & 3) == 0) out[mx_scale_offset(rows, steps, row, b)] = static_cast<uint8_t>(scale);
+    for (int j = 0; j < 4; ++j) {                                                    // 32 pieces of a warp are a stage
+      const int piece = at + 32 * j + lane, b = piece >> 2, u = (at >> 5) + j;
+      float v[8];
+      widen8(p[j], v);
+      uint32_t scale;
+      const uint32_t codes = quantize_block(v, scale);
+      if (u < full) {
+        *reinterpret_cast<uint32_t*>(line + u * stage_bytes + (((b & 7) ^ (row & 7)) << 4) + 4 * (piece & 3)) = codes;
+        if ((piece & 3) == 0) scale_line[u * stage_bytes + ((b & 7) >> 2) * 512 + (b & 3)] = static_cast<uint8_t>(scale);
+      } else if (u == full && (b & 7) < 2 * tail) {              // K may end inside a step: its second block is zeros
+        *reinterpret_cast<uint32_t*>(out + mx_code_offset(rows, steps, row, b) + 4 * (piece & 3)) = codes;
+        if ((piece & 3) == 0) out[mx_scale_offset(rows, steps, row, b)] = static_cast<uint8_t>(scale);
+      }
     }
   }
 }
@@ -236,9 +240,12 @@ bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
                            const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream) {
   const int steps = mx_steps(k), segments = (steps * MX_STEP + ROWS_SEGMENT - 1) / ROWS_SEGMENT;
-  const int64_t warps = (items ? static_cast<int64_t>(max_items) * tile : m) * segments;
+  const int operands = items ? max_items : (m + tile - 1) / tile, used = items ? tile : std::min(m, tile);
+  if (operands > 65535) return cudaErrorInvalidConfiguration;
+  // few rows: a warp a run, for latency; many: a warp a row
+  const int z = static_cast<int64_t>(operands) * used * segments <= 148 * 64 ? segments : 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((warps + 7) / 8));
+  cfg.gridDim = dim3((used + 7) / 8, operands, z);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
@@ -246,7 +253,7 @@ cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, i
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, rows_kernel, static_cast<const __nv_bfloat16*>(x), ldx, m, k, steps, rows, segments, tile, item_bytes, items,
+  return cudaLaunchKernelEx(&cfg, rows_kernel, static_cast<const __nv_bfloat16*>(x), ldx, m, k, steps, rows, tile, item_bytes, items,
                             counts, members, slots, pairs, static_cast<uint8_t*>(out));
 }
 

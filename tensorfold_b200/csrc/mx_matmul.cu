@@ -36,6 +36,8 @@ int* device_error_word();
 cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
                            const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream);
 
+cudaError_t mx_rows_configure();
+
 namespace {
 
 constexpr int MX_THREADS = 384;
@@ -143,10 +145,6 @@ __device__ __forceinline__ uint32_t lane_test(uint32_t bar, uint32_t parity) {
   asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void let_copies_land() {
   for (int i = 0; i < 64; ++i) __nanosleep(20000);
 }
@@ -166,10 +164,14 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const float* v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t rank, const float* v) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+// Four values into the shared memory of block `rank` of the cluster, counted by that block's barrier.
+__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t bar, uint32_t rank, const float* v) {
+  uint32_t to, at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(bar), "r"(rank));
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(__float_as_uint(v[0])),
+               "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(at)
+               : "memory");
 }
 
 // Fours of rows each of the c blocks of a cluster owns when they add their slices.
@@ -216,7 +218,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
   uint64_t* acc_empty = acc_full + 2;                              // [2]
   uint64_t* op_full = acc_empty + 2;                               // [2] FUSED with a plan: an operand is quantised
   uint64_t* op_empty = op_full + 2;                                // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(op_empty + 2);
+  uint64_t* parts = op_empty + 2;                                  // cluster: every part of this block's rows has come
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(parts + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t ring0 = smem_addr(smem) + MX_BAR_BYTES;           // slots, FUSED operands, then the exchange buffers
   const uint32_t operand0 = ring0 + p.ring * S::SLOT;
@@ -293,19 +296,19 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     fill(ti);
   };
 
-  // The weights' thread: the first slots are filled before the block's set-up is complete (nothing has to be free for them).
+  // The weights' thread.  `fresh`: the first round of the ring, whose slots are free.
   const uint32_t last_bytes = tail * 4096 + mx_tail_scales(tail);
   Ring wr = {0, 1u};
   uint32_t w_ready = 1u;
   Tile wt = {};
   int wu = u0;
   bool w_ok = true;
-  auto load_weights = [&](int stages) {
+  auto load_weights = [&](int stages, bool fresh) {
     while (stages-- > 0 && wt.t < end_tile) {
       if (!w_ready && !(w_ok = lane_wait(empty32 + 8 * wr.slot, wr.phase, abort_word))) return;
       const uint32_t bar = full32 + 8 * wr.slot, dst = ring0 + wr.slot * S::SLOT, bytes = wu < full_stages ? MX_UNIT : last_bytes;
       wr.next(p.ring);
-      w_ready = lane_test(empty32 + 8 * wr.slot, wr.phase);
+      w_ready = fresh ? stages > 0 : lane_test(empty32 + 8 * wr.slot, wr.phase);
       mbar32_expect_tx(bar, bytes);
       bulk_load32(dst, p.w + wt.w + static_cast<int64_t>(wu) * MX_UNIT, bytes, bar);
       if (++wu == u1) {
@@ -368,6 +371,10 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   };
 
+  // Set-up.  Warp 0 makes the barriers and goes on to load weights, which need nothing of the others (it arrives and does not
+  // wait); the drain warps rehearse; where every tile has the same rows, the idle warps quantise them.
+  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 where tiles are taller)
+  const bool drains = warp >= 4 && group < S::GROUPS;
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < MX_RING_MAX; ++i) mbar_init(full + i, FUSED ? 1 : 2), mbar_init(empty + i, 1);
@@ -375,31 +382,22 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, 4 * S::GROUPS);
         mbar_init(op_full + i, 4), mbar_init(op_empty + i, 1);
       }
+      mbar_init(parts, 1);
       *abort_flag = 0;
       mbar_fence_init();
       wt = first();
-      load_weights(p.ring);
+      if (c > 1) {
+        const int quads = (wt.rows + 3) / 4, share = quads_of(wt.rows, c);
+        mbar32_expect_tx(smem_addr(parts), c * max(0, min(share, quads - static_cast<int>(rank) * share)) * MX_SB * 16);
+      }
     }
     __syncwarp();
-  } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (FUSED && !GROUPED && warp >= 4) {
-    // every tile has the same rows: all eight warps quantise them, beside the set-up
-    pdl_wait();
-    quantize_rows(smem + (operand0 - smem_addr(smem)), p.M, warp - 4, 8, [](int r) { return static_cast<int64_t>(r); });
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  if (c > 1) cluster_barrier();                                    // the other blocks run before anything is sent to them
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
-  pdl_launch_dependents();
-
-  if (warp == 0) {
+    asm volatile("barrier.cta.arrive 3, %0;" ::"n"(MX_THREADS) : "memory");
+    if (c > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     // ------------------------------------------------------------------ weights
     if (lane == 0) {
-      load_weights(INT32_MAX);
+      load_weights(p.ring, true);
+      load_weights(INT32_MAX, false);
       if (!w_ok) lost(ERR_WAIT_EMPTY), let_copies_land();
       if (GROUPED) {
         for (Tile ti = first(); ti.t < end_tile; next(ti)) {
@@ -409,7 +407,31 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       }
     }
     __syncwarp();
-  } else if (warp == 2 && !FUSED) {
+    if (c > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (FUSED && !GROUPED && !drains) {
+    pdl_wait();
+    quantize_rows(smem + (operand0 - smem_addr(smem)), p.M, warp >= 8 ? warp - 8 : warp + 2, 6, [](int r) { return static_cast<int64_t>(r); });
+  }
+  uint32_t tmem = 0;
+  auto settle_in = [&]() {                                           // every warp but the first: the barriers and tensor memory are there
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("barrier.cta.sync 3, %0;" ::"n"(MX_THREADS) : "memory");
+    // The other blocks run, and their barriers are there, before anything is sent to them.  Warp 0's arrival releases the barriers;
+    // the others' are relaxed: a release beside the weights' copies took as long as those, 1 to 4 us.
+    if (c > 1) {
+      asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
+    pdl_launch_dependents();
+  };
+  if (warp != 0 && !drains) settle_in();
+
+  if (warp == 2 && !FUSED) {
     // ------------------------------------------------------------------ quantised rows
     pdl_wait();
     if (elect_lane()) {
@@ -539,10 +561,6 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     if (!ok) give_up(ERR_WAIT_EMPTY);
   }
 
-  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 where tiles are taller)
-  const bool drains = warp >= 4 && group < S::GROUPS;
-  if (c > 1 && !drains) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-
   if (drains) {
     // ------------------------------------------------------------------ drain
     const int lg = warp & 3;
@@ -633,10 +651,11 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     // it runs once over no rows before the first accumulator is ready: its instructions are at hand then.
     bool ok = true;
     int use = 0;
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(lg * 32) << 16) + 16 * group;
+    uint32_t lanes = 0;
     Tile ti = first();
     const int here = ti.rows;
     ti.rows = 0;
+    if (ti.t >= end_tile) settle_in();
     for (bool rehearsal = true; ti.t < end_tile && ok;) {
       if (!rehearsal) {
         if (slice1 - slice0 > 1) {
@@ -672,12 +691,11 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         if (!ok) break;
       }
       const uint32_t src = lanes + (use & 1) * NT;
-      const int share = quads_of(ti.rows, c);
+      const int share = max(1, quads_of(ti.rows, c));
       int n0 = 0;                                                    // first row this block finishes
       if (c > 1) {
-        // Part [slice][four rows of the owner][128 columns][4] goes to the shared memory of the block that owns the rows.  The
-        // host launches one tile a cluster; when the barrier opens every part has been sent (parts of blocks that gave up are missing,
-        // which the error word says).
+        // Part [slice][four rows of the owner][128 columns][4] goes to the shared memory of the block that owns the rows (the host
+        // launches one tile a cluster, so a block's buffer is written once).
         const uint32_t part = smem_addr(smem) + extra_off + (lg * 32 + lane) * 16;
 #pragma unroll 1
         for (int n = 16 * group; n < ti.rows; n += 16 * S::GROUPS) {
@@ -687,21 +705,17 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
           int owner = (n >> 2) / share, at = (n >> 2) - owner * share;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (n + 4 * j < ti.rows) store_remote(part + (rank * share + at) * (MX_SB * 16), owner, v + 4 * j);
+            if (n + 4 * j < ti.rows) store_remote(part + (rank * share + at) * (MX_SB * 16), smem_addr(parts), owner, v + 4 * j);
             if (++at == share) at = 0, ++owner;
           }
         }
-        if (!rehearsal) {
-          __syncwarp();
-          cluster_barrier();
-          if (*abort_flag != 0) break;
-        }
+        if (!rehearsal && !(ok = warp_wait(smem_addr(parts), 0, abort_word))) break;
         n0 = 4 * rank * share;
       }
       Tile own = ti;
       if (c > 1) own.rows = min(ti.rows, n0 + 4 * share);
       float ahead[16];                                               // the next sixteen rows are on their way meanwhile
-      if (c == 1 && (rehearsal || 16 * group < ti.rows)) tmem_load16(src, ahead);
+      if (c == 1 && 16 * group < ti.rows) tmem_load16(src, ahead);
 #pragma unroll 1
       for (int n = n0 + 16 * group; n < own.rows || (rehearsal && n < n0 + 16 * S::GROUPS); n += 16 * S::GROUPS) {
         float v[16];
@@ -713,8 +727,9 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
 #pragma unroll 1
           for (int s = 0; s < c; ++s) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {                            // (quads past the share are other parts' and are not stored)
-              const float4 a = part[(s * share + min(i + j, share - 1)) * MX_SB];
+            for (int j = 0; j < 4; ++j) {
+              if (i + j >= share) break;
+              const float4 a = part[(s * share + i + j) * MX_SB];
               if (s == 0) {
                 v[4 * j] = a.x, v[4 * j + 1] = a.y, v[4 * j + 2] = a.z, v[4 * j + 3] = a.w;
               } else {
@@ -736,12 +751,14 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
         } else {
           const int col = ti.cb * MX_SB + lg * 32 + lane;
           store8(own, v, n, col);
-          store8(own, v + 8, n + 8, col);
+          if (n + 8 < own.rows || rehearsal) store8(own, v + 8, n + 8, col);
         }
       }
       if (rehearsal) {
         rehearsal = false;
         ti.rows = here;
+        settle_in();
+        lanes = tmem + (static_cast<uint32_t>(lg * 32) << 16) + 16 * group;
         pdl_wait();                                                  // nothing is written before the previous kernel is done
         continue;
       }
@@ -752,15 +769,11 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       if (c > 1) break;                                              // (one tile a cluster)
       next(ti);
     }
-    if (!ok) {
-      give_up(ERR_WAIT_FULL);
-      if (c > 1) cluster_barrier();
-    }
+    if (!ok) give_up(ERR_WAIT_FULL);
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (c > 1 && !drains) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -870,9 +883,9 @@ bool fused_fits(int k, int sk) {
   return longest * MxShape<16, true>::B_BYTES + 4 * MX_UNIT + MX_CLUSTER_MAX * 4 * MX_SB * 4 <= MX_SMEM_MAX;
 }
 
-// Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its eight warps have
-// few segments of 1024 inputs each.
-constexpr int FUSED_SEGMENTS = 24;
+// Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its six idle warps
+// have few segments of 1024 inputs each.
+constexpr int FUSED_SEGMENTS = 18;
 bool fused_pays(int m, int k, int sk) {
   if (m > MX_FUSED_ROWS || !fused_fits(k, sk)) return false;
   const int longest = (mx_stages(mx_steps(k)) + sk - 1) / sk;
@@ -884,7 +897,8 @@ bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 }  // namespace
 
 cudaError_t mx_configure(int device, int sms) {
-  cudaError_t e = configure<16, true, false>();
+  cudaError_t e = mx_rows_configure();
+  if (e == cudaSuccess) e = configure<16, true, false>();
   if (e == cudaSuccess) e = configure<16, true, true>();
   if (e == cudaSuccess) e = configure<16, false, false>();
   if (e == cudaSuccess) e = configure<16, false, true>();

@@ -235,6 +235,12 @@ bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 
 }  // namespace
 
+// The product's blocks, which take nearly all of an SM's shared memory, start while this kernel runs: an SM that has to change its split
+// between cache and shared memory first would wait for this kernel's blocks to leave it.
+cudaError_t mx_rows_configure() {
+  return cudaFuncSetAttribute(rows_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
 // Rows quantised into operands of `rows` rows, `tile` of them used, item_bytes apart: the first half of the products.  items null:
 // the m rows in order.
 cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,

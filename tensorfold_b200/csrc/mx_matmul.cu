@@ -40,14 +40,13 @@ cudaError_t mx_rows_configure();
 
 namespace {
 
-constexpr int MX_THREADS = 384;
 constexpr int MX_RING_MAX = 12;
 constexpr int MX_BAR_BYTES = 1024;
 constexpr int MX_SMEM_MAX = 232448 - 1024 /* alignment slack */ - MX_BAR_BYTES;
 constexpr int MX_FUSED_ROWS = 16;
 constexpr int MX_QUANT_COLS = 128;                 // columns of the buffer in which a drain group collects rows to quantise
 constexpr int MX_QUANT_ROWS = 16;
-constexpr int MX_QUANT_BYTES = MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;
+constexpr int MX_QUANT_BYTES = 2 * MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;    // two buffers in turn
 constexpr int MX_CLUSTER_MAX = 8;
 constexpr int MX_TILE_MAX = 192;                   // rows of a tile: two accumulators and five slots' scales fill tensor memory
 
@@ -193,7 +192,8 @@ struct MxShape {
   static constexpr int SLOT = MX_UNIT + (FUSED ? 0 : B_BYTES);
   static constexpr int SF_COLS = 8 + 8 * SBS;                      // scale columns of a slot
   static constexpr int TMEM = FUSED ? 256 : 512;
-  static constexpr int GROUPS = NT > 16 ? 2 : 1;                   // drain groups of four warps; they take sixteen rows in turn
+  static constexpr int GROUPS = NT > 64 ? 3 : NT > 16 ? 2 : 1;     // drain groups of four warps; they take sixteen rows in turn
+  static constexpr int THREADS = 128 + 128 * (GROUPS > 2 ? GROUPS : 2);
   static constexpr int CHUNKS = (NT / 16 + GROUPS - 1) / GROUPS;   // runs of sixteen rows a group drains
   static constexpr int RING = (TMEM - 2 * NT) / SF_COLS < MX_RING_MAX ? (TMEM - 2 * NT) / SF_COLS : MX_RING_MAX;
 };
@@ -208,7 +208,7 @@ struct Ring {
 };
 
 template <int NT, bool FUSED, bool GROUPED>
-__global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
+__global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(const MxParams p) {
   using S = MxShape<NT, FUSED>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -350,11 +350,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       if (r < rows) fetch(ahead);
       uint32_t codes[4], scale[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[8];
-        widen8(v4[j], v);
-        codes[j] = quantize_block(v, scale[j]);
-      }
+      for (int j = 0; j < 4; ++j) codes[j] = quantize_block(v4[j], scale[j]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int q = q0 + 32 * j, b = q >> 2, u = b >> 3;
@@ -373,7 +369,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
 
   // Set-up.  Warp 0 makes the barriers and goes on to load weights, which need nothing of the others (it arrives and does not
   // wait); the drain warps rehearse; where every tile has the same rows, the idle warps quantise them.
-  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7, and 8-11 where tiles are taller)
+  const int group = (warp - 4) >> 2;                                 // drain group (warps 4-7; two or three groups where tiles are taller)
   const bool drains = warp >= 4 && group < S::GROUPS;
   if (warp == 0) {
     if (lane == 0) {
@@ -392,7 +388,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       }
     }
     __syncwarp();
-    asm volatile("barrier.cta.arrive 3, %0;" ::"n"(MX_THREADS) : "memory");
+    asm volatile("barrier.cta.arrive 4, %0;" ::"n"(S::THREADS) : "memory");
     if (c > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     // ------------------------------------------------------------------ weights
     if (lane == 0) {
@@ -418,7 +414,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
   uint32_t tmem = 0;
   auto settle_in = [&]() {                                           // every warp but the first: the barriers and tensor memory are there
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    asm volatile("barrier.cta.sync 3, %0;" ::"n"(MX_THREADS) : "memory");
+    asm volatile("barrier.cta.sync 4, %0;" ::"n"(S::THREADS) : "memory");
     // The other blocks run, and their barriers are there, before anything is sent to them.  Warp 0's arrival releases the barriers;
     // the others' are relaxed: a release beside the weights' copies took as long as those, 1 to 4 us.
     if (c > 1) {
@@ -567,11 +563,19 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     const bool gated = p.epi == MX_SWIGLU;
     const int ncols = gated ? p.N / 2 : p.N;
     const bool wide = !p.out_f32 && (ncols & 7) == 0 && (p.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-    auto row_of = [&](const Tile& ti, int n) -> int64_t {            // the output row of row n of the tile; below 0: none
-      if (n >= ti.rows) return -1;
-      if (!GROUPED) return ti.m0 + n;
-      const int pair = p.members[ti.m0 + n];
-      return pair < p.pairs ? pair : -1;
+    // The output row of row n of the tile, below 0 for none.  With a plan lane l holds the pair of row l of the sixteen at hand.
+    int pair16 = -1;
+    auto pairs_of = [&](const Tile& ti, int n) {
+      int pair = -1;
+      if (GROUPED && p.q == nullptr && n + (lane & 15) < ti.rows) pair = __ldg(p.members + ti.m0 + n + (lane & 15));
+      return pair;
+    };
+    auto row_of = [&](const Tile& ti, int n) -> int64_t {
+      if (GROUPED) {
+        const int pair = __shfl_sync(0xFFFFFFFFu, pair16, n & 15);
+        return n < ti.rows && pair < p.pairs ? pair : -1;
+      }
+      return n < ti.rows ? ti.m0 + n : -1;
     };
     // v[j] = row n + j of the tile in output column `col`, a lane a column
     auto store8 = [&](const Tile& ti, const float* v, int n, int col) {
@@ -609,11 +613,13 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       }
     };
     // Sixteen rows of activations to the next projection's operand: through shared memory, where four lanes see a block.
+    int turn = 0;
     auto quantize16 = [&](const Tile& ti, const float* v, int n) {
       constexpr int LINE = MX_QUANT_COLS + 4;
-      float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES);
+      // (a warp that writes a buffer again has passed the barrier after which the others read its last contents twice)
+      float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES) + turn * MX_QUANT_ROWS * LINE;
+      turn ^= 1;
       const int shift = gated ? 3 : 4;                               // pieces of eight columns a row: 8 or 16
-      named_barrier(1 + group, 128);                                 // the last sixteen rows have been read
       if (gated) {
         float* to = rows + (lane < 16 ? 0 : 8) * LINE + lg * 16 + (lane & 15);
 #pragma unroll
@@ -652,7 +658,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
     bool ok = true;
     int use = 0;
     uint32_t lanes = 0;
-    Tile ti = first();
+    Tile ti = first(), after = ti;
+    next(after);
     const int here = ti.rows;
     ti.rows = 0;
     if (ti.t >= end_tile) settle_in();
@@ -715,6 +722,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       Tile own = ti;
       if (c > 1) own.rows = min(ti.rows, n0 + 4 * share);
       float ahead[16];                                               // the next sixteen rows are on their way meanwhile
+      int pairs_ahead = pairs_of(own, n0 + 16 * group);
       if (c == 1 && 16 * group < ti.rows) tmem_load16(src, ahead);
 #pragma unroll 1
       for (int n = n0 + 16 * group; n < own.rows || (rehearsal && n < n0 + 16 * S::GROUPS); n += 16 * S::GROUPS) {
@@ -743,6 +751,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
           for (int j = 0; j < 16; ++j) v[j] = ahead[j];
           if (n + 16 * S::GROUPS < own.rows) tmem_load16(src + n + 16 * S::GROUPS - 16 * group, ahead);
         }
+        pair16 = pairs_ahead;
+        pairs_ahead = pairs_of(own, n + 16 * S::GROUPS);
         activate(v);
         if (GROUPED && p.q != nullptr) {
           quantize16(own, v, n);
@@ -767,7 +777,8 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx_kernel(const MxParams p) {
       if (lane == 0) mbar_arrive(acc_empty + (use & 1));
       ++use;
       if (c > 1) break;                                              // (one tile a cluster)
-      next(ti);
+      ti = after;
+      next(after);
     }
     if (!ok) give_up(ERR_WAIT_FULL);
   }
@@ -813,7 +824,7 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl
   const int64_t most = std::max(1, sms / p.cluster);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.cluster > 1 ? tiles : std::min(tiles, most)) * p.cluster));
-  cfg.blockDim = dim3(MX_THREADS);
+  cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = 1024 + MX_BAR_BYTES + p.ring * S::SLOT + p.bufs * operand + extra;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];

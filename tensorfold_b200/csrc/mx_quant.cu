@@ -18,24 +18,40 @@ int cuda_fail_moe(cudaError_t e, const char* what);
 
 namespace {
 
-// Eight values of one of the stored types: 0 bf16, 1 fp16, 2 fp32.
-__device__ __forceinline__ void load8(const void* row, int64_t at, const int dtype, float (&v)[8]) {
-  if (dtype == 0) {
-    widen8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(row) + at), v);
-  } else if (dtype == 1) {
-    const uint4 p = *reinterpret_cast<const uint4*>(static_cast<const __half*>(row) + at);
-    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
-  } else {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
-    const float4 a = p[0], b = p[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// Eight values of a stored type (0 bf16, 1 fp16, 2 fp32) as they lie in memory, and rounded.
+template <int DTYPE>
+struct Piece {
+  uint4 p[DTYPE == 2 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* from, int64_t at) {
+    const uint4* q = reinterpret_cast<const uint4*>(from) + at * (DTYPE == 2 ? 2 : 1);
+    p[0] = q[0];
+    if (DTYPE == 2) p[DTYPE == 2] = q[1];
   }
-}
+  __device__ __forceinline__ void clear() {
+    p[0] = make_uint4(0u, 0u, 0u, 0u);
+    if (DTYPE == 2) p[DTYPE == 2] = p[0];
+  }
+  __device__ __forceinline__ uint32_t quantize(uint32_t& scale) const {
+    if constexpr (DTYPE == 0) {
+      return quantize_block(p[0], scale);
+    } else {
+      float v[8];
+      const uint32_t w[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+      if constexpr (DTYPE == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+      } else {
+        const uint32_t u[4] = {p[1].x, p[1].y, p[1].z, p[1].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]), v[4 + i] = __uint_as_float(u[i]);
+      }
+      return quantize_block(v, scale);
+    }
+  }
+};
 
 // Rows to stored words and scales.  A lane takes eight values, four lanes a block, so loads and stores of a warp are runs; U
 // pieces a thread are in flight at once.  Rows one after another (FLAT) are one run of pieces; others go by blockIdx.y.
@@ -47,19 +63,18 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
     const char* from = static_cast<const char*>(x) + (FLAT ? 0 : row * ldx * (DTYPE == 2 ? 4 : 2));
     // whole warps walk together: a piece past the end computes on zeros and stores nothing
     for (int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + (threadIdx.x & ~31); first < pieces; first += U * step) {
-      float v[U][8];
+      Piece<DTYPE> v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t i = first + u * step + (threadIdx.x & 31);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
-        if (i < pieces) load8(from, i * 8, DTYPE, v[u]);
+        if (i < pieces) v[u].load(from, i);
+        else v[u].clear();
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t i = first + u * step + (threadIdx.x & 31);
         uint32_t scale;
-        const uint32_t codes = quantize_block(v[u], scale);
+        const uint32_t codes = v[u].quantize(scale);
         if (i < pieces) {
           const int64_t to = FLAT ? i : row * pieces + i;
           words[to] = codes;
@@ -209,10 +224,8 @@ __global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restri
 #pragma unroll
     for (int j = 0; j < 4; ++j) {                                                    // 32 pieces of a warp are a stage
       const int piece = at + 32 * j + lane, b = piece >> 2, u = (at >> 5) + j;
-      float v[8];
-      widen8(p[j], v);
       uint32_t scale;
-      const uint32_t codes = quantize_block(v, scale);
+      const uint32_t codes = quantize_block(p[j], scale);
       if (u < full) {
         *reinterpret_cast<uint32_t*>(line + u * stage_bytes + (((b & 7) ^ (row & 7)) << 4) + 4 * (piece & 3)) = codes;
         if ((piece & 3) == 0) scale_line[u * stage_bytes + ((b & 7) >> 2) * 512 + (b & 3)] = static_cast<uint8_t>(scale);

@@ -47,4 +47,22 @@ __device__ __forceinline__ void widen8(uint4 p, float (&v)[8]) {
   for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
 }
 
+// The same from eight bf16 values as they lie in memory: their magnitudes compare two at a time as 16-bit integers.
+__device__ __forceinline__ uint32_t quantize_block(uint4 p, uint32_t& scale) {
+  constexpr uint32_t MAGNITUDE = 0x7FFF7FFFu;
+  uint32_t m = __vmaxu2(__vmaxu2(p.x & MAGNITUDE, p.y & MAGNITUDE), __vmaxu2(p.z & MAGNITUDE, p.w & MAGNITUDE));
+  m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+  m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+  const uint32_t top = max(m >> 16, m & 0xFFFFu);
+  const bool bad = top >= 0x7F80u;
+  scale = bad ? 255u : static_cast<uint32_t>(max(static_cast<int>(top >> 7) - 2, 0));
+  const float inverse = __uint_as_float((254u - min(scale, 254u)) << 23);
+  float v[8];
+  widen8(p, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= inverse;
+  const uint32_t codes = e2m1x8(v);
+  return bad ? 0u : codes;
+}
+
 }  // namespace tf

@@ -22,6 +22,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/tensorfold_b200.h"
 #include "mx_layout.h"
@@ -176,23 +177,18 @@ __device__ __forceinline__ void store_remote(uint32_t addr, uint32_t bar, uint32
 // Fours of rows each of the c blocks of a cluster owns when they add their slices.
 __host__ __device__ __forceinline__ int quads_of(int rows, int c) { return ((rows + 3) / 4 + c - 1) / c; }
 
-// silu(gate) * up in fp32, clipped first where limit > 0.  Comparisons, not fminf: a NaN goes through.
-__device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  if (limit > 0.f) {
-    g = g > limit ? limit : g;
-    u = u > limit ? limit : u < -limit ? -limit : u;
-  }
-  return __fdividef(g, 1.f + expf(-g)) * u;
-}
+// silu(gate) * up in fp32.
+__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 
-template <int NT, bool FUSED>
+template <int NT, bool FUSED, bool GROUPED>
 struct MxShape {
   static constexpr int SBS = (NT + MX_SB - 1) / MX_SB;
   static constexpr int B_BYTES = NT * 128 + SBS * MX_SCALES;
   static constexpr int SLOT = MX_UNIT + (FUSED ? 0 : B_BYTES);
   static constexpr int SF_COLS = 8 + 8 * SBS;                      // scale columns of a slot
   static constexpr int TMEM = FUSED ? 256 : 512;
-  static constexpr int GROUPS = NT > 64 ? 3 : NT > 16 ? 2 : 1;     // drain groups of four warps; they take sixteen rows in turn
+  // Drain groups of four warps; they take sixteen rows in turn.  With a plan the drain has activations to compute and quantise.
+  static constexpr int GROUPS = NT == 16 ? 1 : GROUPED ? 3 : 2;
   static constexpr int THREADS = 128 + 128 * (GROUPS > 2 ? GROUPS : 2);
   static constexpr int CHUNKS = (NT / 16 + GROUPS - 1) / GROUPS;   // runs of sixteen rows a group drains
   static constexpr int RING = (TMEM - 2 * NT) / SF_COLS < MX_RING_MAX ? (TMEM - 2 * NT) / SF_COLS : MX_RING_MAX;
@@ -208,8 +204,8 @@ struct Ring {
 };
 
 template <int NT, bool FUSED, bool GROUPED>
-__global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(const MxParams p) {
-  using S = MxShape<NT, FUSED>;
+__global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_kernel(const MxParams p) {
+  using S = MxShape<NT, FUSED, GROUPED>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);              // [MX_RING_MAX] the slot's copies have landed
@@ -259,22 +255,28 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
   const int end_tile = RUNS ? static_cast<int>(static_cast<int64_t>(tiles) * (mine + 1) / clusters) : tiles;
   const int tile_step = RUNS ? 1 : clusters;
 
+  // A tile is looked up one ahead: `after` starts the loads of the plan's item, `settle` uses what they brought.
   struct Tile {
     int t;                                                         // number of the tile
-    int y, cb, m0, rows, n;                                        // item or row tile, column block, first row (or member), rows, MMA N
+    int y, cb;                                                     // item or row tile, column block
+    int expert, from, count;                                       // the item as it stands in the plan
+    int m0, rows, n;                                               // first row (or member), rows, MMA N
     int64_t w;                                                     // offset of the weights
   };
-  auto fill = [&](Tile& ti) {
-    if (ti.t >= end_tile) return;
+  auto look_up = [&](Tile& ti) {
+    if (GROUPED && ti.t < end_tile) {
+      const int* item = p.items + 3 * ti.y;
+      ti.expert = __ldg(item), ti.from = __ldg(item + 1), ti.count = __ldg(item + 2);
+    }
+  };
+  auto settle = [&](Tile& ti) {
     ti.w = ti.cb * p.sb_bytes;
     if (GROUPED) {
-      const int* item = p.items + 3 * ti.y;
-      const int expert = __ldg(item);
       // an item that names an expert outside the table runs against expert 0 with no rows (the weights' thread reports it)
-      const bool known = expert >= 0 && expert < p.experts;
-      ti.w += (known ? expert : 0) * p.expert_stride;
-      ti.m0 = __ldg(item + 1);
-      ti.rows = known ? min(p.tile, __ldg(item + 2)) : 0;
+      const bool known = ti.expert >= 0 && ti.expert < p.experts;
+      ti.w += (known ? ti.expert : 0) * p.expert_stride;
+      ti.m0 = ti.from;
+      ti.rows = known ? min(p.tile, ti.count) : 0;
       if (ti.m0 < 0 || ti.rows < 0 || ti.m0 > p.pairs - ti.rows) ti.rows = 0;
     } else {
       ti.m0 = ti.y * p.tile;
@@ -286,21 +288,23 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
     Tile ti = {};
     ti.t = first_tile;
     ti.y = FUSED && !GROUPED ? 0 : first_tile / ncb, ti.cb = first_tile - ti.y * ncb;
-    fill(ti);
+    look_up(ti);
+    settle(ti);
     return ti;
   };
-  auto next = [&](Tile& ti) {
+  auto after = [&](Tile ti) {
     ti.t += tile_step, ti.cb += tile_step;
     if (!FUSED || GROUPED)
       while (ti.cb >= ncb) ti.cb -= ncb, ++ti.y;
-    fill(ti);
+    look_up(ti);
+    return ti;
   };
 
   // The weights' thread.  `fresh`: the first round of the ring, whose slots are free.
   const uint32_t last_bytes = tail * 4096 + mx_tail_scales(tail);
   Ring wr = {0, 1u};
   uint32_t w_ready = 1u;
-  Tile wt = {};
+  Tile wt = {}, wt_after = {};
   int wu = u0;
   bool w_ok = true;
   auto load_weights = [&](int stages, bool fresh) {
@@ -313,7 +317,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       bulk_load32(dst, p.w + wt.w + static_cast<int64_t>(wu) * MX_UNIT, bytes, bar);
       if (++wu == u1) {
         wu = u0;
-        next(wt);
+        wt = wt_after;
+        settle(wt);
+        wt_after = after(wt);
       }
     }
   };
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
     const int p0 = u0 * 32, pieces = min(p.steps * 8, u1 * 32) - p0;   // 16-byte pieces of a row in this slice (K padded to 64)
     const int segments = (pieces + 127) >> 7;
     int r = 0, seg = w;
-    auto settle = [&]() {
+    auto wrap = [&]() {
       while (seg >= segments) seg -= segments, ++r;
     };
     auto fetch = [&](uint4 (&v4)[4]) {
@@ -337,7 +343,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
         if (row >= 0 && q < pieces && (p0 + q) * 8 < p.K) v4[j] = from[q];
       }
     };
-    settle();
+    wrap();
     uint4 ahead[4];
     if (r < rows) fetch(ahead);
     while (r < rows) {
@@ -346,7 +352,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
 #pragma unroll
       for (int j = 0; j < 4; ++j) v4[j] = ahead[j];
       seg += stride;
-      settle();
+      wrap();
       if (r < rows) fetch(ahead);
       uint32_t codes[4], scale[4];
 #pragma unroll
@@ -382,6 +388,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       *abort_flag = 0;
       mbar_fence_init();
       wt = first();
+      wt_after = after(wt);
       if (c > 1) {
         const int quads = (wt.rows + 3) / 4, share = quads_of(wt.rows, c);
         mbar32_expect_tx(smem_addr(parts), c * max(0, min(share, quads - static_cast<int>(rank) * share)) * MX_SB * 16);
@@ -396,10 +403,8 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       load_weights(INT32_MAX, false);
       if (!w_ok) lost(ERR_WAIT_EMPTY), let_copies_land();
       if (GROUPED) {
-        for (Tile ti = first(); ti.t < end_tile; next(ti)) {
-          const int expert = __ldg(p.items + 3 * ti.y);
-          if (expert < 0 || expert >= p.experts) atomicCAS(p.err, 0, ERR_BAD_ITEM);
-        }
+        for (Tile ti = first(); ti.t < end_tile; ti = after(ti))
+          if (ti.expert < 0 || ti.expert >= p.experts) atomicCAS(p.err, 0, ERR_BAD_ITEM);
       }
     }
     __syncwarp();
@@ -435,7 +440,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       bool ok = true;
       Ring r = {0, 1u};
       uint32_t ready = 1u;                                         // (a fresh slot's test passes)
-      for (Tile ti = first(); ti.t < end_tile && ok; next(ti)) {
+      for (Tile ti = first(), then = after(ti); ti.t < end_tile && ok; ti = then, settle(ti), then = after(ti)) {
         const int sbs = mx_scale_blocks(ti.n);
         const uint8_t* src = p.b + ti.y * p.item_stride + u0 * stage_bytes;
 #pragma unroll 1
@@ -474,9 +479,8 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       Ring r = {0, 0u};
       int use = 0, op = GROUPED ? -1 : 0, last_y = -1;
       uint32_t ready = 0;
-      for (Tile ti = first(); ti.t < end_tile && ok;) {
+      for (Tile ti = first(), then = after(ti); ti.t < end_tile && ok; ti = then, settle(ti), then = after(ti)) {
         const int n = ti.n, y = ti.y;
-        next(ti);
         if (RUNS && y != last_y) {
           last_y = y;
           ++op;
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
           }
           commit(acc_full32 + 8 * (use & 1));
         }
-        if (RUNS && ok && (ti.t >= end_tile || ti.y != y)) commit(smem_addr(op_empty + buf));
+        if (RUNS && ok && (then.t >= end_tile || then.y != y)) commit(smem_addr(op_empty + buf));
       }
       if (!ok) lost(ERR_WAIT_FULL);
     }
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
     // ------------------------------------------------------------------ bf16 rows of an item -> operand in shared memory
     bool ok = true;
     int op = -1, last_y = -1;
-    for (Tile ti = first(); ti.t < end_tile; next(ti)) {
+    for (Tile ti = first(), then = after(ti); ti.t < end_tile; ti = then, settle(ti), then = after(ti)) {
       if (ti.y == last_y) continue;
       last_y = ti.y;
       ++op;
@@ -577,16 +581,24 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       }
       return n < ti.rows ? ti.m0 + n : -1;
     };
-    // v[j] = row n + j of the tile in output column `col`, a lane a column
-    auto store8 = [&](const Tile& ti, const float* v, int n, int col) {
+    // v[j] = row n + j of the tile in output column `col`, a lane a column; COUNT runs of eight rows, 8 apart
+    auto store = [&](auto count, const Tile& ti, const float* v, int n, int col) {
+      constexpr int COUNT = decltype(count)::value;
       if (wide) {
-        const float t[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-        const uint4 o = transpose8(t, lane);                         // columns col - l8 .. col - l8 + 7 of row n + l8
-        const int64_t row = row_of(ti, n + (lane & 7));
-        if (row >= 0 && col < ncols) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + (col - (lane & 7))) = o;
+        uint4 o[COUNT];
+        int64_t row[COUNT];
+#pragma unroll
+        for (int h = 0; h < COUNT; ++h) {
+          const float t[8] = {v[8 * h], v[8 * h + 1], v[8 * h + 2], v[8 * h + 3], v[8 * h + 4], v[8 * h + 5], v[8 * h + 6], v[8 * h + 7]};
+          o[h] = transpose8(t, lane);                                // columns col - l8 .. col - l8 + 7 of row n + 8 h + l8
+          row[h] = row_of(ti, n + 8 * h + (lane & 7));
+        }
+#pragma unroll
+        for (int h = 0; h < COUNT; ++h)
+          if (row[h] >= 0 && col < ncols) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row[h] * p.ldo + (col - (lane & 7))) = o[h];
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 8 * COUNT; ++j) {
           const int64_t row = row_of(ti, n + j);
           if (row < 0 || col >= ncols) continue;
           if (p.out_f32) static_cast<float*>(p.out)[row * p.ldo + col] = v[j];
@@ -595,15 +607,27 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       }
     };
     // Activations of sixteen rows.  SwiGLU: gate in lanes 0-15, up in lanes 16-31 of the same outputs; the lower lanes come out
-    // with rows 0-7 in v[0..7], the upper ones with rows 8-15.
+    // with rows 0-7 in v[0..7], the upper ones with rows 8-15.  Clips (limit > 0) are comparisons, not fminf: a NaN goes through; and
+    // they stand apart, so that the eight values' chains run side by side.
     auto activate = [&](float* v) {
       if (gated) {
         const bool low = lane < 16;
+        float u[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float got = __shfl_xor_sync(0xFFFFFFFFu, low ? v[8 + j] : v[j], 16);
-          v[j] = swiglu(low ? v[j] : got, low ? got : v[8 + j], p.limit);
+          u[j] = low ? got : v[8 + j];
+          v[j] = low ? v[j] : got;
         }
+        if (p.limit > 0.f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = v[j] > p.limit ? p.limit : v[j];
+            u[j] = u[j] > p.limit ? p.limit : u[j] < -p.limit ? -p.limit : u[j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = swiglu(v[j], u[j]);
       } else if (p.epi == MX_RELU2) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -658,8 +682,8 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
     bool ok = true;
     int use = 0;
     uint32_t lanes = 0;
-    Tile ti = first(), after = ti;
-    next(after);
+    Tile ti = first(), then = {};
+    if (GROUPED) then = after(ti);
     const int here = ti.rows;
     ti.rows = 0;
     if (ti.t >= end_tile) settle_in();
@@ -757,11 +781,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
         if (GROUPED && p.q != nullptr) {
           quantize16(own, v, n);
         } else if (gated) {
-          store8(own, v, n + (lane < 16 ? 0 : 8), ti.cb * 64 + lg * 16 + (lane & 15));
+          store(std::integral_constant<int, 1>(), own, v, n + (lane < 16 ? 0 : 8), ti.cb * 64 + lg * 16 + (lane & 15));
         } else {
-          const int col = ti.cb * MX_SB + lg * 32 + lane;
-          store8(own, v, n, col);
-          if (n + 8 < own.rows || rehearsal) store8(own, v + 8, n + 8, col);
+          store(std::integral_constant<int, 2>(), own, v, n, ti.cb * MX_SB + lg * 32 + lane);
         }
       }
       if (rehearsal) {
@@ -777,8 +799,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED>::THREADS, 1) mx_kernel(cons
       if (lane == 0) mbar_arrive(acc_empty + (use & 1));
       ++use;
       if (c > 1) break;                                              // (one tile a cluster)
-      ti = after;
-      next(after);
+      ti = GROUPED ? then : after(ti);
+      settle(ti);
+      if (GROUPED) then = after(ti);
     }
     if (!ok) give_up(ERR_WAIT_FULL);
   }
@@ -812,7 +835,7 @@ int slices_for(int n, int k) {
 
 template <int NT, bool FUSED, bool GROUPED>
 cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
-  using S = MxShape<NT, FUSED>;
+  using S = MxShape<NT, FUSED, GROUPED>;
   int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
   if (p.cluster > 1) extra = p.cluster * quads_of(std::min(p.tile, p.M), p.cluster) * MX_SB * 16;
   const int operand = FUSED ? p.operand_stages * S::B_BYTES : 0;
@@ -891,7 +914,7 @@ Tiling tiling_for(int m, int n, int stages, int sk) {
 // Whether a block can hold its K slice of sixteen quantised rows beside a ring of four slots.
 bool fused_fits(int k, int sk) {
   const int stages = mx_stages(mx_steps(k)), longest = (stages + sk - 1) / sk;
-  return longest * MxShape<16, true>::B_BYTES + 4 * MX_UNIT + MX_CLUSTER_MAX * 4 * MX_SB * 4 <= MX_SMEM_MAX;
+  return longest * MxShape<16, true, true>::B_BYTES + 4 * MX_UNIT + MX_CLUSTER_MAX * 4 * MX_SB * 4 <= MX_SMEM_MAX;
 }
 
 // Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its six idle warps

@@ -315,7 +315,8 @@ int tf_mx_pack(const void* words, const void* scales, const void* up_words, cons
 int tf_mx_unpack(const void* tiled, int n, int k, void* words, void* scales, void* stream);
 /* out[m, n] = x @ w.T with the rows of x quantised as above, products exact, sums fp32: K slices of tf_mx_split(n, k), each one
  * chain of 64-input steps, added in order, so a row's bits never depend on m.  epi and limit as in tf_qmm_act, but activations
- * are computed from the fp32 sums and rounded once.  pdl as in tf_qmm.
+ * are computed from the fp32 sums and rounded once.  The launches use programmatic stream serialisation and read global memory only
+ * once the previous kernel is done; with pdl = 1 the weights are read before that, so they must be settled (as in tf_qmm).
  *   work     tf_mx_matmul_bytes(m, n, k) bytes (0 for decode and verify windows: the kernel quantises the rows itself), 16-byte
  *            aligned, contents free; calls that may overlap need different work */
 int tf_mx_split(int n, int k);
@@ -326,12 +327,13 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
  * slice.  Input: bf16 rows x with work of tf_mx_experts_bytes(k, tile, max_items) bytes, or with x NULL work that an earlier call
  * filled as out_operands.  Output: out as in tf_moe_experts, or out_operands, where the results (activations: epi 1 or 2) are
  * quantised from their fp32 values for the next projection: max_items * tf_mx_operand_bytes(tile, columns) bytes.  A pair's bits
- * do not depend on the other pairs, nor on the tile. */
+ * do not depend on the other pairs, nor on the tile.  pdl = 1: weights and plan are read while the previous kernel runs, so no
+ * kernel in flight may write them (the second projection after the first, which waited for the plan). */
 int64_t tf_mx_operand_bytes(int rows, int k);
 int64_t tf_mx_experts_bytes(int k, int tile, int max_items);
 int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
                   const int* counts, const int* members, int pairs, int max_items, int tile, void* out, int64_t ldo, int out_f32,
-                  void* out_operands, int epi, float limit, void* work, int64_t work_bytes, void* stream);
+                  void* out_operands, int epi, float limit, void* work, int64_t work_bytes, int pdl, void* stream);
 
 #ifdef __cplusplus
 }

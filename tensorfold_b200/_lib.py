@@ -81,7 +81,7 @@ SIGNATURES = {
     "tf_mx_operand_bytes": (_i64, (_i32, _i32)),
     "tf_mx_experts_bytes": (_i64, (_i32, _i32, _i32)),
     "tf_mx_experts": (_i32, (_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _i32,
-                             ctypes.c_float, _vp, _i64, _vp)),
+                             ctypes.c_float, _vp, _i64, _i32, _vp)),
     "tf_reduce_slices": (_i32, (_vp, _i32, _i64, _vp, _i32, _vp)),
 }
 

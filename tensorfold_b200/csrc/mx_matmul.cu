@@ -35,7 +35,7 @@ int fail_moe(int code, const char* msg);
 int cuda_fail_moe(cudaError_t e, const char* what);
 int* device_error_word();
 cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
-                           const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream);
+                           const int* members, int slots, int pairs, int max_items, void* out, cudaStream_t stream);
 
 cudaError_t mx_rows_configure();
 
@@ -81,6 +81,7 @@ struct MxParams {
   int64_t q_item_stride;
   const int *items, *counts, *members;
   int experts, pairs, max_items;
+  int settled;                  // no kernel in flight writes the weights or the plan: they are read before the dependency wait
   int* err;
 };
 
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
 
   // Tiles: (row tile or item) x 128 columns, columns fastest.  A cluster takes every clusters-th tile; FUSED with a plan a run of
   // neighbours, so that its rows are quantised once an item.
-  if (GROUPED) pdl_wait();                                         // the plan may be the previous kernel's output
+  if (GROUPED && !p.settled) pdl_wait();                           // the plan may be the previous kernel's output
   constexpr bool RUNS = FUSED && GROUPED;
   const int ncb = (p.N + MX_SB - 1) / MX_SB;
   const int tiles = ncb * (GROUPED ? min(p.counts[0], p.max_items) : p.row_tiles);
@@ -398,6 +399,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
     asm volatile("barrier.cta.arrive 4, %0;" ::"n"(S::THREADS) : "memory");
     if (c > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     // ------------------------------------------------------------------ weights
+    if (!GROUPED && !p.settled) pdl_wait();
     if (lane == 0) {
       load_weights(p.ring, true);
       load_weights(INT32_MAX, false);
@@ -544,6 +546,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
     __syncwarp();
   } else if (RUNS && warp >= 8) {
     // ------------------------------------------------------------------ bf16 rows of an item -> operand in shared memory
+    pdl_wait();
     bool ok = true;
     int op = -1, last_y = -1;
     for (Tile ti = first(), then = after(ti); ti.t < end_tile; ti = then, settle(ti), then = after(ti)) {
@@ -834,7 +837,7 @@ int slices_for(int n, int k) {
 }
 
 template <int NT, bool FUSED, bool GROUPED>
-cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl, cudaStream_t stream) {
+cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStream_t stream) {
   using S = MxShape<NT, FUSED, GROUPED>;
   int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
   if (p.cluster > 1) extra = p.cluster * quads_of(std::min(p.tile, p.M), p.cluster) * MX_SB * 16;
@@ -857,11 +860,11 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, bool pdl
     attrs[count].val.clusterDim.x = p.cluster, attrs[count].val.clusterDim.y = 1, attrs[count].val.clusterDim.z = 1;
     ++count;
   }
-  if (pdl) {
-    attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[count].val.programmaticStreamSerializationAllowed = 1;
-    ++count;
-  }
+  // always: a block sets up under the previous kernel's end, and reads and writes global memory once that is done (weights and plan
+  // earlier where they are settled)
+  attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[count].val.programmaticStreamSerializationAllowed = 1;
+  ++count;
   cfg.attrs = attrs;
   cfg.numAttrs = count;
   return cudaLaunchKernelEx(&cfg, mx_kernel<NT, FUSED, GROUPED>, p);
@@ -873,15 +876,15 @@ cudaError_t configure() {
 }
 
 // Rows come as operands: the kernel whose tiles hold `tile` rows.
-cudaError_t launch_rows(MxParams& p, int64_t tiles, int sms, bool pdl, cudaStream_t stream) {
-  if (p.tile <= 16) return launch<16, false, false>(p, tiles, false, sms, pdl, stream);
-  if (p.tile <= 64) return launch<64, false, false>(p, tiles, false, sms, pdl, stream);
-  if (p.tile <= 128) return launch<128, false, false>(p, tiles, false, sms, pdl, stream);
-  return launch<192, false, false>(p, tiles, false, sms, pdl, stream);
+cudaError_t launch_rows(MxParams& p, int64_t tiles, int sms, cudaStream_t stream) {
+  if (p.tile <= 16) return launch<16, false, false>(p, tiles, false, sms, stream);
+  if (p.tile <= 64) return launch<64, false, false>(p, tiles, false, sms, stream);
+  if (p.tile <= 128) return launch<128, false, false>(p, tiles, false, sms, stream);
+  return launch<192, false, false>(p, tiles, false, sms, stream);
 }
-cudaError_t launch_items(MxParams& p, int64_t tiles, int sms, bool pdl, cudaStream_t stream) {
-  return p.tile <= 16 ? launch<16, false, true>(p, tiles, p.q != nullptr, sms, pdl, stream)
-                      : launch<128, false, true>(p, tiles, p.q != nullptr, sms, pdl, stream);
+cudaError_t launch_items(MxParams& p, int64_t tiles, int sms, cudaStream_t stream) {
+  return p.tile <= 16 ? launch<16, false, true>(p, tiles, p.q != nullptr, sms, stream)
+                      : launch<128, false, true>(p, tiles, p.q != nullptr, sms, stream);
 }
 
 int round8(int m) { return (m + 7) / 8 * 8; }
@@ -990,18 +993,19 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     p.cluster = p.sk;
     p.operand_stages = (p.stages + p.sk - 1) / p.sk;
     p.row_tiles = 1;
-    e = launch<16, true, false>(p, ncb, false, sms, pdl != 0, s);
+    p.settled = pdl != 0;
+    e = launch<16, true, false>(p, ncb, false, sms, s);
   } else {
     const Tiling t = tiling_for(m, n, p.stages, p.sk);
     p.tile = p.b_rows = t.tile, p.cluster = t.cluster;
     p.b = static_cast<const uint8_t*>(work), p.item_stride = mx_operand_bytes(t.tile, p.steps);
     const int64_t row_tiles = (m + t.tile - 1) / t.tile;
     if (ncb * row_tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: too many tiles");
-    e = mx_rows_launch(x, ldx, m, k, t.tile, t.tile, p.item_stride, nullptr, nullptr, nullptr, 0, 0, 0, work, pdl != 0, s);
+    e = mx_rows_launch(x, ldx, m, k, t.tile, t.tile, p.item_stride, nullptr, nullptr, nullptr, 0, 0, 0, work, s);
     if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
-    // the rows' kernel lets this one set up and fetch weights while it runs; the weights were settled before it started
+    p.settled = 1;                                                   // the rows' kernel waits before it lets this one start
     p.row_tiles = static_cast<int>(row_tiles);
-    e = launch_rows(p, ncb * row_tiles, sms, true, s);
+    e = launch_rows(p, ncb * row_tiles, sms, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_matmul");
 }
@@ -1018,7 +1022,7 @@ int64_t tf_mx_experts_bytes(int k, int tile, int max_items) {
 
 int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
                   const int* counts, const int* members, int pairs, int max_items, int tile, void* out, int64_t ldo, int out_f32,
-                  void* out_operands, int epi, float limit, void* work, int64_t work_bytes, void* stream) {
+                  void* out_operands, int epi, float limit, void* work, int64_t work_bytes, int pdl, void* stream) {
   if (experts < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || pairs < 1 || max_items < 1 || max_items > (1 << 20) || slots < 0)
     return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad sizes (K a positive multiple of 32)");
   if (tile < 8 || tile > MX_SB || tile % 8) return fail_moe(TF_ERR_ARG, "tf_mx_experts: items of 8 to 128 pairs, in whole eights");
@@ -1051,6 +1055,7 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
   p.items = items, p.counts = counts, p.members = members, p.experts = experts, p.pairs = pairs, p.max_items = max_items;
   p.err = err;
   p.tile = tile;
+  p.settled = pdl != 0;
   const int64_t tiles = static_cast<int64_t>((n + MX_SB - 1) / MX_SB) * max_items;       // upper bound: the plan says how many
   if (tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: too many tiles");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1058,15 +1063,16 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
   if (x && need == 0) {
     p.x = static_cast<const __nv_bfloat16*>(x), p.ldx = ldx, p.slots = slots;
     p.bufs = 2, p.operand_stages = p.stages;
-    e = launch<16, true, true>(p, tiles, out_operands != nullptr, sms, false, s);
+    e = launch<16, true, true>(p, tiles, out_operands != nullptr, sms, s);
   } else {
     if (x) {
-      e = mx_rows_launch(x, ldx, 0, k, rows, tile, operand, items, counts, members, slots, pairs, max_items, work, false, s);
+      e = mx_rows_launch(x, ldx, 0, k, rows, tile, operand, items, counts, members, slots, pairs, max_items, work, s);
       if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_experts: rows");
+      p.settled = 1;                                                 // (as in tf_mx_matmul)
     }
     p.b = static_cast<const uint8_t*>(work), p.b_rows = rows, p.item_stride = operand;
     p.bufs = 1;
-    e = launch_items(p, tiles, sms, x != nullptr, s);
+    e = launch_items(p, tiles, sms, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_experts");
 }

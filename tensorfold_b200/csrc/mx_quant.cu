@@ -257,7 +257,7 @@ cudaError_t mx_rows_configure() {
 // Rows quantised into operands of `rows` rows, `tile` of them used, item_bytes apart: the first half of the products.  items null:
 // the m rows in order.
 cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, int tile, int64_t item_bytes, const int* items, const int* counts,
-                           const int* members, int slots, int pairs, int max_items, void* out, bool pdl, cudaStream_t stream) {
+                           const int* members, int slots, int pairs, int max_items, void* out, cudaStream_t stream) {
   const int steps = mx_steps(k), segments = (steps * MX_STEP + ROWS_SEGMENT - 1) / ROWS_SEGMENT;
   const int operands = items ? max_items : (m + tile - 1) / tile, used = items ? tile : std::min(m, tile);
   if (operands > 65535) return cudaErrorInvalidConfiguration;
@@ -271,7 +271,7 @@ cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, i
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, rows_kernel, static_cast<const __nv_bfloat16*>(x), ldx, m, k, steps, rows, tile, item_bytes, items,
                             counts, members, slots, pairs, static_cast<uint8_t*>(out));
 }

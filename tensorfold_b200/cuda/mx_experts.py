@@ -56,7 +56,7 @@ def _items(plan: grouped.Plan, rows: int) -> int:
     return min(grouped.max_items(rows * plan.slots, plan.experts, plan.tile), plan.items.shape[0])
 
 
-def _call(who, x, slots, table, n, k, plan, rows, out, operands, epi, limit, work):
+def _call(who, x, slots, table, n, k, plan, rows, out, operands, epi, limit, work, pdl=False):
     if plan.experts > table.shape[0]:
         raise ValueError(f"the plan routes to {plan.experts} experts but the table holds {table.shape[0]}")
     pairs = rows * plan.slots
@@ -72,7 +72,7 @@ def _call(who, x, slots, table, n, k, plan, rows, out, operands, epi, limit, wor
     _lib.native().tf_mx_experts(
         who, x, 0 if x is None else x.stride(0), slots, table, table.stride(0), table.shape[0], n, k, plan.items, plan.counts, plan.members,
         pairs, items, plan.tile, out, 0 if out is None else out.stride(0), out is not None and out.dtype == torch.float32, operands, epi, limit,
-        work, 0 if work is None else work.numel(), stream)
+        work, 0 if work is None else work.numel(), pdl, stream)
 
 
 def _inputs(x, k, need, device, who):
@@ -117,4 +117,5 @@ def layer(x: torch.Tensor, ex: Experts, plan: grouped.Plan, out: torch.Tensor, r
     act = torch.empty((_items(plan, rows) * _lib.lib().tf_mx_operand_bytes(plan.tile, ex.width),), dtype=torch.uint8, device=x.device)
     _call("experts (gate, up)", x, plan.slots, ex.up, (2 if ex.gated else 1) * ex.width, ex.dims, plan, rows, None, act, 2 if ex.gated else 1,
           ex.limit, None)
-    _call("experts (down)", None, 0, ex.down, ex.dims, ex.width, plan, rows, out, None, 0, 0.0, act)
+    # the first projection waited for the plan, so the second may read it, and its weights, while the first runs
+    _call("experts (down)", None, 0, ex.down, ex.dims, ex.width, plan, rows, out, None, 0, 0.0, act, pdl=True)

@@ -87,7 +87,7 @@ def test_c_abi_refuses_before_launching():
 
     def experts(**kw):
         a = dict(x=x, ldx=128, slots=2, w=w, stride=1 << 16, experts=4, n=64, k=128, items=work, counts=work, members=work, pairs=8, max_items=8,
-                 tile=16, out=out, ldo=64, f32=0, operands=None, epi=0, limit=0.0, work=None, bytes=0)
+                 tile=16, out=out, ldo=64, f32=0, operands=None, epi=0, limit=0.0, work=None, bytes=0, pdl=0)
         a.update(kw)
         return lib.tf_mx_experts(*a.values(), None)
 

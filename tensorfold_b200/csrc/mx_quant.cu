@@ -53,33 +53,35 @@ struct Piece {
   }
 };
 
-// Rows to stored words and scales.  A lane takes eight values, four lanes a block, so loads and stores of a warp are runs; U
-// pieces a thread are in flight at once.  Rows one after another (FLAT) are one run of pieces; others go by blockIdx.y.
-template <int DTYPE, bool FLAT, int U>
-__global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ x, int64_t ldx, int rows, int64_t pieces, uint32_t* __restrict__ words,
-                                                       uint8_t* __restrict__ scales) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+// Rows to stored words and scales.  A lane takes eight values, four lanes a block, so loads and stores of a warp are runs.  A thread
+// block takes 256 U neighbouring pieces of a run (rows one after another are one run, others one each, by blockIdx.y), its threads
+// U each, all in flight at once and at fixed distances: with 64-bit indexes made piece by piece a piece cost 96 instructions, more
+// than its bytes.
+template <int DTYPE, int U>
+__global__ void __launch_bounds__(256, DTYPE == 2 ? 4 : 6) quantize_kernel(const void* __restrict__ x, int64_t ld_bytes, int rows, int64_t pieces,
+                                                                           uint32_t* __restrict__ words, uint8_t* __restrict__ scales) {
+  constexpr int BYTES = DTYPE == 2 ? 32 : 16;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (256 * U);
+  const int64_t left = pieces - first;
+  const int here = left < 256 * U ? static_cast<int>(left) : 256 * U;
   for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-    const char* from = static_cast<const char*>(x) + (FLAT ? 0 : row * ldx * (DTYPE == 2 ? 4 : 2));
-    // whole warps walk together: a piece past the end computes on zeros and stores nothing
-    for (int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + (threadIdx.x & ~31); first < pieces; first += U * step) {
-      Piece<DTYPE> v[U];
+    const char* from = static_cast<const char*>(x) + row * ld_bytes + (first + threadIdx.x) * BYTES;
+    const int64_t to = row * pieces + first + threadIdx.x;
+    uint32_t* w = words + to;
+    uint8_t* sc = scales + (to >> 2);
+    Piece<DTYPE> v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t i = first + u * step + (threadIdx.x & 31);
-        if (i < pieces) v[u].load(from, i);
-        else v[u].clear();
-      }
+    for (int u = 0; u < U; ++u) {                              // (whole warps: a piece past the end is zeros and stores nothing)
+      if (static_cast<int>(threadIdx.x) + 256 * u < here) v[u].load(from, 256 * u);
+      else v[u].clear();
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t i = first + u * step + (threadIdx.x & 31);
-        uint32_t scale;
-        const uint32_t codes = v[u].quantize(scale);
-        if (i < pieces) {
-          const int64_t to = FLAT ? i : row * pieces + i;
-          words[to] = codes;
-          if ((i & 3) == 0) scales[to >> 2] = static_cast<uint8_t>(scale);
-        }
+    for (int u = 0; u < U; ++u) {
+      uint32_t scale;
+      const uint32_t codes = v[u].quantize(scale);
+      if (static_cast<int>(threadIdx.x) + 256 * u < here) {
+        w[256 * u] = codes;
+        if ((threadIdx.x & 3) == 0) sc[64 * u] = static_cast<uint8_t>(scale);
       }
     }
   }
@@ -87,55 +89,57 @@ __global__ void __launch_bounds__(256) quantize_kernel(const void* __restrict__ 
 
 // Stored words and scales to values, exact in bf16 and fp32 (2^127 times 2 and more overflows).  An e2m1 magnitude m, three
 // bits, moved to the top of a fraction field reads as value * 2^-126 (two exponent bits and one of fraction, subnormals alike), so
-// two products by powers of two make the value; in bf16 two values go at once.
+// two products by powers of two make the value; in bf16 two values go at once.  Pieces as above.
 template <int OUT, int U>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ words, const uint8_t* __restrict__ scales, int64_t pieces,
                                                          void* __restrict__ out) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; first < pieces; first += U * step) {
-    uint32_t w[U], code[U];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (256 * U);
+  const int64_t left = pieces - first;
+  const int here = left < 256 * U ? static_cast<int>(left) : 256 * U;
+  const int64_t at = first + threadIdx.x;
+  words += at, scales += at >> 2;
+  char* to = static_cast<char*>(out) + at * (OUT == 2 ? 32 : 16);
+  uint32_t w[U], code[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t i = first + u * step;
-      w[u] = i < pieces ? words[i] : 0u;
-      code[u] = i < pieces ? scales[i >> 2] : 0u;
-    }
+  for (int u = 0; u < U; ++u) {
+    const bool live = static_cast<int>(threadIdx.x) + 256 * u < here;
+    w[u] = live ? words[256 * u] : 0u;
+    code[u] = live ? scales[64 * u] : 0u;
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t i = first + u * step;
-      if (i >= pieces) break;
-      if (OUT == 0) {
-        const uint32_t s1 = code[u] == 255u ? 0x7FC0u : code[u] == 0u ? 0x0040u : code[u] << 7, s2 = s1 | (s1 << 16), lift2 = 0x7E807E80u;
-        const __nv_bfloat162 lift = *reinterpret_cast<const __nv_bfloat162*>(&lift2), scale = *reinterpret_cast<const __nv_bfloat162*>(&s2);
-        uint32_t p[4];                                               // values j and j + 4
+  for (int u = 0; u < U; ++u) {
+    if (static_cast<int>(threadIdx.x) + 256 * u >= here) break;
+    if (OUT == 0) {
+      const uint32_t s1 = code[u] == 255u ? 0x7FC0u : code[u] == 0u ? 0x0040u : code[u] << 7, s2 = s1 | (s1 << 16), lift2 = 0x7E807E80u;
+      const __nv_bfloat162 lift = *reinterpret_cast<const __nv_bfloat162*>(&lift2), scale = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+      uint32_t p[4];                                                 // values j and j + 4
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t q = w[u] >> (4 * j), bits = ((q & 0x00070007u) << 6) | ((q & 0x00080008u) << 12);
+        const __nv_bfloat162 t = __hmul2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), lift), scale);
+        p[j] = *reinterpret_cast<const uint32_t*>(&t);
+      }
+      reinterpret_cast<uint4*>(to)[256 * u] = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
+                                                         __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
+    } else {
+      const float scale = __uint_as_float(code[u] == 255u ? 0x7FC00000u : code[u] == 0u ? 0x00400000u : code[u] << 23);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t q = w[u] >> (4 * j);
+        v[j] = __uint_as_float(((q & 7u) << 22) | ((q & 8u) << 28)) * 0x1p126f * scale;
+      }
+      if (OUT == 2) {
+        float4* o = reinterpret_cast<float4*>(to) + 512 * u;
+        o[0] = make_float4(v[0], v[1], v[2], v[3]), o[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        uint32_t p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t q = w[u] >> (4 * j), bits = ((q & 0x00070007u) << 6) | ((q & 0x00080008u) << 12);
-          const __nv_bfloat162 t = __hmul2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), lift), scale);
+          const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
           p[j] = *reinterpret_cast<const uint32_t*>(&t);
         }
-        static_cast<uint4*>(out)[i] = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
-                                                 __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
-      } else {
-        const float scale = __uint_as_float(code[u] == 255u ? 0x7FC00000u : code[u] == 0u ? 0x00400000u : code[u] << 23);
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t q = w[u] >> (4 * j);
-          v[j] = __uint_as_float(((q & 7u) << 22) | ((q & 8u) << 28)) * 0x1p126f * scale;
-        }
-        if (OUT == 2) {
-          float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + i * 8);
-          o[0] = make_float4(v[0], v[1], v[2], v[3]), o[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-          uint32_t p[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            p[j] = *reinterpret_cast<const uint32_t*>(&t);
-          }
-          static_cast<uint4*>(out)[i] = make_uint4(p[0], p[1], p[2], p[3]);
-        }
+        reinterpret_cast<uint4*>(to)[256 * u] = make_uint4(p[0], p[1], p[2], p[3]);
       }
     }
   }
@@ -297,11 +301,14 @@ int tf_mx_quantize(const void* x, int64_t ldx, int dtype, int rows, int k, void*
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint32_t* w = static_cast<uint32_t*>(words);
   uint8_t* s = static_cast<uint8_t*>(scales);
-#define TF_MX_QUANTIZE(DT)                                                                                                            \
-  if (dtype == DT) {                                                                                                                  \
-    if (!flat) quantize_kernel<DT, false, 1><<<dim3((k / 8 + 255) / 256, std::min(rows, 65535)), 256, 0, st>>>(x, ldx, rows, k / 8, w, s); \
-    else if (pieces < MANY) quantize_kernel<DT, true, 1><<<blocks_for(pieces), 256, 0, st>>>(x, ldx, 1, pieces, w, s);                 \
-    else quantize_kernel<DT, true, 4><<<blocks_for((pieces + 3) / 4), 256, 0, st>>>(x, ldx, 1, pieces, w, s);                          \
+  const int64_t run = flat ? pieces : k / 8, total = pieces;
+  const int64_t ld = ldx * (dtype == 2 ? 4 : 2);
+  if (total / 256 > INT32_MAX) return fail_moe(TF_ERR_ARG, "tf_mx_quantize: too many values");
+#define TF_MX_QUANTIZE(DT)                                                                                                       \
+  if (dtype == DT) {                                                                                                             \
+    const dim3 grid(static_cast<unsigned>((run + (total < MANY ? 255 : 1023)) / (total < MANY ? 256 : 1024)), flat ? 1 : std::min(rows, 65535)); \
+    if (total < MANY) quantize_kernel<DT, 1><<<grid, 256, 0, st>>>(x, ld, flat ? 1 : rows, run, w, s);                            \
+    else quantize_kernel<DT, 4><<<grid, 256, 0, st>>>(x, ld, flat ? 1 : rows, run, w, s);                                         \
   }
   TF_MX_QUANTIZE(0) TF_MX_QUANTIZE(1) TF_MX_QUANTIZE(2)
 #undef TF_MX_QUANTIZE
@@ -317,10 +324,11 @@ int tf_mx_dequantize(const void* words, const void* scales, int rows, int k, int
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint32_t* w = static_cast<const uint32_t*>(words);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
-#define TF_MX_DEQUANTIZE(OUT)                                                                                             \
-  if (out_type == OUT) {                                                                                                  \
-    if (pieces < MANY) dequantize_kernel<OUT, 1><<<blocks_for(pieces), 256, 0, st>>>(w, s, pieces, out);                   \
-    else dequantize_kernel<OUT, 4><<<blocks_for((pieces + 3) / 4), 256, 0, st>>>(w, s, pieces, out);                       \
+  if (pieces / 256 > INT32_MAX) return fail_moe(TF_ERR_ARG, "tf_mx_dequantize: too many values");
+#define TF_MX_DEQUANTIZE(OUT)                                                                                                  \
+  if (out_type == OUT) {                                                                                                       \
+    if (pieces < MANY) dequantize_kernel<OUT, 1><<<static_cast<unsigned>((pieces + 255) / 256), 256, 0, st>>>(w, s, pieces, out); \
+    else dequantize_kernel<OUT, 4><<<static_cast<unsigned>((pieces + 1023) / 1024), 256, 0, st>>>(w, s, pieces, out);            \
   }
   TF_MX_DEQUANTIZE(0) TF_MX_DEQUANTIZE(1) TF_MX_DEQUANTIZE(2)
 #undef TF_MX_DEQUANTIZE

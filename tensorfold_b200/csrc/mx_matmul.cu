@@ -94,24 +94,52 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t atom_bytes, uin
 }
 constexpr uint32_t SWIZZLE_NONE = 0, SWIZZLE_128 = 2, SWIZZLE_32 = 6;
 
-// e2m1 x e2m1 with power-of-two scales per 32 inputs, K = 64, M = 128.  `half`: which two of a line's four scales.
+// e2m1 x e2m1 with power-of-two scales per 32 inputs, K = 64, M = 128 (256 for a pair).  `half`: which two of a line's four scales.
+template <bool PAIR>
 __device__ __forceinline__ uint32_t instruction(int n, uint32_t half) {
-  return (half * 2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (1u << 27) | (half * 2u << 29);
+  return (half * 2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | ((PAIR ? 2u : 1u) << 27) | (half * 2u << 29);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-      : "memory");
+  if constexpr (PAIR) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+  }
 }
-// 32 lines of 16 bytes to four columns, the same in each of the four lane groups.
+// 32 lines of 16 bytes to four columns, the same in each of the four lane groups (a pair: each block's own lines to its own columns).
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t from) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(from) : "memory");
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(from) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(from) : "memory");
 }
+// Arrives once every MMA and copy issued so far is done; for a pair on that barrier of both blocks.
+template <bool PAIR>
 __device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+  else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
+  uint32_t to;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(addr), "r"(rank));
+  return to;
+}
+// (A release at cluster scope would wait for the memory system each time; what these arrivals order, landed copies and tensor memory
+// that has been read, is ordered by the barrier and the tcgen05 fence before them.)
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool elect_lane() {
   uint32_t one;
@@ -181,10 +209,11 @@ __host__ __device__ __forceinline__ int quads_of(int rows, int c) { return ((row
 // silu(gate) * up in fp32.
 __device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 
-template <int NT, bool FUSED, bool GROUPED>
+template <int NT, bool FUSED, bool GROUPED, bool PAIR = false>
 struct MxShape {
   static constexpr int SBS = (NT + MX_SB - 1) / MX_SB;
-  static constexpr int B_BYTES = NT * 128 + SBS * MX_SCALES;
+  static constexpr int B_ROWS = PAIR ? NT / 2 : NT;                // rows of the tile in this block's shared memory
+  static constexpr int B_BYTES = B_ROWS * 128 + SBS * MX_SCALES;
   static constexpr int SLOT = MX_UNIT + (FUSED ? 0 : B_BYTES);
   static constexpr int SF_COLS = 8 + 8 * SBS;                      // scale columns of a slot
   static constexpr int TMEM = FUSED ? 256 : 512;
@@ -204,9 +233,10 @@ struct Ring {
   }
 };
 
-template <int NT, bool FUSED, bool GROUPED>
-__global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_kernel(const MxParams p) {
-  using S = MxShape<NT, FUSED, GROUPED>;
+template <int NT, bool FUSED, bool GROUPED, bool PAIR>
+__global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1) mx_kernel(const MxParams p) {
+  using S = MxShape<NT, FUSED, GROUPED, PAIR>;
+  static_assert(!PAIR || (!FUSED && !GROUPED), "pairs are for prompts");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);              // [MX_RING_MAX] the slot's copies have landed
@@ -226,7 +256,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
   const uint32_t full32 = smem_addr(full), empty32 = smem_addr(empty), acc_full32 = smem_addr(acc_full), acc_empty32 = smem_addr(acc_empty);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-  const int c = GROUPED ? 1 : p.cluster;
+  const int c = GROUPED || PAIR ? 1 : p.cluster;
   const int full_stages = p.steps >> 2, tail = p.steps & 3;
   uint32_t rank, mine, clusters;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -250,7 +280,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
   // neighbours, so that its rows are quantised once an item.
   if (GROUPED && !p.settled) pdl_wait();                           // the plan may be the previous kernel's output
   constexpr bool RUNS = FUSED && GROUPED;
-  const int ncb = (p.N + MX_SB - 1) / MX_SB;
+  const int nsb = (p.N + MX_SB - 1) / MX_SB, ncb = PAIR ? (nsb + 1) / 2 : nsb;
   const int tiles = ncb * (GROUPED ? min(p.counts[0], p.max_items) : p.row_tiles);
   const int first_tile = RUNS ? static_cast<int>(static_cast<int64_t>(tiles) * mine / clusters) : mine;
   const int end_tile = RUNS ? static_cast<int>(static_cast<int64_t>(tiles) * (mine + 1) / clusters) : tiles;
@@ -259,7 +289,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
   // A tile is looked up one ahead: `after` starts the loads of the plan's item, `settle` uses what they brought.
   struct Tile {
     int t;                                                         // number of the tile
-    int y, cb;                                                     // item or row tile, column block
+    int y, cb;                                                     // item or row tile, column block (of a pair: two super-blocks)
     int expert, from, count;                                       // the item as it stands in the plan
     int m0, rows, n;                                               // first row (or member), rows, MMA N
     int64_t w;                                                     // offset of the weights
@@ -271,7 +301,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
     }
   };
   auto settle = [&](Tile& ti) {
-    ti.w = ti.cb * p.sb_bytes;
+    ti.w = (PAIR ? min(2 * ti.cb + static_cast<int>(rank), nsb - 1) : ti.cb) * p.sb_bytes;
     if (GROUPED) {
       // an item that names an expert outside the table runs against expert 0 with no rows (the weights' thread reports it)
       const bool known = ti.expert >= 0 && ti.expert < p.experts;
@@ -283,7 +313,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
       ti.m0 = ti.y * p.tile;
       ti.rows = min(p.tile, p.M - ti.m0);
     }
-    ti.n = max(8, (ti.rows + 7) & ~7);
+    ti.n = PAIR ? (ti.rows + 15) & ~15 : max(8, (ti.rows + 7) & ~7);
   };
   auto first = [&]() {
     Tile ti = {};
@@ -380,9 +410,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
   const bool drains = warp >= 4 && group < S::GROUPS;
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < MX_RING_MAX; ++i) mbar_init(full + i, FUSED ? 1 : 2), mbar_init(empty + i, 1);
+      for (int i = 0; i < MX_RING_MAX; ++i) mbar_init(full + i, FUSED ? 1 : PAIR && rank == 0 ? 3 : 2), mbar_init(empty + i, 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, 4 * S::GROUPS);
+        mbar_init(acc_full + i, 1), mbar_init(acc_empty + i, (PAIR ? 8 : 4) * S::GROUPS);
         mbar_init(op_full + i, 4), mbar_init(op_empty + i, 1);
       }
       mbar_init(parts, 1);
@@ -397,7 +427,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
     }
     __syncwarp();
     asm volatile("barrier.cta.arrive 4, %0;" ::"n"(S::THREADS) : "memory");
-    if (c > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (c > 1 || PAIR) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     // ------------------------------------------------------------------ weights
     if (!GROUPED && !p.settled) pdl_wait();
     if (lane == 0) {
@@ -410,10 +440,15 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
       }
     }
     __syncwarp();
-    if (c > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (c > 1 || PAIR) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(S::TMEM) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   } else if (FUSED && !GROUPED && !drains) {
     pdl_wait();
     quantize_rows(smem + (operand0 - smem_addr(smem)), p.M, warp >= 8 ? warp - 8 : warp + 2, 6, [](int r) { return static_cast<int64_t>(r); });
@@ -424,7 +459,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
     asm volatile("barrier.cta.sync 4, %0;" ::"n"(S::THREADS) : "memory");
     // The other blocks run, and their barriers are there, before anything is sent to them.  Warp 0's arrival releases the barriers;
     // the others' are relaxed: a release beside the weights' copies took as long as those, 1 to 4 us.
-    if (c > 1) {
+    if (c > 1 || PAIR) {
       asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
       asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
@@ -451,23 +486,42 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
           const uint32_t bar = full32 + 8 * r.slot, dst = ring0 + r.slot * S::SLOT + MX_UNIT;
           r.next(p.ring);
           ready = lane_test(empty32 + 8 * r.slot, r.phase);
+          // a pair: half of the rows to each block, all scales to both
+          const int rows_here = PAIR ? ti.n / 2 : ti.n, skip = PAIR ? static_cast<int>(rank) * rows_here : 0;
           if (u < full_stages) {
-            mbar32_expect_tx(bar, ti.n * 128 + sbs * MX_SCALES);
-            bulk_load32(dst, src, ti.n * 128, bar);
-            bulk_load32(dst + NT * 128, src + p.b_rows * 128, sbs * MX_SCALES, bar);
+            mbar32_expect_tx(bar, rows_here * 128 + sbs * MX_SCALES);
+            bulk_load32(dst, src + skip * 128, rows_here * 128, bar);
+            bulk_load32(dst + S::B_ROWS * 128, src + p.b_rows * 128, sbs * MX_SCALES, bar);
           } else {
             const uint32_t scales = sbs * mx_tail_scales(tail);
-            mbar32_expect_tx(bar, ti.n * 32 * tail + scales);
-            for (int j = 0; j < tail; ++j) bulk_load32(dst + j * NT * 32, src + j * p.b_rows * 32, ti.n * 32, bar);
-            bulk_load32(dst + NT * 128, src + tail * p.b_rows * 32, scales, bar);
+            mbar32_expect_tx(bar, rows_here * 32 * tail + scales);
+            for (int j = 0; j < tail; ++j) bulk_load32(dst + j * S::B_ROWS * 32, src + (j * p.b_rows + skip) * 32, rows_here * 32, bar);
+            bulk_load32(dst + S::B_ROWS * 128, src + tail * p.b_rows * 32, scales, bar);
           }
         }
       }
       if (!ok) lost(ERR_WAIT_EMPTY), let_copies_land();
     }
     __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issue
+  } else if (PAIR && warp == 3 && rank == 1) {
+    // ------------------------------------------------------------------ this block's copies have landed: tell the first block
+    if (elect_lane()) {
+      const uint32_t first_full = in_block(full32, 0);
+      bool ok = true;
+      Ring r = {0, 0u};
+      for (Tile ti = first(); ti.t < end_tile && ok; ti = after(ti)) {
+#pragma unroll 1
+        for (int u = u0; u < u1; ++u) {
+          if (!(ok = lane_wait(full32 + 8 * r.slot, r.phase, abort_word))) break;
+          arrive_remote(first_full + 8 * r.slot);
+          r.next(p.ring);
+        }
+      }
+      if (!ok) lost(ERR_WAIT_FULL);
+    }
+    __syncwarp();
+  } else if (warp == 1 && (!PAIR || rank == 0)) {
+    // ------------------------------------------------------------------ MMA issue (a pair's by its first block)
     // Measured on one block: an MMA of N columns takes N / 2 cycles but no less than 40 to issue, a scale copy 10 beside MMAs and
     // 37 alone, a commit 34 alone, a wait that passes 110.  The pipe takes few instructions ahead of it, so what a stage costs this
     // thread beyond them shows: descriptors are kept to adds, the next stage's barrier is tested before this stage's MMAs, and
@@ -476,7 +530,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
       const uint32_t sf0 = tmem + 2 * NT;
       const uint64_t a0 = desc(ring0, 1024, SWIZZLE_128), as0 = desc(ring0 + MX_SB * 128, 128, SWIZZLE_NONE);
       const uint64_t b0 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 1024, SWIZZLE_128);
-      const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + NT * 128, 128, SWIZZLE_NONE);
+      const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + S::B_ROWS * 128, 128, SWIZZLE_NONE);
       bool ok = true;
       Ring r = {0, 0u};
       int use = 0, op = GROUPED ? -1 : 0, last_y = -1;
@@ -489,7 +543,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
           if (!(ok = lane_wait(smem_addr(op_full + op % p.bufs), (op / p.bufs) & 1, abort_word))) break;
         }
         const int buf = RUNS ? op % p.bufs : 0;
-        const uint32_t id0 = instruction(n, 0), id1 = instruction(n, 1);
+        const uint32_t id0 = instruction<PAIR>(n, 0), id1 = instruction<PAIR>(n, 1);
         for (int s = slice0; s < slice1 && ok; ++s, ++use) {
           const int start = p.bounds[s], end = p.bounds[s + 1], last_whole = min(end, full_stages);
           if (use >= 2 && !(ok = lane_wait(acc_empty32 + 8 * (use & 1), ((use >> 1) - 1) & 1, abort_word))) break;
@@ -506,15 +560,15 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
             ready = lane_test(full32 + 8 * r.slot, r.phase);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              copy_scales(sa + 4 * h, as0 + at + 32 * h);
+              copy_scales<PAIR>(sa + 4 * h, as0 + at + 32 * h);
 #pragma unroll
-              for (int q = 0; q < S::SBS; ++q) copy_scales(sb + 4 * S::SBS * h + 4 * q, bs0 + bt + (MX_SCALES >> 4) * q + 32 * h);
+              for (int q = 0; q < S::SBS; ++q) copy_scales<PAIR>(sb + 4 * S::SBS * h + 4 * q, bs0 + bt + (MX_SCALES >> 4) * q + 32 * h);
             }
-            mma_mxf4(d, a0 + at, b0 + bt, id0, sa, sb, more);
-            mma_mxf4(d, a0 + at + 2, b0 + bt + 2, id1, sa, sb, 1u);
-            mma_mxf4(d, a0 + at + 4, b0 + bt + 4, id0, sa + 4, sb + 4 * S::SBS, 1u);
-            mma_mxf4(d, a0 + at + 6, b0 + bt + 6, id1, sa + 4, sb + 4 * S::SBS, 1u);
-            commit(done);
+            mma_mxf4<PAIR>(d, a0 + at, b0 + bt, id0, sa, sb, more);
+            mma_mxf4<PAIR>(d, a0 + at + 2, b0 + bt + 2, id1, sa, sb, 1u);
+            mma_mxf4<PAIR>(d, a0 + at + 4, b0 + bt + 4, id0, sa + 4, sb + 4 * S::SBS, 1u);
+            mma_mxf4<PAIR>(d, a0 + at + 6, b0 + bt + 6, id1, sa + 4, sb + 4 * S::SBS, 1u);
+            commit<PAIR>(done);
             more = 1;
             if (FUSED) fused_at += S::B_BYTES >> 4;
           }
@@ -525,21 +579,21 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
             const uint32_t sb_bytes = FUSED ? MX_SCALES : mx_tail_scales(tail), sa = sf0 + r.slot * S::SF_COLS, sb = sa + 8;
 #pragma unroll 1
             for (int h = 0; 2 * h < tail; ++h) {
-              copy_scales(sa + 4 * h, desc(a + tail * 4096 + 512 * h, 128, SWIZZLE_NONE));
+              copy_scales<PAIR>(sa + 4 * h, desc(a + tail * 4096 + 512 * h, 128, SWIZZLE_NONE));
               for (int q = 0; q < S::SBS; ++q)
-                copy_scales(sb + 4 * S::SBS * h + 4 * q, desc(b + NT * 128 + q * sb_bytes + 512 * h, 128, SWIZZLE_NONE));
+                copy_scales<PAIR>(sb + 4 * S::SBS * h + 4 * q, desc(b + S::B_ROWS * 128 + q * sb_bytes + 512 * h, 128, SWIZZLE_NONE));
             }
 #pragma unroll 1
             for (int j = 0; j < tail; ++j)
-              mma_mxf4(d, desc(a + j * 4096, 256, SWIZZLE_32), desc(b + j * NT * 32, 256, SWIZZLE_32), j & 1 ? id1 : id0, sa + 4 * (j >> 1),
+              mma_mxf4<PAIR>(d, desc(a + j * 4096, 256, SWIZZLE_32), desc(b + j * S::B_ROWS * 32, 256, SWIZZLE_32), j & 1 ? id1 : id0, sa + 4 * (j >> 1),
                        sb + 4 * S::SBS * (j >> 1), more | (j > 0));
-            commit(empty32 + 8 * r.slot);
+            commit<PAIR>(empty32 + 8 * r.slot);
             r.next(p.ring);
             ready = 0;
           }
-          commit(acc_full32 + 8 * (use & 1));
+          commit<PAIR>(acc_full32 + 8 * (use & 1));
         }
-        if (RUNS && ok && (then.t >= end_tile || then.y != y)) commit(smem_addr(op_empty + buf));
+        if (RUNS && ok && (then.t >= end_tile || then.y != y)) commit<PAIR>(smem_addr(op_empty + buf));
       }
       if (!ok) lost(ERR_WAIT_FULL);
     }
@@ -567,6 +621,12 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
   if (drains) {
     // ------------------------------------------------------------------ drain
     const int lg = warp & 3;
+    const uint32_t empty_at = PAIR ? in_block(acc_empty32, 0) : acc_empty32;
+    auto release = [&](int acc) {                                    // an accumulator has been read
+      if constexpr (PAIR) arrive_remote(empty_at + 8 * acc);
+      else mbar32_arrive(empty_at + 8 * acc);
+    };
+    auto block_of = [&](const Tile& ti) { return PAIR ? 2 * ti.cb + static_cast<int>(rank) : ti.cb; };
     const bool gated = p.epi == MX_SWIGLU;
     const int ncols = gated ? p.N / 2 : p.N;
     const bool wide = !p.out_f32 && (ncols & 7) == 0 && (p.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
@@ -716,7 +776,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + (use & 1));
+            if (lane == 0) release(use & 1);
           }
         } else {
           ok = warp_wait(acc_full32 + 8 * (use & 1), (use >> 1) & 1, abort_word);
@@ -784,9 +844,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
         if (GROUPED && p.q != nullptr) {
           quantize16(own, v, n);
         } else if (gated) {
-          store(std::integral_constant<int, 1>(), own, v, n + (lane < 16 ? 0 : 8), ti.cb * 64 + lg * 16 + (lane & 15));
+          store(std::integral_constant<int, 1>(), own, v, n + (lane < 16 ? 0 : 8), block_of(ti) * 64 + lg * 16 + (lane & 15));
         } else {
-          store(std::integral_constant<int, 2>(), own, v, n, ti.cb * MX_SB + lg * 32 + lane);
+          store(std::integral_constant<int, 2>(), own, v, n, block_of(ti) * MX_SB + lg * 32 + lane);
         }
       }
       if (rehearsal) {
@@ -799,7 +859,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + (use & 1));
+      if (lane == 0) release(use & 1);
       ++use;
       if (c > 1) break;                                              // (one tile a cluster)
       ti = GROUPED ? then : after(ti);
@@ -811,10 +871,15 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (PAIR) {                                                        // neither block leaves before both are done
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM) : "memory");
   }
 }
 
@@ -824,11 +889,13 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED>::THREADS, 1) mx_ke
 
 int g_mx_sms[64] = {};
 
-int device_sms() {
+int g_mx_pairs[64] = {};            // pairs of blocks a device runs at once
+
+int current_device() {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  return g_mx_sms[dev];
+  return cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 ? 63 : dev;
 }
+int device_sms() { return g_mx_sms[current_device()]; }
 
 // K slices of an (n, k) weight: enough (128-column block, slice) units for one block an SM, no slice below two stages.
 int slices_for(int n, int k) {
@@ -836,9 +903,9 @@ int slices_for(int n, int k) {
   return std::max(1, std::min({MX_CLUSTER_MAX, 148 / std::min(blocks, 148), stages / 2}));
 }
 
-template <int NT, bool FUSED, bool GROUPED>
+template <int NT, bool FUSED, bool GROUPED, bool PAIR = false>
 cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStream_t stream) {
-  using S = MxShape<NT, FUSED, GROUPED>;
+  using S = MxShape<NT, FUSED, GROUPED, PAIR>;
   int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
   if (p.cluster > 1) extra = p.cluster * quads_of(std::min(p.tile, p.M), p.cluster) * MX_SB * 16;
   const int operand = FUSED ? p.operand_stages * S::B_BYTES : 0;
@@ -847,17 +914,18 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStre
   p.ring = std::min(S::RING, room / S::SLOT);
   if (p.ring < 2) return cudaErrorInvalidConfiguration;              // (the callers' rules keep shapes that would not fit out)
   for (int i = 0; i <= p.sk; ++i) p.bounds[i] = static_cast<int>(static_cast<int64_t>(p.stages) * i / p.sk);
-  const int64_t most = std::max(1, sms / p.cluster);
+  const int width = PAIR ? 2 : p.cluster;                            // blocks of a cluster
+  const int64_t most = PAIR ? std::max(1, g_mx_pairs[current_device()]) : std::max(1, sms / p.cluster);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.cluster > 1 ? tiles : std::min(tiles, most)) * p.cluster));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.cluster > 1 ? tiles : std::min(tiles, most)) * width));
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = 1024 + MX_BAR_BYTES + p.ring * S::SLOT + p.bufs * operand + extra;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
   int count = 0;
-  if (p.cluster > 1) {
+  if (width > 1) {
     attrs[count].id = cudaLaunchAttributeClusterDimension;
-    attrs[count].val.clusterDim.x = p.cluster, attrs[count].val.clusterDim.y = 1, attrs[count].val.clusterDim.z = 1;
+    attrs[count].val.clusterDim.x = width, attrs[count].val.clusterDim.y = 1, attrs[count].val.clusterDim.z = 1;
     ++count;
   }
   // always: a block sets up under the previous kernel's end, and reads and writes global memory once that is done (weights and plan
@@ -867,12 +935,12 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStre
   ++count;
   cfg.attrs = attrs;
   cfg.numAttrs = count;
-  return cudaLaunchKernelEx(&cfg, mx_kernel<NT, FUSED, GROUPED>, p);
+  return cudaLaunchKernelEx(&cfg, mx_kernel<NT, FUSED, GROUPED, PAIR>, p);
 }
 
-template <int NT, bool FUSED, bool GROUPED>
+template <int NT, bool FUSED, bool GROUPED, bool PAIR = false>
 cudaError_t configure() {
-  return cudaFuncSetAttribute(mx_kernel<NT, FUSED, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  return cudaFuncSetAttribute(mx_kernel<NT, FUSED, GROUPED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
 }
 
 // Rows come as operands: the kernel whose tiles hold `tile` rows.
@@ -882,6 +950,24 @@ cudaError_t launch_rows(MxParams& p, int64_t tiles, int sms, cudaStream_t stream
   if (p.tile <= 128) return launch<128, false, false>(p, tiles, false, sms, stream);
   return launch<192, false, false>(p, tiles, false, sms, stream);
 }
+// Two blocks on an SM pair share a tile of 256 columns.
+cudaError_t launch_pairs(MxParams& p, int64_t row_tiles, int sms, cudaStream_t stream) {
+  return launch<MX_TILE_MAX, false, false, true>(p, ((p.N + MX_SB - 1) / MX_SB + 1) / 2 * row_tiles, false, sms, stream);
+}
+cudaError_t pairs_resident(int* pairs) {
+  cudaError_t e = configure<MX_TILE_MAX, false, false, true>();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(MxShape<MX_TILE_MAX, false, false, true>::THREADS);
+  cfg.dynamicSmemBytes = 232448;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(pairs, mx_kernel<MX_TILE_MAX, false, false, true>, &cfg);
+}
 cudaError_t launch_items(MxParams& p, int64_t tiles, int sms, cudaStream_t stream) {
   return p.tile <= 16 ? launch<16, false, true>(p, tiles, p.q != nullptr, sms, stream)
                       : launch<128, false, true>(p, tiles, p.q != nullptr, sms, stream);
@@ -889,26 +975,31 @@ cudaError_t launch_items(MxParams& p, int64_t tiles, int sms, cudaStream_t strea
 
 int round8(int m) { return (m + 7) / 8 * 8; }
 
-// Rows of a tile of an m-row call, and blocks that share a tile (all K slices or one): the fewest cycles by a plain model.  A stage
-// takes 2 cycles a row of math, but no less than its copies (17 KB and 136 bytes a row, at COPY bytes a cycle); a tile has a start
+// Rows of a tile of an m-row call, blocks that share a tile (all K slices or one), and whether two blocks work as a pair: the fewest
+// cycles by a plain model.  What paces a stage is shared memory, 128 bytes a cycle: 17 KB of weights and 136 bytes a row come in, and
+// four MMAs read 16 KB and 128 bytes a row again; a pair halves the rows' part.  The math takes 2 cycles a row.  A tile has a start
 // and an end besides.
 struct Tiling {
   int tile, cluster;
+  bool pair;
 };
 Tiling tiling_for(int m, int n, int stages, int sk) {
-  constexpr int SMS = 148, COPY = 48, ENDS = 1500;
+  constexpr int SMS = 148;
+  constexpr double ENDS = 2500, STAGE = 270, ROW = 2.06;
   const int64_t ncb = (n + MX_SB - 1) / MX_SB;
-  Tiling best = {8, 1};
+  Tiling best = {8, 1, false};
   double cost = 1e30;
+  auto offer = [&](int64_t blocks, int waves_of, double work, Tiling t) {
+    const double here = static_cast<double>((blocks + waves_of - 1) / waves_of) * (work + ENDS);
+    if (here <= cost) cost = here, best = t;
+  };
   for (int t = 8; t <= MX_TILE_MAX; t += 8) {
-    const int64_t tiles = ncb * ((m + t - 1) / t);
-    for (int c = 1; c <= sk; c += sk > 1 ? sk - 1 : 1) {
-      if (c > 1 && t > MX_SB) continue;                              // (no room for the exchange beside the ring)
-      const int64_t waves = (tiles * c + SMS - 1) / SMS;
-      const double stage = std::max(2.0 * t, (MX_UNIT + 136.0 * t) / COPY);
-      const double here = waves * (stages / static_cast<double>(c) * stage + ENDS + (c > 1 ? ENDS : 0));
-      if (here <= cost) cost = here, best = {t, c};
-    }
+    const int64_t row_tiles = (m + t - 1) / t;
+    const double stage = std::max(2.0 * t, STAGE + ROW * t), paired = std::max(2.0 * t, STAGE + 16 + ROW / 2 * t);
+    offer(ncb * row_tiles, SMS, stages * stage, {t, 1, false});
+    // (taller tiles leave no room for the exchange beside the ring)
+    if (sk > 1 && t <= MX_SB) offer(ncb * row_tiles * sk, SMS, stages * stage / sk + ENDS, {t, sk, false});
+    if (t % 16 == 0 && m > MX_SB) offer((ncb + 1) / 2 * row_tiles, SMS / 2, stages * paired, {t, 1, true});
     if (t >= m) break;
   }
   return best;
@@ -943,7 +1034,9 @@ cudaError_t mx_configure(int device, int sms) {
   if (e == cudaSuccess) e = configure<128, false, false>();
   if (e == cudaSuccess) e = configure<128, false, true>();
   if (e == cudaSuccess) e = configure<192, false, false>();
-  if (e == cudaSuccess && device >= 0 && device < 64) g_mx_sms[device] = sms;
+  int pairs = 0;
+  if (e == cudaSuccess) e = pairs_resident(&pairs);
+  if (e == cudaSuccess && device >= 0 && device < 64) g_mx_sms[device] = sms, g_mx_pairs[device] = pairs;
   return e;
 }
 
@@ -1005,7 +1098,7 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
     p.settled = 1;                                                   // the rows' kernel waits before it lets this one start
     p.row_tiles = static_cast<int>(row_tiles);
-    e = launch_rows(p, ncb * row_tiles, sms, s);
+    e = t.pair ? launch_pairs(p, row_tiles, sms, s) : launch_rows(p, ncb * row_tiles, sms, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_matmul");
 }

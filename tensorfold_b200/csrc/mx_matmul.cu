@@ -203,6 +203,16 @@ __device__ __forceinline__ void store_remote(uint32_t addr, uint32_t bar, uint32
                : "memory");
 }
 
+// Whether `ok` holds in all 128 threads that meet at this barrier.
+__device__ __forceinline__ bool agreed(int barrier, bool ok) {
+  uint32_t all;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %2, 0;\nbarrier.cta.red.and.pred q, %1, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
+               : "=r"(all)
+               : "r"(barrier), "r"(static_cast<uint32_t>(ok))
+               : "memory");
+  return all != 0;
+}
+
 // Fours of rows each of the c blocks of a cluster owns when they add their slices.
 __host__ __device__ __forceinline__ int quads_of(int rows, int c) { return ((rows + 3) / 4 + c - 1) / c; }
 
@@ -221,6 +231,8 @@ struct MxShape {
   static constexpr int GROUPS = NT == 16 ? 1 : GROUPED ? 3 : 2;
   static constexpr int THREADS = 128 + 128 * (GROUPS > 2 ? GROUPS : 2);
   static constexpr int CHUNKS = (NT / 16 + GROUPS - 1) / GROUPS;   // runs of sixteen rows a group drains
+  // Slots: each has scale columns of its own.  (Pairs with seven slots in shared memory and five for scales, whose reuse the MMA
+  // thread then waits for, took 94 us for 2048 rows by 17408 x 5120 against 88.)
   static constexpr int RING = (TMEM - 2 * NT) / SF_COLS < MX_RING_MAX ? (TMEM - 2 * NT) / SF_COLS : MX_RING_MAX;
 };
 
@@ -782,6 +794,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
           ok = warp_wait(acc_full32 + 8 * (use & 1), (use >> 1) & 1, abort_word);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
+        if (GROUPED && p.q != nullptr) ok = agreed(1 + group, ok);   // (a group's warps meet at barriers below: all of them or none)
         if (!ok) break;
       }
       const uint32_t src = lanes + (use & 1) * NT;
@@ -1093,7 +1106,7 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     p.tile = p.b_rows = t.tile, p.cluster = t.cluster;
     p.b = static_cast<const uint8_t*>(work), p.item_stride = mx_operand_bytes(t.tile, p.steps);
     const int64_t row_tiles = (m + t.tile - 1) / t.tile;
-    if (ncb * row_tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: too many tiles");
+    if (row_tiles > 65535 || ncb * row_tiles > (1 << 28)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: too many rows");
     e = mx_rows_launch(x, ldx, m, k, t.tile, t.tile, p.item_stride, nullptr, nullptr, nullptr, 0, 0, 0, work, s);
     if (e != cudaSuccess) return cuda_fail_moe(e, "tf_mx_matmul: rows");
     p.settled = 1;                                                   // the rows' kernel waits before it lets this one start
@@ -1116,7 +1129,7 @@ int64_t tf_mx_experts_bytes(int k, int tile, int max_items) {
 int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
                   const int* counts, const int* members, int pairs, int max_items, int tile, void* out, int64_t ldo, int out_f32,
                   void* out_operands, int epi, float limit, void* work, int64_t work_bytes, int pdl, void* stream) {
-  if (experts < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || pairs < 1 || max_items < 1 || max_items > (1 << 20) || slots < 0)
+  if (experts < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || pairs < 1 || max_items < 1 || max_items > 65535 || slots < 0)
     return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad sizes (K a positive multiple of 32)");
   if (tile < 8 || tile > MX_SB || tile % 8) return fail_moe(TF_ERR_ARG, "tf_mx_experts: items of 8 to 128 pairs, in whole eights");
   if (epi < 0 || epi > 2 || (epi == 2 && n % 32)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad epilogue");

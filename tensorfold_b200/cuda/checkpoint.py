@@ -234,10 +234,50 @@ class Checkpoint:
         weight = parts[0].view(torch.int32) if parts[0].dtype == torch.uint32 else parts[0]
         return QLinear(weight, parts[1], parts[2], gs=gs, bits=bits)
 
+    def microscaled(self, prefix: str, *, device: torch.device | str = "cpu", rank: int = 0, world: int = 1, parallel: str | None = None,
+                    segments: Sequence[int] | None = None, block: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+        """``prefix``.weight (words) and .scales (bytes) of a microscaled 4-bit projection, the share of rank ``rank`` of ``world``
+        cut as ``linear`` cuts it ("row": whole blocks of 32 inputs).  (words int32 [n, k / 8], scales uint8 [n, k / 32])."""
+
+        names = [f"{prefix}.weight", f"{prefix}.scales"]
+        for name in names:
+            if name not in self.index:
+                raise KeyError(name)
+        w, s = (self.index[name] for name in names)
+        if len(w.shape) != 2 or w.dtype not in (torch.int32, torch.uint32) or s.dtype != torch.uint8 or s.shape != (w.shape[0], w.shape[1] // 4) \
+                or w.shape[1] % 4:
+            raise ValueError(f"{prefix}: weight {w.shape} and scales {s.shape} are not a microscaled projection")
+        n, blocks = w.shape[0], w.shape[1] // 4
+        if world < 1 or not 0 <= rank < world:
+            raise ValueError("rank outside the world")
+        if parallel not in (None, "column", "row"):
+            raise ValueError("parallel is None, 'column' or 'row'")
+        if parallel == "column" and world > 1:
+            lengths = tuple(segments) if segments is not None else (n,)
+            if sum(lengths) != n or any(v <= 0 or v % (world * block) for v in lengths):
+                raise ValueError(f"output segments {lengths} do not split into {world} blocks of {block}")
+            parts = []
+            for name in names:
+                runs, base = [], 0
+                for length in lengths:
+                    share = length // world
+                    runs.append(self.rows(name, base + rank * share, base + (rank + 1) * share, device))
+                    base += length
+                parts.append(runs[0] if len(runs) == 1 else torch.cat(runs))
+        else:
+            parts = [self.tensor(name, device) for name in names]
+            if parallel == "row" and world > 1:
+                if blocks % world:
+                    raise ValueError(f"{prefix}: {blocks} blocks of inputs do not divide across {world} ranks")
+                lo, hi = rank * blocks // world, (rank + 1) * blocks // world
+                parts = [parts[0][:, 4 * lo:4 * hi].contiguous(), parts[1][:, lo:hi].contiguous()]
+        return parts[0].view(torch.int32) if parts[0].dtype == torch.uint32 else parts[0], parts[1]
+
 
 def expert_tables(ckpt: Checkpoint, prefix: str, projections: Sequence[str] = ("gate_proj", "up_proj", "down_proj"), *,
-                  device: torch.device | str = "cpu", rank: int = 0, world: int = 1):
-    """A routed layer's expert tables ``prefix.<projection>.weight / .scales / .biases`` of shape [E, ...] as the
+                  device: torch.device | str = "cpu", rank: int = 0, world: int = 1,
+                  parts: Sequence[str] = ("weight", "scales", "biases")):
+    """A routed layer's expert tables ``prefix.<projection>.weight / .scales / .biases`` (``parts``) of shape [E, ...] as the
     experts rank ``rank`` of ``world`` owns, [rank E / world, (rank + 1) E / world): the experts are the tensors' first
     dimension, so a rank's share is one contiguous byte range per tensor and only that is read.  Returns
     ({projection: (words, scales, biases)}, first): what ``tp.shard_experts`` cuts from the whole tables
@@ -247,7 +287,7 @@ def expert_tables(ckpt: Checkpoint, prefix: str, projections: Sequence[str] = ("
         raise ValueError("rank outside the world")
     tables, first = {}, 0
     for proj in projections:
-        names = [f"{prefix}.{proj}.{part}" for part in ("weight", "scales", "biases")]
+        names = [f"{prefix}.{proj}.{part}" for part in parts]
         for name in names:
             if name not in ckpt:
                 raise KeyError(name)
@@ -255,9 +295,9 @@ def expert_tables(ckpt: Checkpoint, prefix: str, projections: Sequence[str] = ("
         if any(ckpt.index[name].shape[0] != e for name in names) or e % world:
             raise ValueError(f"{prefix}.{proj}: {e} experts do not divide across {world} ranks")
         first = rank * e // world
-        parts = [ckpt.rows(name, first, (rank + 1) * e // world, device) for name in names]
-        words = parts[0].view(torch.int32) if parts[0].dtype == torch.uint32 else parts[0]
-        tables[proj] = (words, parts[1], parts[2])
+        read = [ckpt.rows(name, first, (rank + 1) * e // world, device) for name in names]
+        words = read[0].view(torch.int32) if read[0].dtype == torch.uint32 else read[0]
+        tables[proj] = (words, *read[1:])
     return tables, first
 
 
@@ -280,4 +320,22 @@ def load_packed(ckpt: Checkpoint, prefix: str, device: torch.device | str, **kw)
     return qmm.pack(q.weight, q.scales, q.biases, q.gs, bits=q.bits)
 
 
-__all__ = ["ALIGN", "PIECE", "Spans", "read_header", "Entry", "Checkpoint", "expert_tables", "load_experts", "load_packed"]
+def load_microscaled(ckpt: Checkpoint, prefix: str, device: torch.device | str, **kw):
+    """The rank's shard of a microscaled 4-bit projection, uploaded and packed (``kernels.mx.pack``)."""
+
+    from .kernels import mx
+
+    return mx.pack(*ckpt.microscaled(prefix, device=device, **kw))
+
+
+def load_microscaled_experts(ckpt: Checkpoint, prefix: str, device: torch.device | str, *, rank: int = 0, world: int = 1, limit: float = 0.0):
+    """The rank's microscaled experts of a SwiGLU layer, uploaded and packed: (``mx_experts.Experts``, first)."""
+
+    from . import mx_experts
+
+    tables, first = expert_tables(ckpt, prefix, device=device, rank=rank, world=world, parts=("weight", "scales"))
+    return mx_experts.make([tables["gate_proj"], tables["up_proj"]], tables["down_proj"], limit=limit), first
+
+
+__all__ = ["ALIGN", "PIECE", "Spans", "read_header", "Entry", "Checkpoint", "expert_tables", "load_experts", "load_packed", "load_microscaled",
+           "load_microscaled_experts"]

@@ -62,6 +62,8 @@ def _call(who, x, slots, table, n, k, plan, rows, out, operands, epi, limit, wor
     pairs = rows * plan.slots
     if rows < 1 or pairs > plan.members.shape[0]:
         raise ValueError(f"{who}: 1 to {plan.rows} rows fit the plan")
+    if table.dtype != torch.uint8 or table.shape[1:] != (-(-n // 128), mx.super_block_bytes(k)) or not table[0].is_contiguous():
+        raise ValueError(f"{who}: the table does not have the super-blocks of its shape")
     if table.device != plan.items.device:
         raise ValueError(f"{who}: the plan and the weights must share a CUDA device")
     stream = _lib.stream_of(table)

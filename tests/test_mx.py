@@ -96,3 +96,41 @@ def test_c_abi_refuses_before_launching():
                dict(ldx=132), dict(stride=8), dict(ldo=32), dict(tile=128), dict(x=None), dict(epi=2, f32=1), dict(slots=-1)):
         assert experts(**kw) < 0, kw
     assert experts() != 0
+
+
+def stored(n, k, seed, lead=()):
+    codes, scales = mx_util.random_weight(n, k, seed, "cpu", lead=lead)
+    return {"weight": mx_util.to_words(codes).view(torch.uint32), "scales": scales.to(torch.uint8)}
+
+
+def test_checkpoint_shards(tmp_path):
+    """Words and scale bytes of a microscaled projection as each rank reads them."""
+
+    from tensorfold_b200.cuda import checkpoint
+    from test_checkpoint import write_safetensors
+
+    path = tmp_path / "model.safetensors"
+    src, table = stored(96, 256, 1), stored(32, 64, 2, lead=(4,))
+    write_safetensors(path, {**{f"q.{k}": v for k, v in src.items()}, **{f"moe.up_proj.{k}": v for k, v in table.items()},
+                             "bad.weight": src["weight"], "bad.scales": src["scales"][:, :4].contiguous()}, pad=2)
+    ckpt = checkpoint.Checkpoint([path])
+    words, scales = src["weight"].view(torch.int32), src["scales"]
+    whole = ckpt.microscaled("q")
+    assert torch.equal(whole[0], words) and torch.equal(whole[1], scales) and whole[0].dtype == torch.int32
+    for rank in range(2):
+        w, s = ckpt.microscaled("q", rank=rank, world=2, parallel="column", segments=(64, 32))
+        rows = torch.cat([torch.arange(32) + 32 * rank, torch.arange(16) + 64 + 16 * rank])
+        assert torch.equal(w, words[rows]) and torch.equal(s, scales[rows])
+        w, s = ckpt.microscaled("q", rank=rank, world=2, parallel="row")
+        assert torch.equal(w, words[:, 16 * rank:16 * rank + 16]) and torch.equal(s, scales[:, 4 * rank:4 * rank + 4])
+        tables, first = checkpoint.expert_tables(ckpt, "moe", ("up_proj",), rank=rank, world=2, parts=("weight", "scales"))
+        assert first == 2 * rank and torch.equal(tables["up_proj"][0], table["weight"].view(torch.int32)[first:first + 2])
+        assert torch.equal(tables["up_proj"][1], table["scales"][first:first + 2])
+    for kw in (dict(world=3, parallel="row"), dict(world=2, parallel="column", segments=(95, 1)), dict(rank=2, world=2), dict(parallel="diagonal")):
+        with pytest.raises(ValueError):
+            ckpt.microscaled("q", **kw)
+    with pytest.raises(ValueError):
+        ckpt.microscaled("bad")
+    with pytest.raises(KeyError):
+        ckpt.microscaled("none")
+    ckpt.close()

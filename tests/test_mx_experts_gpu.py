@@ -139,10 +139,11 @@ def test_ragged_plans(prefill):
     picks[:, 0] = 5
     picks[::7, 1] = 23
     picks[3, 2] = 0
+    picks[11, 1:] = 5                                          # the same expert in all three slots of a row
     act, y, whole = run(x, ex, picks, prefill)
     out = (picks.flatten() < 0)
     assert (act[out] == 3).all() and (y[out] == 3).all() and (whole[out] == 3).all()
-    for r in (0, 3, 7, 299):
+    for r in (0, 3, 7, 11, 299):
         alone = run(x[r:r + 1], ex, picks[r:r + 1], False)
         assert all(torch.equal(a, b[3 * r:3 * r + 3]) for a, b in zip(alone, (act, y, whole)))
     # fewer rows than the plan's buffers hold, nothing routed at all
@@ -257,6 +258,31 @@ def test_refusals():
                  lambda: mx_experts.layer(x, ex, plan, y, 0), lambda: mx_experts.gate_up(x, ex, plan, y, 4),
                  lambda: mx_experts.down(x, ex, plan, y, 4),
                  lambda: mx_experts.layer(x, ex, plan_of(picks_for(4, 2, 5, 1), ex.count + 1, False), y, 4),
-                 lambda: mx_experts.make([stored(up[0])], stored(up[0]))):
+                 lambda: mx_experts.make([stored(up[0])], stored(up[0])),
+                 lambda: mx_experts.layer(x, mx_experts.Experts(ex.up, ex.up, ex.width, ex.dims), plan, y, 4),
+                 lambda: mx_experts.layer(x, mx_experts.Experts(ex.up.cpu(), ex.down, ex.width, ex.dims), plan, y, 4)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_checkpoint_to_layer(tmp_path):
+    """A projection and a routed layer read from safetensors are those packed from the whole tensors."""
+
+    from tensorfold_b200.cuda import checkpoint
+    from test_checkpoint import write_safetensors
+
+    host = lambda w: {"weight": stored(w)[0].cpu().view(torch.uint32), "scales": stored(w)[1].cpu()}
+    parts = {"gate_proj": mx_util.random_weight(64, 128, 1, DEV, lead=(4,)), "up_proj": mx_util.random_weight(64, 128, 2, DEV, lead=(4,)),
+             "down_proj": mx_util.random_weight(128, 64, 3, DEV, lead=(4,))}
+    dense = mx_util.random_weight(200, 128, 4, DEV)
+    path = tmp_path / "model.safetensors"
+    tensors = {f"moe.{name}.{key}": t for name, w in parts.items() for key, t in host(w).items()}
+    write_safetensors(path, {**tensors, **{f"o.{key}": t for key, t in host(dense).items()}}, pad=3)
+    ckpt = checkpoint.Checkpoint([path])
+    q = checkpoint.load_microscaled(ckpt, "o", DEV)
+    assert (q.n, q.k) == (200, 128) and torch.equal(q.weight, mx.pack(*stored(dense)).weight)
+    ex, first = checkpoint.load_microscaled_experts(ckpt, "moe", DEV, rank=1, world=2, limit=3.0)
+    cut = {name: tuple(t[2:] for t in stored(w)) for name, w in parts.items()}
+    want = mx_experts.make([cut["gate_proj"], cut["up_proj"]], cut["down_proj"], limit=3.0)
+    assert first == 2 and ex.limit == 3.0 and torch.equal(ex.up, want.up) and torch.equal(ex.down, want.down)
+    ckpt.close()

@@ -71,6 +71,7 @@ struct MxParams {
   int64_t ldx;
   int slots;                    // FUSED with a plan: rows of x are pair / slots (0: the pair itself)
   int tile, row_tiles;          // rows of a tile; tiles of rows (dense form)
+  int step_cb, step_y;          // dense form: a cluster's next tile, as column blocks and row tiles further
   void* out;
   int64_t ldo;
   int out_f32, epi;
@@ -288,8 +289,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     atomicCAS(p.err, 0, code);
   };
 
-  // Tiles: (row tile or item) x 128 columns, columns fastest.  A cluster takes every clusters-th tile; FUSED with a plan a run of
-  // neighbours, so that its rows are quantised once an item.
+  // Tiles: (row tile or item) x 128 columns.  Row tiles fastest, so that a column block's weights are read while they are in L2; with a
+  // plan columns fastest.  A cluster takes every clusters-th tile; FUSED with a plan a run of neighbours, so that its rows are
+  // quantised once an item.
   if (GROUPED && !p.settled) pdl_wait();                           // the plan may be the previous kernel's output
   constexpr bool RUNS = FUSED && GROUPED;
   const int nsb = (p.N + MX_SB - 1) / MX_SB, ncb = PAIR ? (nsb + 1) / 2 : nsb;
@@ -330,15 +332,25 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
   auto first = [&]() {
     Tile ti = {};
     ti.t = first_tile;
-    ti.y = FUSED && !GROUPED ? 0 : first_tile / ncb, ti.cb = first_tile - ti.y * ncb;
+    if (GROUPED) ti.y = first_tile / ncb, ti.cb = first_tile - ti.y * ncb;
+    else if (FUSED) ti.cb = first_tile;
+    else if (p.row_tiles == 1) ti.cb = first_tile;
+    else ti.cb = first_tile / p.row_tiles, ti.y = first_tile - ti.cb * p.row_tiles;
     look_up(ti);
     settle(ti);
     return ti;
   };
   auto after = [&](Tile ti) {
-    ti.t += tile_step, ti.cb += tile_step;
-    if (!FUSED || GROUPED)
+    ti.t += tile_step;
+    if (GROUPED) {
+      ti.cb += tile_step;
       while (ti.cb >= ncb) ti.cb -= ncb, ++ti.y;
+    } else if (FUSED) {
+      ti.cb += tile_step;
+    } else {
+      ti.y += p.step_y, ti.cb += p.step_cb;
+      if (ti.y >= p.row_tiles) ti.y -= p.row_tiles, ++ti.cb;
+    }
     look_up(ti);
     return ti;
   };
@@ -929,8 +941,10 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStre
   for (int i = 0; i <= p.sk; ++i) p.bounds[i] = static_cast<int>(static_cast<int64_t>(p.stages) * i / p.sk);
   const int width = PAIR ? 2 : p.cluster;                            // blocks of a cluster
   const int64_t most = PAIR ? std::max(1, g_mx_pairs[current_device()]) : std::max(1, sms / p.cluster);
+  const int64_t clusters = p.cluster > 1 ? tiles : std::min(tiles, most);
+  if (p.row_tiles > 0) p.step_cb = static_cast<int>(clusters / p.row_tiles), p.step_y = static_cast<int>(clusters % p.row_tiles);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.cluster > 1 ? tiles : std::min(tiles, most)) * width));
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * width));
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = 1024 + MX_BAR_BYTES + p.ring * S::SLOT + p.bufs * operand + extra;
   cfg.stream = stream;

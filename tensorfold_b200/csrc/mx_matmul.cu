@@ -555,6 +555,10 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
       const uint64_t a0 = desc(ring0, 1024, SWIZZLE_128), as0 = desc(ring0 + MX_SB * 128, 128, SWIZZLE_NONE);
       const uint64_t b0 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 1024, SWIZZLE_128);
       const uint64_t bs0 = desc((FUSED ? operand0 : ring0 + MX_UNIT) + S::B_ROWS * 128, 128, SWIZZLE_NONE);
+      // of the last stage, whose scales lie behind fewer codes
+      const uint64_t a1 = desc(ring0, 256, SWIZZLE_32), as1 = desc(ring0 + tail * 4096, 128, SWIZZLE_NONE);
+      const uint64_t b1 = desc(FUSED ? operand0 : ring0 + MX_UNIT, 256, SWIZZLE_32);
+      const uint32_t sb_step = (FUSED ? MX_SCALES : mx_tail_scales(tail)) >> 4;
       bool ok = true;
       Ring r = {0, 0u};
       int use = 0, op = GROUPED ? -1 : 0, last_y = -1;
@@ -599,21 +603,24 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
           if (!ok) break;
           if (end > full_stages) {                                   // the last stage: `tail` steps, each a region of its own
             if (!ready && !(ok = lane_wait(full32 + 8 * r.slot, r.phase, abort_word))) break;
-            const uint32_t a = ring0 + r.slot * S::SLOT, b = FUSED ? operand0 + fused_at * 16 : a + MX_UNIT;
-            const uint32_t sb_bytes = FUSED ? MX_SCALES : mx_tail_scales(tail), sa = sf0 + r.slot * S::SF_COLS, sb = sa + 8;
-#pragma unroll 1
-            for (int h = 0; 2 * h < tail; ++h) {
-              copy_scales<PAIR>(sa + 4 * h, desc(a + tail * 4096 + 512 * h, 128, SWIZZLE_NONE));
-              for (int q = 0; q < S::SBS; ++q)
-                copy_scales<PAIR>(sb + 4 * S::SBS * h + 4 * q, desc(b + S::B_ROWS * 128 + q * sb_bytes + 512 * h, 128, SWIZZLE_NONE));
-            }
-#pragma unroll 1
-            for (int j = 0; j < tail; ++j)
-              mma_mxf4<PAIR>(d, desc(a + j * 4096, 256, SWIZZLE_32), desc(b + j * S::B_ROWS * 32, 256, SWIZZLE_32), j & 1 ? id1 : id0, sa + 4 * (j >> 1),
-                       sb + 4 * S::SBS * (j >> 1), more | (j > 0));
-            commit<PAIR>(empty32 + 8 * r.slot);
+            const uint32_t at = r.slot * (S::SLOT >> 4), bt = FUSED ? fused_at : at, sa = sf0 + r.slot * S::SF_COLS, sb = sa + 8;
+            const uint32_t done = empty32 + 8 * r.slot;
             r.next(p.ring);
-            ready = 0;
+            ready = lane_test(full32 + 8 * r.slot, r.phase);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (2 * h >= tail) break;
+              copy_scales<PAIR>(sa + 4 * h, as1 + at + 32 * h);
+#pragma unroll
+              for (int q = 0; q < S::SBS; ++q) copy_scales<PAIR>(sb + 4 * S::SBS * h + 4 * q, bs0 + bt + sb_step * q + 32 * h);
+            }
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+              if (j >= tail) break;
+              mma_mxf4<PAIR>(d, a1 + at + j * (4096 >> 4), b1 + bt + j * (S::B_ROWS * 32 >> 4), j & 1 ? id1 : id0, sa + 4 * (j >> 1),
+                             sb + 4 * S::SBS * (j >> 1), j == 0 ? more : 1u);
+            }
+            commit<PAIR>(done);
           }
           commit<PAIR>(acc_full32 + 8 * (use & 1));
         }

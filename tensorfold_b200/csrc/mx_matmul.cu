@@ -6,18 +6,28 @@
 // weight's shape only; a slice is one chain of MMAs of 64 inputs, slices are added in order, so a row's bits depend neither on the
 // number of rows nor on which of the forms below runs it.
 //
-// "Swap-AB": the weights are the MMA's A operand (M = 128 output columns a block), the rows its B operand (N = 8 to 256).  Both lie
-// in memory as the MMA reads them (mx_layout.h), so a stage of 256 inputs is one bulk copy of 17 KB of weights beside the rows' copies; nothing
-// passes through registers.  Scales go from the stage to tensor memory (tcgen05.cp, the same thread that issues the MMAs), to
-// columns that belong to the stage's slot: they are free when the slot is.
+// "Swap-AB": the weights are the MMA's A operand (M = 128 output columns a block), the rows its B operand (N = 8 to 192).  Both lie
+// in memory as the MMA reads them (mx_layout.h), so a stage of 256 inputs is one bulk copy of 17 KB of weights beside the rows'
+// copies; nothing passes through registers.  Scales go from the stage to tensor memory (tcgen05.cp, by the thread that issues the
+// MMAs), to columns that belong to the stage's slot: they are free when the slot is.
 //
-// Forms (template): FUSED (up to 16 rows): bf16 rows are quantised by the block itself into shared memory while its weights
-// arrive, one launch in all; the block is bound by its weights' bytes.  Otherwise rows come quantised, as operands, in the ring.
-// `cluster` blocks (one a K slice) share a tile where there are few tiles: each sends its part to the block that owns the rows,
-// through distributed shared memory.  With a plan a tile is an item (expert, first, count) x 128 columns.
+// Forms (template):
+//   FUSED    up to 16 rows: the block quantises bf16 rows itself into shared memory while its weights arrive, one launch in all
+//   GROUPED  a tile is a plan's item (expert, first, count) x 128 columns; activations may leave quantised, as the next
+//            projection's operands
+//   PAIR     prompts: two blocks on an SM pair share 256 columns x up to 192 rows (cta_group::2), half of the rows in each one's
+//            shared memory.  The second block's copies land on its own barriers and a thread of it tells the first block, which issues
+//            the MMAs
+//   else     rows come quantised, as operands, in the ring.  `cluster` blocks (one a K slice) share a tile where there are few: each
+//            sends its part to the blocks that own the rows, with counted stores through distributed shared memory
 //
-// Roles: warp 0 loads weights, warp 1 owns tensor memory and issues the MMAs, warp 2 loads rows, warps 4-11 drain (FUSED: 4-7
-// drain, 8-11 quantise, and where every tile has the same rows 4-7 help before they drain).
+// Roles: warp 0 makes the barriers and loads weights, warp 1 owns tensor memory and issues the MMAs, warp 2 loads rows, warp 3
+// forwards (PAIR); from warp 4 on groups of four drain (FUSED: 4-7 drain, the others but 0 and 1 quantise).
+//
+// What bounds it: windows by the weights' bytes and a fixed start and end (17408 x 5120 at one row 9.8 us among others, 4.8 TB/s;
+// 248320 x 5120 99 us, 6.8 TB/s, where the measured copy runs at 6.55); prompts by shared memory, which takes a stage's copies and
+// gives them to the MMAs again at 128 bytes a cycle, and by the stores of the results beside that (2048 rows by 17408 x 5120
+// 85 us in bursts, 4.3 PFLOP/s; 74 without the stores; one block a tile 96).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -58,7 +58,7 @@ constexpr int MX_FUSED_ROWS = 16;
 constexpr int MX_QUANT_COLS = 128;                 // columns of the buffer in which a drain group collects rows to quantise
 constexpr int MX_QUANT_ROWS = 16;
 constexpr int MX_QUANT_BYTES = 2 * MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;    // two buffers in turn
-constexpr int MX_CLUSTER_MAX = 8;
+constexpr int MX_CLUSTER_MAX = 4;
 constexpr int MX_TILE_MAX = 192;                   // rows of a tile: two accumulators and five slots' scales fill tensor memory
 
 enum MxEpilogue : int { MX_STORE = 0, MX_RELU2 = 1, MX_SWIGLU = 2 };
@@ -939,10 +939,18 @@ int current_device() {
 }
 int device_sms() { return g_mx_sms[current_device()]; }
 
-// K slices of an (n, k) weight: enough (128-column block, slice) units for one block an SM, no slice below two stages.
+// K slices of an (n, k) weight: the most, up to four, whose blocks run at once as clusters, no slice below two stages.  A B200 holds
+// 148, 74, 45 or 33 clusters of one to four blocks of this size (fewer than 148 / c: they lie inside a processor cluster), and a
+// second round costs more than slices gain: 6144 x 5120 (48 column blocks) at one row takes 6.9, 6.1, 10.0 and 9.5 us in one to four
+// slices, 5120 x 17408 (40) 17.6, 12.3, 11.1 and 15.6, 4096 x 4096 (32) 5.9, 5.0, 4.9 and 5.1, at sixteen rows 7.5, 7.6, 6.8 and
+// 6.5.  Eight slices are fewer us for a narrow weight in small windows (512 x 16384 at one row 5.4 against 6.4) but not past them (at 32
+// rows 13.1 against 8.5).
+constexpr int MX_CLUSTERS[MX_CLUSTER_MAX + 1] = {0, 148, 74, 45, 33};
 int slices_for(int n, int k) {
   const int blocks = (n + MX_SB - 1) / MX_SB, stages = mx_stages(mx_steps(k));
-  return std::max(1, std::min({MX_CLUSTER_MAX, 148 / std::min(blocks, 148), stages / 2}));
+  int c = MX_CLUSTER_MAX;
+  while (c > 1 && (blocks > MX_CLUSTERS[c] || stages < 2 * c)) --c;
+  return c;
 }
 
 template <int NT, bool FUSED, bool GROUPED, bool PAIR = false>
@@ -1021,29 +1029,32 @@ int round8(int m) { return (m + 7) / 8 * 8; }
 
 // Rows of a tile of an m-row call, blocks that share a tile (all K slices or one), and whether two blocks work as a pair: the fewest
 // cycles by a plain model.  What paces a stage is shared memory, 128 bytes a cycle: 17 KB of weights and 136 bytes a row come in, and
-// four MMAs read 16 KB and 128 bytes a row again; a pair halves the rows' part.  The math takes 2 cycles a row.  A tile has a start
-// and an end besides.
+// four MMAs read 16 KB and 128 bytes a row again; a pair halves the rows' part, but its stages pass from block to block.  A tile has a
+// start and an end besides, and slices that blocks exchange cost by the row.  Tiles in several slices stay below 128 rows: the
+// sums of taller ones do not fit the drain's registers.
+// Measured, us from graphs, as chosen / the other way: pairs 17408 x 5120 at 2048 rows 84 with / 94 without, at 391 28.3 without / 29.1,
+// at 200 18.4 without / 21.7, 10240 x 2560 at 1000 23.1 with / 26.7; exchange 5120 x 17408 at 48 rows 14.3 with / 18.8 without, 6144 x 5120
+// 8.9 with / 9.8, at 128 11.0 without / 13.5, 4096 x 4096 at 32 7.5 with / 8.1, at 128 9.1 without / 11.5.
 struct Tiling {
   int tile, cluster;
   bool pair;
 };
 Tiling tiling_for(int m, int n, int stages, int sk) {
-  constexpr int SMS = 148;
-  constexpr double ENDS = 2500, STAGE = 270, ROW = 2.06;
+  constexpr double ENDS = 3200, STAGE = 270, ROW = 2.06, PAIR_ENDS = 2500, PAIR_STAGE = 440, PAIR_ROW = 1.05, SWAP = 300, SWAP_ROW = 60;
   const int64_t ncb = (n + MX_SB - 1) / MX_SB;
   Tiling best = {8, 1, false};
   double cost = 1e30;
-  auto offer = [&](int64_t blocks, int waves_of, double work, Tiling t) {
-    const double here = static_cast<double>((blocks + waves_of - 1) / waves_of) * (work + ENDS);
+  auto offer = [&](int64_t tiles, int at_once, double work, Tiling t) {
+    const double here = static_cast<double>((tiles + at_once - 1) / at_once) * work;
     if (here <= cost) cost = here, best = t;
   };
-  for (int t = 8; t <= MX_TILE_MAX; t += 8) {
+  for (int t = 8; t <= (sk > 1 ? MX_SB : MX_TILE_MAX); t += 8) {
     const int64_t row_tiles = (m + t - 1) / t;
-    const double stage = std::max(2.0 * t, STAGE + ROW * t), paired = std::max(2.0 * t, STAGE + 16 + ROW / 2 * t);
-    offer(ncb * row_tiles, SMS, stages * stage, {t, 1, false});
-    // (taller tiles leave no room for the exchange beside the ring)
-    if (sk > 1 && t <= MX_SB) offer(ncb * row_tiles * sk, SMS, stages * stage / sk + ENDS, {t, sk, false});
-    if (t % 16 == 0 && m > MX_SB) offer((ncb + 1) / 2 * row_tiles, SMS / 2, stages * paired, {t, 1, true});
+    const double stage = std::max(2.0 * t, STAGE + ROW * t);
+    offer(ncb * row_tiles, MX_CLUSTERS[1], stages * stage + ENDS, {t, 1, false});
+    if (sk > 1) offer(ncb * row_tiles, MX_CLUSTERS[sk], stages * stage / sk + ENDS + SWAP + SWAP_ROW * t, {t, sk, false});
+    if (sk == 1 && t % 16 == 0 && m > MX_SB && stages >= 8)
+      offer((ncb + 1) / 2 * row_tiles, MX_CLUSTERS[2], stages * (PAIR_STAGE + PAIR_ROW * t) + PAIR_ENDS, {t, 1, true});
     if (t >= m) break;
   }
   return best;
@@ -1057,7 +1068,9 @@ bool fused_fits(int k, int sk) {
 
 // Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its six idle warps
 // have few segments of 1024 inputs each.
-constexpr int FUSED_SEGMENTS = 18;
+// Measured, us from graphs, in the block / from their own kernel: 17408 x 5120 (five segments a row) at 2 rows 10.3 / 11.9, at 4 11.5 / 11.9,
+// at 6 12.7 / 11.8; 5120 x 17408 (six) at 1 row 11.1 / 12.7, at 4 13.1 / 12.6; 4096 x 4096 (one) at 16 rows 6.5 / 6.7.
+constexpr int FUSED_SEGMENTS = 24;
 bool fused_pays(int m, int k, int sk) {
   if (m > MX_FUSED_ROWS || !fused_fits(k, sk)) return false;
   const int longest = (mx_stages(mx_steps(k)) + sk - 1) / sk;

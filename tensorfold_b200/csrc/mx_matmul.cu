@@ -58,7 +58,7 @@ constexpr int MX_FUSED_ROWS = 16;
 constexpr int MX_QUANT_COLS = 128;                 // columns of the buffer in which a drain group collects rows to quantise
 constexpr int MX_QUANT_ROWS = 16;
 constexpr int MX_QUANT_BYTES = 2 * MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;    // two buffers in turn
-constexpr int MX_CLUSTER_MAX = 4;
+constexpr int MX_CLUSTER_MAX = 6;
 constexpr int MX_TILE_MAX = 192;                   // rows of a tile: two accumulators and five slots' scales fill tensor memory
 
 enum MxEpilogue : int { MX_STORE = 0, MX_RELU2 = 1, MX_SWIGLU = 2 };
@@ -939,17 +939,16 @@ int current_device() {
 }
 int device_sms() { return g_mx_sms[current_device()]; }
 
-// K slices of an (n, k) weight: the most, up to four, whose blocks run at once as clusters, no slice below two stages.  A B200 holds
-// 148, 74, 45 or 33 clusters of one to four blocks of this size (fewer than 148 / c: they lie inside a processor cluster), and a
-// second round costs more than slices gain: 6144 x 5120 (48 column blocks) at one row takes 6.9, 6.1, 10.0 and 9.5 us in one to four
-// slices, 5120 x 17408 (40) 17.6, 12.3, 11.1 and 15.6, 4096 x 4096 (32) 5.9, 5.0, 4.9 and 5.1, at sixteen rows 7.5, 7.6, 6.8 and
-// 6.5.  Eight slices are fewer us for a narrow weight in small windows (512 x 16384 at one row 5.4 against 6.4) but not past them (at 32
-// rows 13.1 against 8.5).
-constexpr int MX_CLUSTERS[MX_CLUSTER_MAX + 1] = {0, 148, 74, 45, 33};
+// K slices of an (n, k) weight: the most of 1, 2, 3, 4 and 6 whose blocks run at once as clusters, no slice below two stages (three in
+// six slices).  A B200 holds 148, 74, 45, 33 or 22 clusters of that many blocks of this size (fewer than 148 / c: they lie inside a
+// processor cluster), and a second round costs more than slices gain: 6144 x 5120 (48 column blocks) at one row takes 6.9, 6.1, 10.0 and
+// 9.5 us in one to four slices, 5120 x 17408 (40) 17.6, 12.3, 11.1 and 15.6, 4096 x 4096 (32) 5.9, 5.0, 4.9 and 5.1.  Six slices serve
+// windows and cost more rows a little: 1024 x 5120 in four / six, at 13 rows 6.8 / 6.0, at 32 6.9 / 7.0, at 300 9.9 / 10.3.
+constexpr int MX_CLUSTERS[MX_CLUSTER_MAX + 1] = {0, 148, 74, 45, 33, 0, 22};
 int slices_for(int n, int k) {
   const int blocks = (n + MX_SB - 1) / MX_SB, stages = mx_stages(mx_steps(k));
   int c = MX_CLUSTER_MAX;
-  while (c > 1 && (blocks > MX_CLUSTERS[c] || stages < 2 * c)) --c;
+  while (c > 1 && (blocks > MX_CLUSTERS[c] || stages < (c > 4 ? 3 : 2) * c)) --c;
   return c;
 }
 

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restri
                                                    const int* __restrict__ members, int slots, int pairs, uint8_t* __restrict__ out) {
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), y = blockIdx.y;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), y = blockIdx.y;
   int64_t src = static_cast<int64_t>(y) * tile + row;
   if (row >= tile) return;
   if (items != nullptr) {
@@ -265,11 +265,12 @@ cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, i
   const int steps = mx_steps(k), segments = (steps * MX_STEP + ROWS_SEGMENT - 1) / ROWS_SEGMENT;
   const int operands = items ? max_items : (m + tile - 1) / tile, used = items ? tile : std::min(m, tile);
   if (operands > 65535) return cudaErrorInvalidConfiguration;
-  // few rows: a warp a run, for latency; many: a warp a row
-  const int z = static_cast<int64_t>(operands) * used * segments <= 148 * 64 ? segments : 1;
+  // few rows: a warp a run, for latency, in blocks whose registers leave the product's block room beside them; many: a warp a row
+  const bool few = static_cast<int64_t>(operands) * used * segments <= 148 * 64;
+  const int warps = few ? 4 : 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((used + 7) / 8, operands, z);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((used + warps - 1) / warps, operands, few ? segments : 1);
+  cfg.blockDim = dim3(32 * warps);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -34,7 +34,7 @@ def test_sizes():
     assert lib.tf_mx_tiled_bytes(0, 32) < 0 and lib.tf_mx_tiled_bytes(8, 48) < 0 and lib.tf_mx_tiled_bytes(8, 0) < 0
     for n, k in ((1, 32), (1024, 5120), (5120, 17408), (17408, 5120), (248320, 5120), (128, 100000)):
         sk = lib.tf_mx_split(n, k)
-        assert 1 <= sk <= 4 and sk <= max(1, k // 512)
+        assert 1 <= sk <= 6 and sk <= max(1, k // 512)
         assert lib.tf_mx_matmul_bytes(17, n, k) > 0 and lib.tf_mx_matmul_bytes(1, n, k) >= 0
     assert lib.tf_mx_matmul_bytes(1, 17408, 5120) == 0                               # windows need no scratch
     assert lib.tf_mx_split(4, 40) < 0 and lib.tf_mx_matmul_bytes(0, 128, 64) < 0 and lib.tf_mx_experts_bytes(64, 7, 1) < 0

@@ -100,6 +100,29 @@ def test_matmul_tracks_float64(n, k):
     assert _lib.device_error(x) == 0
 
 
+# wide weights on prompts: two blocks share a tile, with an odd number of column blocks and K that ends in every part of a stage
+@pytest.mark.parametrize("n,k", [(9500, 2080), (9728, 2048), (9601, 2176), (9856, 2240)])
+def test_prompts_on_wide_weights(n, k):
+    codes, scales, q = weight(n, k, n + k)
+    x = mx_util.rows(391, k, 5, DEV)
+    x[300, 7] = float("nan")
+    y = mx.matmul(x, q, f32=True)
+    good = torch.arange(391, device=DEV) != 300
+    ref, terms = mx_util.sums(x[good], codes, scales)
+    mx_util.assert_product(y[good], ref, terms, k)
+    assert bool(torch.isnan(y[300]).all())
+    want = y.to(torch.bfloat16).nan_to_num(0.5)
+    out = torch.full((393, n + 8), 7.0, dtype=torch.bfloat16, device=DEV)
+    mx.matmul(x, q, out=out[1:392, 8:])
+    assert torch.equal(out[1:392, 8:].nan_to_num(0.5), want) and (out[0] == 7).all() and (out[392] == 7).all() and (out[:, :8] == 7).all()
+    for m in (1, 16, 40, 129, 300):                            # the other forms, and pairs with other tiles
+        assert torch.equal(mx.matmul(x[:m], q, f32=True), y[:m]), m
+    if n % 32 == 0:
+        act = mx.matmul_act(x[good], q, limit=3.0)             # (any weight of whole tiles is a pair of something)
+        assert torch.equal(mx.matmul_act(x[:9], q, limit=3.0), act[:9]) and bool(torch.isfinite(act).all())
+    assert _lib.device_error(x) == 0
+
+
 @pytest.mark.parametrize("n,k", [(257, 160), (1024, 5120), (2500, 736)])
 def test_whole_numbers_are_exact(n, k):
     """Scales of one and whole values: every partial sum is a whole number of quarters below 2^24, so any order is exact."""
@@ -206,27 +229,27 @@ def test_matmul_act(m, act, limit):
                                      limit=limit), y[:1])
 
 
-@pytest.mark.parametrize("m", [4, 40, 300])
-def test_graphs_and_streams(m):
-    """Two calls captured in one graph and replayed on new rows, and calls on two streams at once."""
+@pytest.mark.parametrize("m,wide", [(4, False), (40, False), (300, False), (391, True)])
+def test_graphs_and_streams(m, wide):
+    """Two calls captured in one graph and replayed on new rows, and calls on three streams at once."""
 
-    _, _, qa = weight(1024, 1184, 5)
-    _, _, qb = weight(512, 1024, 6)
-    x = mx_util.rows(m, 1184, 1, DEV)
+    _, _, qa = weight(9600 if wide else 1024, 2048 if wide else 1184, 5)
+    _, _, qb = weight(512, qa.n, 6)
+    x = mx_util.rows(m, qa.k, 1, DEV)
     want = []
     for seed in (1, 2, 3):
-        h = mx.matmul(mx_util.rows(m, 1184, seed, DEV), qa)
+        h = mx.matmul(mx_util.rows(m, qa.k, seed, DEV), qa)
         want.append((h, mx.matmul(h, qb)))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         h = mx.matmul(x, qa, pdl=True)
         y = mx.matmul(h, qb, pdl=True)
     for i, seed in enumerate((1, 2, 3)):
-        x.copy_(mx_util.rows(m, 1184, seed, DEV))
+        x.copy_(mx_util.rows(m, qa.k, seed, DEV))
         graph.replay()
         assert torch.equal(h, want[i][0]) and torch.equal(y, want[i][1])
     streams = [torch.cuda.Stream() for _ in range(3)]
-    inputs = [mx_util.rows(m, 1184, seed, DEV) for seed in (1, 2, 3)]
+    inputs = [mx_util.rows(m, qa.k, seed, DEV) for seed in (1, 2, 3)]
     torch.cuda.synchronize()
     got = [[] for _ in streams]
     for _ in range(5):

@@ -31,10 +31,11 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------
 
 #define TF_WRAPPED(X) X(tf_qmm) X(tf_qmm_set) X(tf_qmm_set_scratch_bytes) X(tf_qmm_window) X(tf_qmm_window_part_bytes) X(tf_qmm_prefill) X(tf_qmm_prefill_act) X(tf_qmm_act) \
-  X(tf_add_rmsnorm) X(tf_swiglu) X(tf_mx_quantize) X(tf_mx_dequantize) X(tf_mx_tiled_bytes) X(tf_mx_matmul) X(tf_mx_matmul_bytes)
+  X(tf_add_rmsnorm) X(tf_swiglu) X(tf_mx_quantize) X(tf_mx_dequantize) X(tf_mx_tiled_bytes) X(tf_mx_matmul) X(tf_mx_matmul_bytes) \
+  X(tf_mx_experts) X(tf_mx_experts_bytes) X(tf_mx_operand_bytes)
 #define TF_THUNKS(X) X(tf_pack) X(tf_pack_pair) X(tf_unpack) X(tf_group_sums) X(tf_affine_rows) X(tf_moe_plan) X(tf_moe_experts) \
   X(tf_moe_experts_prefill) X(tf_moe_gather) X(tf_moe_experts_sorted) X(tf_moe_router) X(tf_moe_router_tiles) X(tf_moe_topk) X(tf_moe_topk_local) X(tf_moe_combine) \
-  X(tf_mx_pack) X(tf_mx_unpack) X(tf_mx_experts)
+  X(tf_mx_pack) X(tf_mx_unpack)
 
 #define TF_POINTER(name) decltype(&::name) p_##name = nullptr;
 TF_WRAPPED(TF_POINTER)
@@ -639,6 +640,88 @@ PyObject* mx_matmul(PyObject* const* a) {
   return THPVariable_Wrap(out);
 }
 
+// One layer's microscaled experts and the plan of a call.
+struct MxExperts {
+  at::Tensor up, down, items, counts, members;
+  int64_t dims, width, slots, experts, tile;
+  bool gated;
+  float limit;
+};
+
+void mx_table(const at::Tensor& t, int64_t n, int64_t k, const char* who) {
+  const int64_t bytes = k > 0 && k <= INT32_MAX ? p_tf_mx_tiled_bytes(MX_COLS, static_cast<int>(k)) : -1;
+  if (t.scalar_type() != at::kByte || t.dim() != 3 || n < 1 || n > INT32_MAX || bytes < 0 || t.size(1) != (n + MX_COLS - 1) / MX_COLS ||
+      t.size(2) != bytes || t.stride(2) != 1 || t.stride(1) != bytes || (t.size(0) > 1 && t.stride(0) < t.size(1) * bytes))
+    refuse("%s: the table does not have the super-blocks of its shape", who);
+}
+
+// One projection over the plan: rows `x` (bf16) or, with x null, operands `work`; results to `out` or quantised to `operands`.
+void mx_project(const MxExperts& e, const char* who, const at::Tensor& table, int64_t n, int64_t k, const at::Tensor* x, int64_t slots,
+                const at::Tensor* out, void* operands, int epi, at::Tensor work, int64_t rows, int64_t items, bool pdl, cudaStream_t stream) {
+  if (x != nullptr) {
+    const int64_t need = p_tf_mx_experts_bytes(static_cast<int>(k), static_cast<int>(e.tile), static_cast<int>(items));
+    if (need > 0) work = empty({need}, at::kByte, table);
+  }
+  check(unlocked([&] {
+          return p_tf_mx_experts(x ? x->data_ptr() : nullptr, x ? x->stride(0) : 0, static_cast<int>(slots), table.data_ptr(), table.stride(0),
+                                 static_cast<int>(table.size(0)), static_cast<int>(n), static_cast<int>(k), e.items.data_ptr<int>(),
+                                 e.counts.data_ptr<int>(), e.members.data_ptr<int>(), static_cast<int>(rows * e.slots), static_cast<int>(items),
+                                 static_cast<int>(e.tile), out ? out->data_ptr() : nullptr, out ? out->stride(0) : 0,
+                                 out && out->scalar_type() == at::kFloat, operands, epi, epi == 2 ? e.limit : 0.f,
+                                 work.defined() ? work.data_ptr() : nullptr, work.defined() ? work.numel() : 0, pdl, stream);
+        }),
+        who);
+}
+
+// mx_experts(what, x, up, down, dims, width, gated, limit, items, counts, members, slots, experts, tile, out, rows)
+//   what 0: both projections, x [R, D] -> out [pairs, D]; 1: gate and up, x [R, D] -> out [pairs, NI] bf16; 2: down, x [pairs, NI] -> out
+PyObject* mx_experts(PyObject* const* a) {
+  const int what = static_cast<int>(integer(a[0]));
+  const char* who = what == 0 ? "experts" : what == 1 ? "gate_up" : "down";
+  const at::Tensor& given = tensor(a[1], who);
+  MxExperts e;
+  e.up = tensor(a[2], who), e.down = tensor(a[3], who);
+  e.dims = integer(a[4]), e.width = integer(a[5]), e.gated = truth(a[6]), e.limit = static_cast<float>(number(a[7]));
+  e.items = tensor(a[8], who), e.counts = tensor(a[9], who), e.members = tensor(a[10], who);
+  e.slots = integer(a[11]), e.experts = integer(a[12]), e.tile = integer(a[13]);
+  const at::Tensor& out = tensor(a[14], who);
+  const int64_t rows = integer(a[15]), up_n = (e.gated ? 2 : 1) * e.width;
+  mx_table(e.up, up_n, e.dims, who);
+  mx_table(e.down, e.dims, e.width, who);
+  if (e.experts > e.up.size(0) || e.experts > e.down.size(0))
+    refuse("%s: the plan routes to %lld experts but the table holds %lld", who, static_cast<long long>(e.experts),
+           static_cast<long long>(std::min(e.up.size(0), e.down.size(0))));
+  const cudaStream_t stream = stream_of(e.up);
+  for (const at::Tensor* t : {&e.items, &e.counts, &e.members})
+    if (t->device() != e.up.device() || t->scalar_type() != at::kInt || !t->is_contiguous()) refuse("%s: the plan and the weights must share a CUDA device", who);
+  if (e.slots < 1 || rows < 1 || rows > e.members.numel() / e.slots) refuse("%s: %lld rows do not fit the plan", who, static_cast<long long>(rows));
+  if (e.down.device() != e.up.device() || given.device() != e.up.device() || out.device() != e.up.device())
+    refuse("%s: x, out and the weights must share a CUDA device", who);
+  const int64_t pairs = rows * e.slots, k = what == 2 ? e.width : e.dims, need = what == 2 ? pairs : rows, cols = what == 1 ? e.width : e.dims;
+  if (given.scalar_type() != at::kBFloat16 || given.dim() != 2 || given.size(1) != k || given.size(0) < need)
+    refuse("%s: x must be (%lld, %lld) bf16", who, static_cast<long long>(need), static_cast<long long>(k));
+  const bool type_ok = out.scalar_type() == at::kBFloat16 || (what != 1 && out.scalar_type() == at::kFloat);
+  if (!type_ok || out.dim() != 2 || out.size(1) != cols || out.size(0) < pairs || out.stride(1) != 1 || (out.size(0) > 1 && out.stride(0) < cols))
+    refuse("%s: out must be (%lld, %lld) with unit-stride rows, of the requested type", who, static_cast<long long>(pairs), static_cast<long long>(cols));
+  // (the rows are strided by the C entry, so a single row needs a legal stride too)
+  const bool fetchable = given.stride(1) == 1 && given.stride(0) % 8 == 0 && given.stride(0) >= k && aligned(given.data_ptr(), 16);
+  const at::Tensor x = fetchable ? given : given.clone(at::MemoryFormat::Contiguous);
+  const int64_t items = std::min(std::min(pairs, e.experts) + pairs / e.tile, e.items.size(0));
+  const int epi = e.gated ? 2 : 1;
+  if (what == 1) {
+    mx_project(e, who, e.up, up_n, e.dims, &x, e.slots, &out, nullptr, epi, at::Tensor(), rows, items, false, stream);
+  } else if (what == 2) {
+    mx_project(e, who, e.down, e.dims, e.width, &x, 0, &out, nullptr, 0, at::Tensor(), rows, items, false, stream);
+  } else {
+    const at::Tensor act =
+        empty({items * p_tf_mx_operand_bytes(static_cast<int>(e.tile), static_cast<int>(e.width))}, at::kByte, e.up);
+    mx_project(e, "experts (gate, up)", e.up, up_n, e.dims, &x, e.slots, nullptr, act.data_ptr(), epi, at::Tensor(), rows, items, false, stream);
+    // the first projection waited for the plan, so the second may read it, and its weights, while the first runs
+    mx_project(e, "experts (down)", e.down, e.dims, e.width, nullptr, 0, &out, nullptr, 0, act, rows, items, true, stream);
+  }
+  Py_RETURN_NONE;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // thunks: name(what, ...) calls the C-ABI entry `name` with tensors (or addresses, or None) for its pointers
 // ---------------------------------------------------------------------------------------------------------------------
@@ -707,6 +790,7 @@ TF_WHOLE(swiglu, 3)
 TF_WHOLE(mx_quantize, 1)
 TF_WHOLE(mx_dequantize, 3)
 TF_WHOLE(mx_matmul, 7)
+TF_WHOLE(mx_experts, 16)
 
 #define TF_THUNK(name)                                                                          \
   PyObject* py_##name(PyObject*, PyObject* const* args, Py_ssize_t nargs) {                     \
@@ -757,7 +841,7 @@ PyMethodDef g_methods[] = {
     {"stream_of", py_stream_of, METH_O, nullptr},
     {"forget_scratch", py_forget_scratch, METH_NOARGS, nullptr},
     TF_FAST(matmul) TF_FAST(matmul_set) TF_FAST(prefill_matmul) TF_FAST(matmul_act) TF_FAST(add_rmsnorm) TF_FAST(swiglu)
-    TF_FAST(mx_quantize) TF_FAST(mx_dequantize) TF_FAST(mx_matmul)
+    TF_FAST(mx_quantize) TF_FAST(mx_dequantize) TF_FAST(mx_matmul) TF_FAST(mx_experts)
     TF_THUNKS(TF_FAST){nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

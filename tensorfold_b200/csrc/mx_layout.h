@@ -30,7 +30,9 @@ constexpr int MX_STAGE = 256;                    // inputs of a stage: one 128-b
 constexpr int MX_SB = 128;                       // rows of a super-block
 constexpr int MX_SCALES = 1024;                  // scale bytes of a full stage per 128 rows
 constexpr int MX_UNIT = MX_SB * 128 + MX_SCALES; // bytes of a full stage of a super-block
+constexpr int MX_LONGEST = 0x7FFFFFFF - 255;     // of rows, columns or inputs: rounding up to tiles and stages stays an int
 
+TF_MX_HD constexpr bool mx_sizes(int n, int k) { return n >= 1 && n <= MX_LONGEST && k >= MX_BLOCK && k <= MX_LONGEST && k % MX_BLOCK == 0; }
 TF_MX_HD constexpr int mx_steps(int k) { return (k + MX_STEP - 1) / MX_STEP; }
 TF_MX_HD constexpr int mx_stages(int steps) { return (steps + 3) / 4; }
 TF_MX_HD constexpr int mx_scale_blocks(int rows) { return (rows + MX_SB - 1) / MX_SB; }

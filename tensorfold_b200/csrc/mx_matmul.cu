@@ -27,7 +27,7 @@
 // What bounds it: windows by the weights' bytes and a fixed start and end (17408 x 5120 at one row 9.8 us among others, 4.8 TB/s;
 // 248320 x 5120 99 us, 6.8 TB/s, where the measured copy runs at 6.55); prompts by shared memory, which takes a stage's copies and
 // gives them to the MMAs again at 128 bytes a cycle, and by the stores of the results beside that (2048 rows by 17408 x 5120
-// 85 us in bursts, 4.3 PFLOP/s; 74 without the stores; one block a tile 96).
+// 85 us in bursts, 4.3 PFLOP/s; 76 without the stores; one block a tile 94).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -1062,7 +1062,7 @@ Tiling tiling_for(int m, int n, int stages, int sk) {
 // Whether a block can hold its K slice of sixteen quantised rows beside a ring of four slots.
 bool fused_fits(int k, int sk) {
   const int stages = mx_stages(mx_steps(k)), longest = (stages + sk - 1) / sk;
-  return longest * MxShape<16, true, true>::B_BYTES + 4 * MX_UNIT + MX_CLUSTER_MAX * 4 * MX_SB * 4 <= MX_SMEM_MAX;
+  return static_cast<int64_t>(longest) * MxShape<16, true, true>::B_BYTES + 4 * MX_UNIT + MX_CLUSTER_MAX * 4 * MX_SB * 4 <= MX_SMEM_MAX;
 }
 
 // Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its six idle warps
@@ -1102,10 +1102,10 @@ using namespace tf;
 
 extern "C" {
 
-int tf_mx_split(int n, int k) { return n < 1 || k < MX_BLOCK || k % MX_BLOCK ? TF_ERR_ARG : slices_for(n, k); }
+int tf_mx_split(int n, int k) { return !mx_sizes(n, k) ? TF_ERR_ARG : slices_for(n, k); }
 
 int64_t tf_mx_matmul_bytes(int m, int n, int k) {
-  if (m < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  if (m < 1 || m > MX_LONGEST || !mx_sizes(n, k)) return TF_ERR_ARG;
   if (fused_pays(m, k, slices_for(n, k))) return 0;
   const int steps = mx_steps(k), tile = tiling_for(m, n, mx_stages(steps), slices_for(n, k)).tile;
   return (m + tile - 1) / tile * mx_operand_bytes(tile, steps);
@@ -1113,7 +1113,7 @@ int64_t tf_mx_matmul_bytes(int m, int n, int k) {
 
 int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
                  void* work, int64_t work_bytes, int pdl, void* stream) {
-  if (m < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: K must be a positive multiple of 32, n and m positive");
+  if (m < 1 || m > MX_LONGEST || !mx_sizes(n, k)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: K must be a positive multiple of 32, n and m positive");
   if (epi < 0 || epi > 2 || (epi == 2 && n % 32) || (epi != 0 && out_f32)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: bad epilogue");
   if (!x || !tiled || !out || ldo < (epi == 2 ? n / 2 : n) || ldx < k) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: null pointer or short rows");
   if (misaligned(x, 16) || (m > 1 && ldx % 8)) return fail_moe(TF_ERR_ALIGN, "tf_mx_matmul: x rows must start on 16-byte boundaries");
@@ -1160,19 +1160,19 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
 }
 
 int64_t tf_mx_operand_bytes(int rows, int k) {
-  if (rows < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  if (!mx_sizes(rows, k)) return TF_ERR_ARG;
   return mx_operand_bytes(round8(rows), mx_steps(k));
 }
 
 int64_t tf_mx_experts_bytes(int k, int tile, int max_items) {
-  if (tile < 8 || tile > MX_SB || max_items < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  if (tile < 8 || tile > MX_SB || max_items < 1 || !mx_sizes(tile, k)) return TF_ERR_ARG;
   return tile <= MX_FUSED_ROWS && fused_fits(k, 1) ? 0 : max_items * mx_operand_bytes(round8(tile), mx_steps(k));
 }
 
 int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int64_t expert_stride, int experts, int n, int k, const int* items,
                   const int* counts, const int* members, int pairs, int max_items, int tile, void* out, int64_t ldo, int out_f32,
                   void* out_operands, int epi, float limit, void* work, int64_t work_bytes, int pdl, void* stream) {
-  if (experts < 1 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || pairs < 1 || max_items < 1 || max_items > 65535 || slots < 0)
+  if (experts < 1 || !mx_sizes(n, k) || pairs < 1 || max_items < 1 || max_items > 65535 || slots < 0)
     return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad sizes (K a positive multiple of 32)");
   if (tile < 8 || tile > MX_SB || tile % 8) return fail_moe(TF_ERR_ARG, "tf_mx_experts: items of 8 to 128 pairs, in whole eights");
   if (epi < 0 || epi > 2 || (epi == 2 && n % 32)) return fail_moe(TF_ERR_ARG, "tf_mx_experts: bad epilogue");

@@ -288,12 +288,12 @@ using namespace tf;
 extern "C" {
 
 int64_t tf_mx_tiled_bytes(int n, int k) {
-  if (n < 1 || k < MX_BLOCK || k % MX_BLOCK) return TF_ERR_ARG;
+  if (!mx_sizes(n, k)) return TF_ERR_ARG;
   return static_cast<int64_t>((n + MX_SB - 1) / MX_SB) * mx_operand_bytes(MX_SB, mx_steps(k));
 }
 
 int tf_mx_quantize(const void* x, int64_t ldx, int dtype, int rows, int k, void* words, void* scales, void* stream) {
-  if (dtype < 0 || dtype > 2 || rows < 1 || k < MX_BLOCK || k % MX_BLOCK || ldx < k || !x || !words || !scales)
+  if (dtype < 0 || dtype > 2 || !mx_sizes(rows, k) || ldx < k || !x || !words || !scales)
     return fail_moe(TF_ERR_ARG, "tf_mx_quantize: rows of a positive multiple of 32 values, none null");
   if (misaligned(x, 16) || (rows > 1 && ldx % (dtype == 2 ? 4 : 8)) || misaligned(words, 4))
     return fail_moe(TF_ERR_ALIGN, "tf_mx_quantize: rows must start on 16-byte boundaries");
@@ -318,7 +318,7 @@ int tf_mx_quantize(const void* x, int64_t ldx, int dtype, int rows, int k, void*
 }
 
 int tf_mx_dequantize(const void* words, const void* scales, int rows, int k, int out_type, void* out, void* stream) {
-  if (out_type < 0 || out_type > 2 || rows < 1 || k < MX_BLOCK || k % MX_BLOCK || !words || !scales || !out)
+  if (out_type < 0 || out_type > 2 || !mx_sizes(rows, k) || !words || !scales || !out)
     return fail_moe(TF_ERR_ARG, "tf_mx_dequantize: rows of a positive multiple of 32 values, none null");
   if (misaligned(words, 4) || misaligned(out, 16)) return fail_moe(TF_ERR_ALIGN, "tf_mx_dequantize: out must start on a 16-byte boundary");
   const int64_t pieces = static_cast<int64_t>(rows) * (k / 8);
@@ -340,7 +340,7 @@ int tf_mx_dequantize(const void* words, const void* scales, int rows, int k, int
 int tf_mx_pack(const void* words, const void* scales, const void* up_words, const void* up_scales, int experts, int n, int k, void* tiled,
                void* stream) {
   const bool pair = up_words != nullptr;
-  if (experts < 1 || experts > 65535 || n < 1 || k < MX_BLOCK || k % MX_BLOCK || !words || !scales || !tiled || pair != (up_scales != nullptr))
+  if (experts < 1 || experts > 65535 || !mx_sizes(n, k) || !words || !scales || !tiled || pair != (up_scales != nullptr))
     return fail_moe(TF_ERR_ARG, "tf_mx_pack: rows of a positive multiple of 32 values, none null");
   if (pair && n % 32) return fail_moe(TF_ERR_ARG, "tf_mx_pack: a pair interleaves whole tiles of 16 rows");
   if (misaligned(words, 16) || misaligned(up_words, 16) || misaligned(tiled, 16))
@@ -356,7 +356,7 @@ int tf_mx_pack(const void* words, const void* scales, const void* up_words, cons
 }
 
 int tf_mx_unpack(const void* tiled, int n, int k, void* words, void* scales, void* stream) {
-  if (n < 1 || k < MX_BLOCK || k % MX_BLOCK || !words || !scales || !tiled) return fail_moe(TF_ERR_ARG, "tf_mx_unpack: bad shape or null pointer");
+  if (!mx_sizes(n, k) || !words || !scales || !tiled) return fail_moe(TF_ERR_ARG, "tf_mx_unpack: bad shape or null pointer");
   if (misaligned(words, 16) || misaligned(tiled, 16))
     return fail_moe(TF_ERR_ALIGN, "tf_mx_unpack: words and units must start on 16-byte boundaries");
   const int steps = mx_steps(k);

@@ -694,6 +694,7 @@ PyObject* mx_experts(PyObject* const* a) {
   const cudaStream_t stream = stream_of(e.up);
   for (const at::Tensor* t : {&e.items, &e.counts, &e.members})
     if (t->device() != e.up.device() || t->scalar_type() != at::kInt || !t->is_contiguous()) refuse("%s: the plan and the weights must share a CUDA device", who);
+  if (e.tile < 8) refuse("%s: items of 8 pairs and more are wanted", who);
   if (e.slots < 1 || rows < 1 || rows > e.members.numel() / e.slots) refuse("%s: %lld rows do not fit the plan", who, static_cast<long long>(rows));
   if (e.down.device() != e.up.device() || given.device() != e.up.device() || out.device() != e.up.device())
     refuse("%s: x, out and the weights must share a CUDA device", who);

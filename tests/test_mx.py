@@ -98,6 +98,14 @@ def test_c_abi_refuses_before_launching():
     assert experts() != 0
 
 
+def test_sizes_at_the_end_of_an_int_are_refused():
+    lib, end = _lib.lib(), 2 ** 31 - 1
+    assert lib.tf_mx_matmul_bytes(end, 64, 128) < 0 and lib.tf_mx_matmul_bytes(4, end, 128) < 0 and lib.tf_mx_matmul_bytes(4, 64, end - 31) < 0
+    assert lib.tf_mx_tiled_bytes(end, 128) < 0 and lib.tf_mx_tiled_bytes(64, end - 31) < 0 and lib.tf_mx_split(end, 128) < 0
+    assert lib.tf_mx_matmul_bytes(1 << 30, 64, 128) > (1 << 30) * 64
+    assert lib.tf_mx_matmul_bytes(1, 1, 1 << 30) > 0 and lib.tf_mx_experts_bytes(1 << 30, 16, 4) > 0    # rows too long to be held by a block
+
+
 def stored(n, k, seed, lead=()):
     codes, scales = mx_util.random_weight(n, k, seed, "cpu", lead=lead)
     return {"weight": mx_util.to_words(codes).view(torch.uint32), "scales": scales.to(torch.uint8)}

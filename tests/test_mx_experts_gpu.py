@@ -169,6 +169,24 @@ def test_items_outside_the_table_are_reported():
         assert _lib.device_error(x) == 5 and int((y == 3).all(1).sum()) == int(plan.items[1, 2])
 
 
+@pytest.mark.parametrize("prefill", [False, True])
+def test_tables_past_32_bits(prefill):
+    """Experts that lie gigabytes apart give what they give side by side."""
+
+    ex, _, _ = build(CASES[0], 9)
+
+    def apart(t):
+        step = 2 ** 29 + 4096
+        big = torch.empty((t.shape[0] * step,), dtype=torch.uint8, device=DEV).as_strided(t.shape, (step, t.shape[2], 1))
+        return big.copy_(t)
+
+    wide = mx_experts.Experts(apart(ex.up), apart(ex.down), ex.width, ex.dims, ex.limit, ex.gated)
+    assert wide.up[-1].data_ptr() - wide.up[0].data_ptr() > 2 ** 32
+    x, picks = mx_util.rows(40, ex.dims, 2, DEV, std=0.5), picks_for(40, 4, ex.count, 3)
+    for a, b in zip(run(x, ex, picks, prefill), run(x, wide, picks, prefill)):
+        assert torch.equal(a, b)
+
+
 def test_infinite_rows_stay_in_their_pairs():
     for case, prefill in ((CASES[1], False), (CASES[1], True), (CASES[2], False), (CASES[2], True)):
         ex, _, _ = build(case, 6)

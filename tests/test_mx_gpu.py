@@ -6,7 +6,7 @@ import torch
 
 import mx_util
 from tensorfold_b200 import _lib
-from tensorfold_b200.cuda.kernels import mx
+from tensorfold_b200.cuda.kernels import mx, qmm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -258,6 +258,55 @@ def test_graphs_and_streams(m, wide):
                 got[i].append(mx.matmul(mx.matmul(inputs[i], qa), qb))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i][1]) for i in range(3) for y in got[i])
+
+
+def test_offsets_past_32_bits():
+    """Inputs and outputs of more than 2^31 values: the first and last rows are what they are in small calls."""
+
+    x = torch.zeros((65552, 32768), dtype=torch.bfloat16, device=DEV)
+    ends = mx_util.rows(4, 32768, 1, DEV)
+    x[:2], x[-2:] = ends[:2], ends[2:]
+    words, scales = mx.quantize(x)
+    few = mx.quantize(ends)
+    assert torch.equal(words[[0, 1, -2, -1]], few[0]) and torch.equal(scales[[0, 1, -2, -1]], few[1]) and not words[2:-2].any()
+    del x
+    back = mx.dequantize(words, scales)
+    assert torch.equal(back[[0, 1, -2, -1]], mx.dequantize(*few)) and not back[2:-2].any()
+    del back, words, scales
+    _, _, q = weight(11000, 96, 3)
+    rows = mx_util.rows(64, 96, 2, DEV)
+    y = mx.matmul(rows.repeat(3200, 1), q)
+    assert y.numel() > 2 ** 31
+    want = mx.matmul(rows, q)
+    assert all(torch.equal(y[i:i + 64], want) for i in (0, 64 * 1600, 64 * 3050, 64 * 3199))
+
+
+def test_beside_other_products():
+    """Affine and microscaled products in turn on one stream with early launches, and both kinds at once on two streams: they share
+    tensor memory and shared memory of the SMs."""
+
+    _, _, q = weight(4096, 1024, 7)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    w = torch.randint(-2 ** 31, 2 ** 31, (1024, 4096 // 8), generator=g, device=DEV).to(torch.int32)
+    s = (torch.rand((1024, 4096 // 64), generator=g, device=DEV) * .01).bfloat16()
+    affine = qmm.pack(w, s, -8 * s, 64)
+    for m in (1, 16, 300):
+        x = mx_util.rows(m, 1024, m, DEV)
+        h0 = mx.matmul(x, q)
+        y0 = qmm.matmul(h0, affine)
+        for _ in range(4):
+            h = mx.matmul(x, q, pdl=True)
+            assert torch.equal(h, h0) and torch.equal(qmm.matmul(h, affine), y0)
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        got = [], []
+        for _ in range(8):
+            with torch.cuda.stream(a):
+                got[0].append(mx.matmul(x, q, pdl=True))
+            with torch.cuda.stream(b):
+                got[1].append(qmm.matmul(h0, affine))
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, h0) for t in got[0]) and all(torch.equal(t, y0) for t in got[1])
 
 
 def test_refusals_on_the_device():

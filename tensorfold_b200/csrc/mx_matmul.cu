@@ -15,8 +15,8 @@
 //   FUSED    up to 16 rows: the block quantises bf16 rows itself into shared memory while its weights arrive, one launch in all
 //   GROUPED  a tile is a plan's item (expert, first, count) x 128 columns; activations may leave quantised, as the next
 //            projection's operands
-//   PAIR     prompts: two blocks on an SM pair share 256 columns x up to 192 rows (cta_group::2), half of the rows in each one's
-//            shared memory.  The second block's copies land on its own barriers and a thread of it tells the first block, which issues
+//   PAIR     prompts: two blocks on an SM pair share 256 columns x up to 192 rows, or an item's 128 (cta_group::2), half of the rows
+//            in each one's shared memory.  The second block's copies land on its own barriers and a thread of it tells the first block, which issues
 //            the MMAs
 //   else     rows come quantised, as operands, in the ring.  `cluster` blocks (one a K slice) share a tile where there are few: each
 //            sends its part to the blocks that own the rows, with counted stores through distributed shared memory
@@ -57,7 +57,9 @@ constexpr int MX_SMEM_MAX = 232448 - 1024 /* alignment slack */ - MX_BAR_BYTES;
 constexpr int MX_FUSED_ROWS = 16;
 constexpr int MX_QUANT_COLS = 128;                 // columns of the buffer in which a drain group collects rows to quantise
 constexpr int MX_QUANT_ROWS = 16;
-constexpr int MX_QUANT_BYTES = 2 * MX_QUANT_ROWS * (MX_QUANT_COLS + 4) * 4;    // two buffers in turn
+__host__ __device__ constexpr int quant_bytes(bool gated) {                     // two buffers in turn; SwiGLU leaves half of the columns
+  return 2 * MX_QUANT_ROWS * ((gated ? MX_QUANT_COLS / 2 : MX_QUANT_COLS) + 4) * 4;
+}
 constexpr int MX_CLUSTER_MAX = 6;
 constexpr int MX_TILE_MAX = 192;                   // rows of a tile: two accumulators and five slots' scales fill tensor memory
 
@@ -259,7 +261,7 @@ struct Ring {
 template <int NT, bool FUSED, bool GROUPED, bool PAIR>
 __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1) mx_kernel(const MxParams p) {
   using S = MxShape<NT, FUSED, GROUPED, PAIR>;
-  static_assert(!PAIR || (!FUSED && !GROUPED), "pairs are for prompts");
+  static_assert(!PAIR || !FUSED, "pairs are for prompts");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);              // [MX_RING_MAX] the slot's copies have landed
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
       ti.m0 = ti.y * p.tile;
       ti.rows = min(p.tile, p.M - ti.m0);
     }
-    ti.n = PAIR ? (ti.rows + 15) & ~15 : max(8, (ti.rows + 7) & ~7);
+    ti.n = PAIR ? max(16, (ti.rows + 15) & ~15) : max(8, (ti.rows + 7) & ~7);
   };
   auto first = [&]() {
     Tile ti = {};
@@ -743,9 +745,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     // Sixteen rows of activations to the next projection's operand: through shared memory, where four lanes see a block.
     int turn = 0;
     auto quantize16 = [&](const Tile& ti, const float* v, int n) {
-      constexpr int LINE = MX_QUANT_COLS + 4;
+      const int LINE = (gated ? MX_QUANT_COLS / 2 : MX_QUANT_COLS) + 4;
       // (a warp that writes a buffer again has passed the barrier after which the others read its last contents twice)
-      float* rows = reinterpret_cast<float*>(smem + extra_off + group * MX_QUANT_BYTES) + turn * MX_QUANT_ROWS * LINE;
+      float* rows = reinterpret_cast<float*>(smem + extra_off + group * quant_bytes(gated)) + turn * MX_QUANT_ROWS * LINE;
       turn ^= 1;
       const int shift = gated ? 3 : 4;                               // pieces of eight columns a row: 8 or 16
       if (gated) {
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
       }
       named_barrier(1 + group, 128);
       // the tile's blocks lie in one stage of the operand
-      const int block0 = ti.cb << (shift - 2), u = block0 >> 3;
+      const int block0 = block_of(ti) << (shift - 2), u = block0 >> 3;
       uint8_t* op = p.q + ti.y * p.q_item_stride + u * mx_stage_bytes(p.q_rows);
       const bool whole = u < p.q_steps >> 2;
       const int q_tail = p.q_steps & 3;
@@ -793,7 +795,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     if (ti.t >= end_tile) settle_in();
     for (bool rehearsal = true; ti.t < end_tile && ok;) {
       if (!rehearsal) {
-        if (slice1 - slice0 > 1) {
+        if (!GROUPED && slice1 - slice0 > 1) {
           // slices are added in registers, and the sum goes back to where the last one came from
           float acc[S::CHUNKS][16];
           for (int s = slice0; s < slice1; ++s, ++use) {
@@ -955,7 +957,7 @@ int slices_for(int n, int k) {
 template <int NT, bool FUSED, bool GROUPED, bool PAIR = false>
 cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStream_t stream) {
   using S = MxShape<NT, FUSED, GROUPED, PAIR>;
-  int extra = quant_out ? S::GROUPS * MX_QUANT_BYTES : 0;
+  int extra = quant_out ? S::GROUPS * quant_bytes(p.epi == MX_SWIGLU) : 0;
   if (p.cluster > 1) extra = p.cluster * quads_of(std::min(p.tile, p.M), p.cluster) * MX_SB * 16;
   const int operand = FUSED ? p.operand_stages * S::B_BYTES : 0;
   if (FUSED && p.bufs == 2 && MX_SMEM_MAX - extra - 2 * operand < 4 * S::SLOT) p.bufs = 1;
@@ -1019,9 +1021,15 @@ cudaError_t pairs_resident(int* pairs) {
   cfg.numAttrs = 1;
   return cudaOccupancyMaxActiveClusters(pairs, mx_kernel<MX_TILE_MAX, false, false, true>, &cfg);
 }
+// A plan's items.  Pairs take items of prompts where there are many tiles: their rows go to half as many blocks, but a tile begins and
+// ends later.  Measured, us a layer of both projections (experts, D, NI, picks; up to 16 tiles an SM go to single blocks): 128, 2688,
+// 1856, 6 at 2048 rows 210 in pairs / 216, at 64 rows 166 / 170, at 8000 rows 603 / 609; 64, 2048, 768, 8 at 2048 rows 124.0 / 124.3;
+// 16, 4096, 1024, 2 at 512 rows 39.6 / 39.3, at 100 rows 30.0 / 28.8.
+constexpr int PAIR_TILES = 16;
 cudaError_t launch_items(MxParams& p, int64_t tiles, int sms, cudaStream_t stream) {
-  return p.tile <= 16 ? launch<16, false, true>(p, tiles, p.q != nullptr, sms, stream)
-                      : launch<128, false, true>(p, tiles, p.q != nullptr, sms, stream);
+  if (p.tile <= 16) return launch<16, false, true>(p, tiles, p.q != nullptr, sms, stream);
+  if (tiles < static_cast<int64_t>(PAIR_TILES) * sms) return launch<MX_SB, false, true>(p, tiles, p.q != nullptr, sms, stream);
+  return launch<MX_SB, false, true, true>(p, tiles, p.q != nullptr, sms, stream);
 }
 
 int round8(int m) { return (m + 7) / 8 * 8; }
@@ -1089,6 +1097,7 @@ cudaError_t mx_configure(int device, int sms) {
   if (e == cudaSuccess) e = configure<64, false, false>();
   if (e == cudaSuccess) e = configure<128, false, false>();
   if (e == cudaSuccess) e = configure<128, false, true>();
+  if (e == cudaSuccess) e = configure<128, false, true, true>();
   if (e == cudaSuccess) e = configure<192, false, false>();
   int pairs = 0;
   if (e == cudaSuccess) e = pairs_resident(&pairs);

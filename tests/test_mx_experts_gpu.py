@@ -157,6 +157,35 @@ def test_ragged_plans(prefill):
     assert (part == 3).all() and _lib.device_error(x) == 0
 
 
+@pytest.mark.parametrize("case", [(400, 800, 416, True, 1.0), (420, 768, 800, False, 0.0)])
+def test_many_tiles(case):
+    """Tables of so many tiles that blocks take them in pairs: the bits of the form for few rows, over a ragged plan, odd numbers of
+    column blocks, a row of NaN and an item outside the table."""
+
+    ex, _, _ = build(case, 31)
+    rows = 150
+    x = mx_util.rows(rows, ex.dims, 2, DEV, std=0.5)
+    x[9, 3] = float("nan")
+    picks = picks_for(rows, 4, ex.count, 3)
+    picks[:140, 0] = 7                                         # two items of one expert
+    picks[20:30, 1] = -1
+    got = run(x, ex, picks, True)
+    for lo in range(0, rows, 16):
+        few = run(x[lo:lo + 16], ex, picks[lo:lo + 16], False)
+        for a, b in zip(few, got):
+            assert torch.equal(a.view(torch.int16 if a.dtype == torch.bfloat16 else torch.int32),
+                               b[4 * lo:4 * lo + a.shape[0]].view(torch.int16 if a.dtype == torch.bfloat16 else torch.int32))
+    assert bool(torch.isnan(got[2][36:40]).all()) and not torch.isnan(got[2][40:]).any() and _lib.device_error(x) == 0
+    plan = plan_of(picks, ex.count, True)
+    plan.items[1, 0] = ex.count + 3
+    y = torch.full((rows * 4, ex.dims), 3.0, dtype=torch.float32, device=DEV)
+    mx_experts.layer(x, ex, plan, y, rows)
+    assert _lib.device_error(x) == 5
+    left = (y == 3).all(1)
+    unrouted = int((picks < 0).sum())
+    assert int(left.sum()) == int(plan.items[1, 2]) + unrouted and torch.equal(y[~left].nan_to_num(), got[2][~left].nan_to_num())
+
+
 def test_items_outside_the_table_are_reported():
     ex, _, _ = build(CASES[0], 5)
     x = mx_util.rows(8, ex.dims, 2, DEV)

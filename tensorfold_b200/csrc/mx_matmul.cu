@@ -27,7 +27,7 @@
 // What bounds it: windows by the weights' bytes and a fixed start and end (17408 x 5120 at one row 9.8 us among others, 4.8 TB/s;
 // 248320 x 5120 99 us, 6.8 TB/s, where the measured copy runs at 6.55); prompts by shared memory, which takes a stage's copies and
 // gives them to the MMAs again at 128 bytes a cycle, and by the stores of the results beside that (2048 rows by 17408 x 5120
-// 85 us in bursts, 4.3 PFLOP/s; 76 without the stores; one block a tile 94).
+// 83 us in bursts, 4.4 PFLOP/s; 9 less without the stores; one block a tile 94).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

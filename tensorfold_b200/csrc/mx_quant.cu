@@ -190,8 +190,8 @@ __global__ void __launch_bounds__(256) unpack_kernel(const uint8_t* __restrict__
   }
 }
 
-// bf16 rows to the operand layout: operand y (blockIdx.y) holds `tile` rows, a warp a row and as many runs of 1024 inputs as gridDim.z
-// leaves it, four 16-byte loads in flight a lane.  With a plan, row r of item y is row members[first + r] / slots of x
+// bf16 rows to the operand layout: operand y (blockIdx.y) holds `tile` rows, a warp (a row, as many runs of 1024 inputs as gridDim.z
+// leaves it), four 16-byte loads in flight a lane.  With a plan, row r of item y is row members[first + r] / slots of x
 // (members[first + r] itself with slots 0).
 constexpr int ROWS_SEGMENT = 1024;
 __global__ void __launch_bounds__(256) rows_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int m, int k, int steps, int rows, int tile,
@@ -246,7 +246,9 @@ int blocks_for(int64_t threads) {
   return static_cast<int>(b < 1 ? 1 : b > 148 * 64 ? 148 * 64 : b);
 }
 
-constexpr int64_t MANY = 148 * 2048 * 4;      // pieces past which a thread takes four at a time
+// Pieces from which a thread takes four.  Measured, us from graphs, one / four: 256 x 5120 1.8 / 2.1 (back 1.8 / 2.1), 1024 x 5120 3.7 / 3.3
+// (3.3 / 3.3), 2048 x 5120 5.9 / 4.7 (5.1 / 4.7), 17408 x 5120 48 / 34 (47 / 36).
+constexpr int64_t MANY = 148 * 2048 * 4;
 
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
@@ -265,11 +267,15 @@ cudaError_t mx_rows_launch(const void* x, int64_t ldx, int m, int k, int rows, i
   const int steps = mx_steps(k), segments = (steps * MX_STEP + ROWS_SEGMENT - 1) / ROWS_SEGMENT;
   const int operands = items ? max_items : (m + tile - 1) / tile, used = items ? tile : std::min(m, tile);
   if (operands > 65535) return cudaErrorInvalidConfiguration;
-  // few rows: a warp a run, for latency, in blocks whose registers leave the product's block room beside them; many: a warp a row
+  // Few rows: a warp a run, for latency, in blocks whose registers leave the product's block room beside them.  Many: two warps a row,
+  // or one with a plan, where a warp starts with a chain of look-ups and blocks of short items have nothing to do.
+  // Measured, us of the whole product from graphs: the first form / one warp a row: 48 rows by 6144 x 5120 9.3 / 12.4, 391 by 17408 x 5120
+  // 28.7 / 35.5, 1000 by 6144 x 5120 24.9 / 31.8; the first form / two warps a row / one: 2048 by 17408 x 5120 87 / 82 / 84, by
+  // 5120 x 17408 - / 104 / 121; routed layer, 2048 rows (12288 pairs), 246 / 242 / 237.
   const bool few = static_cast<int64_t>(operands) * used * segments <= 148 * 64;
   const int warps = few ? 4 : 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((used + warps - 1) / warps, operands, few ? segments : 1);
+  cfg.gridDim = dim3((used + warps - 1) / warps, operands, few ? segments : items ? 1 : std::min(segments, 2));
   cfg.blockDim = dim3(32 * warps);
   cfg.stream = stream;
   cudaLaunchAttribute attr;

@@ -27,7 +27,7 @@
 // What bounds it: windows by the weights' bytes and a fixed start and end (17408 x 5120 at one row 9.8 us among others, 4.8 TB/s;
 // 248320 x 5120 99 us, 6.8 TB/s, where the measured copy runs at 6.55); prompts by shared memory, which takes a stage's copies and
 // gives them to the MMAs again at 128 bytes a cycle, and by the stores of the results beside that (2048 rows by 17408 x 5120
-// 83 us in bursts, 4.4 PFLOP/s; 9 less without the stores; one block a tile 94).
+// 81 us in bursts, 4.5 PFLOP/s; 9 less without the stores; one block a tile 87).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -243,6 +243,7 @@ struct MxShape {
   // Drain groups of four warps; they take sixteen rows in turn.  With a plan the drain has activations to compute and quantise.
   static constexpr int GROUPS = NT == 16 ? 1 : GROUPED ? 3 : 2;
   static constexpr int THREADS = 128 + 128 * (GROUPS > 2 ? GROUPS : 2);
+  static constexpr bool SLICED = !GROUPED && NT <= MX_SB;          // may run all K slices itself (experts' and tall tiles' weights have one)
   static constexpr int CHUNKS = (NT / 16 + GROUPS - 1) / GROUPS;   // runs of sixteen rows a group drains
   // Slots: each has scale columns of its own.  (Pairs with seven slots in shared memory and five for scales, whose reuse the MMA
   // thread then waits for, took 94 us for 2048 rows by 17408 x 5120 against 88.)
@@ -795,7 +796,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     if (ti.t >= end_tile) settle_in();
     for (bool rehearsal = true; ti.t < end_tile && ok;) {
       if (!rehearsal) {
-        if (!GROUPED && slice1 - slice0 > 1) {
+        if (S::SLICED && slice1 - slice0 > 1) {
           // slices are added in registers, and the sum goes back to where the last one came from
           float acc[S::CHUNKS][16];
           for (int s = slice0; s < slice1; ++s, ++use) {
@@ -1039,8 +1040,8 @@ int round8(int m) { return (m + 7) / 8 * 8; }
 // four MMAs read 16 KB and 128 bytes a row again; a pair halves the rows' part, but its stages pass from block to block.  A tile has a
 // start and an end besides, and slices that blocks exchange cost by the row.  Tiles in several slices stay below 128 rows: the
 // sums of taller ones do not fit the drain's registers.
-// Measured, us from graphs, as chosen / the other way: pairs 17408 x 5120 at 2048 rows 84 with / 94 without, at 391 28.3 without / 29.1,
-// at 200 18.4 without / 21.7, 10240 x 2560 at 1000 23.1 with / 26.7; exchange 5120 x 17408 at 48 rows 14.3 with / 18.8 without, 6144 x 5120
+// Measured, us from graphs, as chosen / the other way: pairs 17408 x 5120 at 2048 rows 80 with / 87 without, at 700 35 with / 36,
+// at 150 15.4 without / 18.8, 10240 x 2560 at 1000 19.5 with / 20.3; exchange 5120 x 17408 at 48 rows 14.3 with / 18.8 without, 6144 x 5120
 // 8.9 with / 9.8, at 128 11.0 without / 13.5, 4096 x 4096 at 32 7.5 with / 8.1, at 128 9.1 without / 11.5.
 struct Tiling {
   int tile, cluster;

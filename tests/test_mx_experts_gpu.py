@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 # experts, D, NI, SwiGLU, limit: K of both projections ends in every part of a stage; a table wider than a block of columns
-CASES = [(9, 256, 96, True, 0.0), (24, 416, 160, True, 1.0), (12, 1184, 224, False, 0.0), (5, 2688, 1856, True, 0.0)]
+CASES = [(9, 256, 96, True, 0.0), (24, 416, 160, True, 1.0), (12, 1184, 224, False, 0.0), (5, 2688, 1856, True, 0.0), (3, 32, 32, True, 0.0)]
 
 
 def stored(w):
@@ -157,7 +157,7 @@ def test_ragged_plans(prefill):
     assert (part == 3).all() and _lib.device_error(x) == 0
 
 
-@pytest.mark.parametrize("case", [(400, 800, 416, True, 1.0), (420, 768, 800, False, 0.0)])
+@pytest.mark.parametrize("case", [(400, 800, 416, True, 1.0), (420, 768, 800, False, 0.0), (2400, 32, 32, True, 0.0)])
 def test_many_tiles(case):
     """Tables of so many tiles that blocks take them in pairs: the bits of the form for few rows, over a ragged plan, odd numbers of
     column blocks, a row of NaN and an item outside the table."""

@@ -464,6 +464,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     }
     __syncwarp();
     asm volatile("barrier.cta.arrive 4, %0;" ::"n"(S::THREADS) : "memory");
+    if (RUNS) asm volatile("barrier.cta.arrive 5, %0;" ::"n"(32 + 128) : "memory");
     if (c > 1 || PAIR) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     // ------------------------------------------------------------------ weights
     if (!GROUPED && !p.settled) pdl_wait();
@@ -504,7 +505,10 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
     pdl_launch_dependents();
   };
-  if (warp != 0 && !drains) settle_in();
+  // (an item's rows lie behind a chain of look-ups: the warps that quantise them start on it at once, and only their first arrival
+  // waits for the barriers: 1 us less a call)
+  if (RUNS && warp >= 8) asm volatile("barrier.cta.arrive 4, %0;" ::"n"(S::THREADS) : "memory");
+  else if (warp != 0 && !drains) settle_in();
 
   if (warp == 2 && !FUSED) {
     // ------------------------------------------------------------------ quantised rows
@@ -652,13 +656,16 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
       last_y = ti.y;
       ++op;
       if (op >= p.bufs && !(ok = warp_wait(smem_addr(op_empty + op % p.bufs), (op / p.bufs - 1) & 1, abort_word))) break;
+      const int member = lane < ti.rows ? __ldg(p.members + ti.m0 + lane) : -1;    // of row `lane`: a tile has at most 16
       quantize_rows(smem + (operand0 - smem_addr(smem)) + (op % p.bufs) * operand_bytes, ti.rows, warp - 8, 4, [&](int r) -> int64_t {
-        const int pair = p.members[ti.m0 + r];
+        const int pair = __shfl_sync(0xFFFFFFFFu, member, r);
         return pair < 0 || pair >= p.pairs ? -1 : p.slots > 0 ? pair / p.slots : pair;
       });
       __syncwarp();
+      if (op == 0) asm volatile("barrier.cta.sync 5, %0;" ::"n"(32 + 128) : "memory");
       if (lane == 0) mbar_arrive(op_full + op % p.bufs);
     }
+    if (op < 0) asm volatile("barrier.cta.sync 5, %0;" ::"n"(32 + 128) : "memory");
     if (!ok) give_up(ERR_WAIT_EMPTY);
   }
 
@@ -795,6 +802,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     ti.rows = 0;
     if (ti.t >= end_tile) settle_in();
     for (bool rehearsal = true; ti.t < end_tile && ok;) {
+      int pairs_ahead = pairs_of(ti, 16 * group);                    // (c is 1 with a plan)
       if (!rehearsal) {
         if (S::SLICED && slice1 - slice0 > 1) {
           // slices are added in registers, and the sum goes back to where the last one came from
@@ -854,7 +862,6 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
       Tile own = ti;
       if (c > 1) own.rows = min(ti.rows, n0 + 4 * share);
       float ahead[16];                                               // the next sixteen rows are on their way meanwhile
-      int pairs_ahead = pairs_of(own, n0 + 16 * group);
       if (c == 1 && 16 * group < ti.rows) tmem_load16(src, ahead);
 #pragma unroll 1
       for (int n = n0 + 16 * group; n < own.rows || (rehearsal && n < n0 + 16 * S::GROUPS); n += 16 * S::GROUPS) {

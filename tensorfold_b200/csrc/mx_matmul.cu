@@ -1228,6 +1228,8 @@ int tf_mx_experts(const void* x, int64_t ldx, int slots, const void* tiled, int6
   cudaError_t e;
   if (x && need == 0) {
     p.x = static_cast<const __nv_bfloat16*>(x), p.ldx = ldx, p.slots = slots;
+    // the next item's rows are quantised meanwhile (`launch` takes one buffer where two would leave under four slots).  Measured, us a
+    // layer, two / one: 128 experts 2688 / 1856, top 6, 4 rows 35.9 / 37.0, 64 experts 2048 / 768, top 8, 16 rows 34.9 / 36.8
     p.bufs = 2, p.operand_stages = p.stages;
     e = launch<16, true, true>(p, tiles, out_operands != nullptr, sms, s);
   } else {

@@ -33,9 +33,13 @@ def router(x: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None,
 
 
 class MoEBuffers:
-    """Static scratch for up to ``rows`` rows (CUDA-graph safe); ``prefill`` picks the experts' prefill arithmetic."""
+    """Static scratch for up to ``rows`` rows (CUDA-graph safe); ``prefill`` picks the experts' prefill arithmetic.  ``f32`` keeps the
+    pairs' results unrounded until ``combine`` adds them, as decode buffers always do.  Without it prompt buffers hold them in bf16,
+    as the reference does: half the bytes between the experts and the sum, and one rounding more in each pair (2.4e-3 of the
+    layer's output in place of 1.7e-3, 2048 rows of top-6 experts against 64 bits)."""
 
-    def __init__(self, rows: int, cfg, device: torch.device | str, *, prefill: bool = False, table_experts: int | None = None) -> None:
+    def __init__(self, rows: int, cfg, device: torch.device | str, *, prefill: bool = False, table_experts: int | None = None,
+                 f32: bool = False) -> None:
         slots = cfg.num_experts_per_tok + 1
         self.rows, self.slots = rows, slots
         self.logits = torch.empty((rows, cfg.num_experts + 1), dtype=torch.float32, device=device)
@@ -45,7 +49,7 @@ class MoEBuffers:
         self.plan = grouped.Plan(rows, slots, experts, device, prefill=prefill)
         # [row, slot] in the decode form; the prefill form keeps its pairs in member order (by expert) instead
         self.act = torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=torch.bfloat16, device=device)
-        self.y = torch.empty((rows, slots, cfg.hidden_size), dtype=torch.bfloat16 if prefill else torch.float32,
+        self.y = torch.empty((rows, slots, cfg.hidden_size), dtype=torch.bfloat16 if prefill and not f32 else torch.float32,
                              device=device)
 
 
@@ -90,7 +94,7 @@ class SharedExpert:
 
 def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts | mx_experts.Experts, buf: MoEBuffers, top_k: int,
         experts: int, shared: SharedExpert | None = None) -> MoEBuffers:
-    """Route x [R, D] and run its experts into buf.y [R, k + 1, D] (bf16 in prefill); slot k is the shared expert.  The experts
+    """Route x [R, D] and run its experts into buf.y [R, k + 1, D]; slot k is the shared expert.  The experts
     are affine (``experts.make``) or microscaled (``mx_experts.make``)."""
 
     rows = x.shape[0]
@@ -127,7 +131,7 @@ def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts | mx_exp
 
 
 def combine(y: torch.Tensor, wts: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """y [R, S, D] (fp32, or bf16 in prefill) and wts [R, S] fp32 -> [R, D] bf16; a row's bits never depend on R."""
+    """y [R, S, D] (fp32 or bf16) and wts [R, S] fp32 -> [R, D] bf16; a row's bits never depend on R."""
 
     rows, slots, dims = y.shape
     if not y.is_contiguous() or wts.dtype != torch.float32 or wts.shape != (rows, slots) or not wts.is_contiguous():
@@ -165,14 +169,15 @@ class _Shape:
 _scratch: dict[tuple, MoEBuffers] = {}
 
 
-def run(x: torch.Tensor, m: Routed, *, prefill: bool = False) -> torch.Tensor:
-    """x [R, D] bf16 -> [R, D] bf16: its top-k experts by renormalized softmax weight plus the shared expert."""
+def run(x: torch.Tensor, m: Routed, *, prefill: bool = False, f32: bool = False) -> torch.Tensor:
+    """x [R, D] bf16 -> [R, D] bf16: its top-k experts by renormalized softmax weight plus the shared expert.  ``f32``: prompts
+    keep the pairs' results unrounded until they are added, as decode does (see ``MoEBuffers``)."""
 
     rows = x.shape[0]
     size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
-    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, x.device, m.experts.count)
+    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, prefill and f32, x.device, m.experts.count)
     buf = _scratch.get(key)
     if buf is None:
-        buf = _scratch[key] = MoEBuffers(size, _Shape(m), x.device, prefill=prefill, table_experts=m.experts.count)
+        buf = _scratch[key] = MoEBuffers(size, _Shape(m), x.device, prefill=prefill, table_experts=m.experts.count, f32=f32)
     moe(x.contiguous(), m.router, m.experts, buf, m.top_k, m.count, m.shared)
     return combine(buf.y[:rows], buf.wts[:rows])

@@ -188,7 +188,7 @@ def prepare(case: dict, seed: int) -> dict:
         prompt = c["rows"] > ROUTED_DECODE_ROWS
         s["table"] = mx_experts.make([s["gate"], s["up"]], s["down"])
         s["plan"] = experts.Plan(c["rows"], c["top_k"], e, DEV, prefill=prompt)
-        s["y"] = torch.empty((c["rows"] * c["top_k"], d), dtype=torch.bfloat16 if prompt else torch.float32, device=DEV)
+        s["y"] = torch.empty((c["rows"] * c["top_k"], d), dtype=torch.float32, device=DEV)   # rounded once, after the slots are added
     return s
 
 

@@ -323,6 +323,10 @@ int tf_mx_split(int n, int k);
 int64_t tf_mx_matmul_bytes(int m, int n, int k);
 int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
                  void* work, int64_t work_bytes, int pdl, void* stream);
+/* tf_mx_matmul of one row (x: k bf16 values, out: n fp32 values) in which the block of K slice `slice` (of tf_mx_split(n, k) > 1)
+ * gives up at once and sends nothing: the others wait their limit (about a second), all of them return, and tf_device_error
+ * reports 1.  For hosts that check, on a healthy GPU, that a lost slice leaves the context usable (tf_selftest_lost_wait). */
+int tf_mx_selftest_lost_slice(int slice, const void* x, const void* tiled, int n, int k, void* out, void* stream);
 /* The grouped form over a plan (tf_moe_plan, items of `tile` pairs: a multiple of 8 up to 128): as tf_moe_experts, with K in one
  * slice.  Input: bf16 rows x with work of tf_mx_experts_bytes(k, tile, max_items) bytes, or with x NULL work that an earlier call
  * filled as out_operands.  Output: out as in tf_moe_experts, or out_operands, where the results (activations: epi 1 or 2) are

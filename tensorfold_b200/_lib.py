@@ -78,6 +78,7 @@ SIGNATURES = {
     "tf_mx_split": (_i32, (_i32, _i32)),
     "tf_mx_matmul_bytes": (_i64, (_i32, _i32, _i32)),
     "tf_mx_matmul": (_i32, (_vp, _i64, _i32, _vp, _i32, _i32, _vp, _i64, _i32, _i32, ctypes.c_float, _vp, _i64, _i32, _vp)),
+    "tf_mx_selftest_lost_slice": (_i32, (_i32, _vp, _vp, _i32, _i32, _vp, _vp)),
     "tf_mx_operand_bytes": (_i64, (_i32, _i32)),
     "tf_mx_experts_bytes": (_i64, (_i32, _i32, _i32)),
     "tf_mx_experts": (_i32, (_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _i32,

@@ -95,6 +95,7 @@ struct MxParams {
   const int *items, *counts, *members;
   int experts, pairs, max_items;
   int settled;                  // no kernel in flight writes the weights or the plan: they are read before the dependency wait
+  int lose;                     // self-test: the drain of cluster rank `lose` - 1 gives up its wait for the accumulator at once (0: none)
   int* err;
 };
 
@@ -187,6 +188,11 @@ __device__ __forceinline__ uint32_t lane_test(uint32_t bar, uint32_t parity) {
   asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
+// A block of a cluster sends slices into the others' shared memory, so none of them leaves before all have sent theirs or given up:
+// every thread arrives once its sends are issued, and waits before the block returns.  Relaxed: the slices are counted by the barrier
+// that their owner waits for.
+__device__ __forceinline__ void sends_are_issued() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void all_sends_are_issued() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ void let_copies_land() {
   for (int i = 0; i < 64; ++i) __nanosleep(20000);
 }
@@ -671,6 +677,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     if (!ok) give_up(ERR_WAIT_EMPTY);
   }
 
+  if (c > 1 && !drains) sends_are_issued();
   if (drains) {
     // ------------------------------------------------------------------ drain
     const int lg = warp & 3;
@@ -795,7 +802,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
     // Sixteen rows at a time straight from tensor memory.  The loop is not unrolled and its body is kept small: unrolled over
     // a tile (5900 instructions) the warps mostly waited for instructions, and a tile of 256 rows took 42 us.  For the same reason
     // it runs once over no rows before the first accumulator is ready: its instructions are at hand then.
-    bool ok = true;
+    bool ok = true, sending = c > 1;
     int use = 0;
     uint32_t lanes = 0;
     Tile ti = first(), then = {};
@@ -833,7 +840,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
             if (lane == 0) release(use & 1);
           }
         } else {
-          ok = warp_wait(acc_full32 + 8 * (use & 1), (use >> 1) & 1, abort_word);
+          ok = (c == 1 || p.lose != static_cast<int>(rank) + 1) && warp_wait(acc_full32 + 8 * (use & 1), (use >> 1) & 1, abort_word);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         if (GROUPED && p.q != nullptr) ok = agreed(1 + group, ok);   // (a group's warps meet at barriers below: all of them or none)
@@ -858,7 +865,12 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
             if (++at == share) at = 0, ++owner;
           }
         }
-        if (!rehearsal && !(ok = warp_wait(smem_addr(parts), 0, abort_word))) break;
+        if (!rehearsal) {
+          ok = warp_wait(smem_addr(parts), 0, abort_word);
+          sends_are_issued();
+          sending = false;
+          if (!ok) break;
+        }
         n0 = 4 * rank * share;
       }
       Tile own = ti;
@@ -921,6 +933,7 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
       if (GROUPED) then = after(ti);
     }
     if (!ok) give_up(ERR_WAIT_FULL);
+    if (sending) sends_are_issued();                                 // gave up before it had any
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -928,6 +941,9 @@ __global__ void __launch_bounds__(MxShape<NT, FUSED, GROUPED, PAIR>::THREADS, 1)
   if (PAIR) {                                                        // neither block leaves before both are done
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  } else if (c > 1) {
+    all_sends_are_issued();
+    if (*abort_flag) let_copies_land();                              // (the last ones sent to a block that did not wait for them)
   }
   if (warp == 1) {
     __syncwarp();
@@ -1130,8 +1146,8 @@ int64_t tf_mx_matmul_bytes(int m, int n, int k) {
   return (m + tile - 1) / tile * mx_operand_bytes(tile, steps);
 }
 
-int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
-                 void* work, int64_t work_bytes, int pdl, void* stream) {
+static int mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
+                     void* work, int64_t work_bytes, int pdl, int lose, void* stream) {
   if (m < 1 || m > MX_LONGEST || !mx_sizes(n, k)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: K must be a positive multiple of 32, n and m positive");
   if (epi < 0 || epi > 2 || (epi == 2 && n % 32) || (epi != 0 && out_f32)) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: bad epilogue");
   if (!x || !tiled || !out || ldo < (epi == 2 ? n / 2 : n) || ldx < k) return fail_moe(TF_ERR_ARG, "tf_mx_matmul: null pointer or short rows");
@@ -1151,6 +1167,7 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
   p.sk = slices_for(n, k);
   p.out = out, p.ldo = ldo, p.out_f32 = out_f32, p.epi = epi, p.limit = limit;
   p.err = err;
+  p.lose = lose;
   p.bufs = 1;
   const int64_t ncb = (n + MX_SB - 1) / MX_SB;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1176,6 +1193,19 @@ int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, in
     e = t.pair ? launch_pairs(p, row_tiles, sms, s) : launch_rows(p, ncb * row_tiles, sms, s);
   }
   return e == cudaSuccess ? TF_OK : cuda_fail_moe(e, "tf_mx_matmul");
+}
+
+int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,
+                 void* work, int64_t work_bytes, int pdl, void* stream) {
+  return mx_matmul(x, ldx, m, tiled, n, k, out, ldo, out_f32, epi, limit, work, work_bytes, pdl, 0, stream);
+}
+
+int tf_mx_selftest_lost_slice(int slice, const void* x, const void* tiled, int n, int k, void* out, void* stream) {
+  if (!mx_sizes(n, k)) return fail_moe(TF_ERR_ARG, "tf_mx_selftest_lost_slice: K must be a positive multiple of 32, n positive");
+  const int sk = slices_for(n, k);
+  if (sk < 2 || slice < 0 || slice >= sk || !fused_pays(1, k, sk))
+    return fail_moe(TF_ERR_ARG, "tf_mx_selftest_lost_slice: one of the slices of a weight that runs in several, and in the block");
+  return mx_matmul(x, k, 1, tiled, n, k, out, n, 1, MX_STORE, 0.f, nullptr, 0, 0, slice + 1, stream);
 }
 
 int64_t tf_mx_operand_bytes(int rows, int k) {

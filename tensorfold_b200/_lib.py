@@ -145,6 +145,12 @@ def stream_of(t) -> int:
     return native().stream_of(t)
 
 
+def use_of(t) -> tuple:
+    """``stream_of`` and the capture that stream is in (None: not capturing): buffers kept from call to call belong to the pair."""
+
+    return native().use_of(t)
+
+
 def device_error(t) -> int:
     """Read and clear the error word kernels set when a bounded wait gave up (0: none).  Synchronises the stream."""
 

@@ -803,6 +803,18 @@ PyObject* py_stream_of(PyObject*, PyObject* t) {
   return guarded([&] { return PyLong_FromVoidPtr(stream_of(tensor(t, "stream_of"))); });
 }
 
+// use_of(tensor) -> (current stream, the capture it is in or None): what buffers that a call keeps for the next one belong to
+PyObject* py_use_of(PyObject*, PyObject* t) {
+  return guarded([&]() -> PyObject* {
+    const cudaStream_t stream = stream_of(tensor(t, "use_of"));
+    cudaStreamCaptureStatus status;
+    unsigned long long capture = 0;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &capture));
+    if (status == cudaStreamCaptureStatusNone) return Py_BuildValue("(NO)", PyLong_FromVoidPtr(stream), Py_None);
+    return Py_BuildValue("(NK)", PyLong_FromVoidPtr(stream), capture);
+  });
+}
+
 PyObject* py_forget_scratch(PyObject*, PyObject*) {
   g_scratch.clear();
   g_counters.clear();
@@ -840,6 +852,7 @@ PyMethodDef g_methods[] = {
     {"bind", py_bind, METH_VARARGS, nullptr},
     {"hooks", py_hooks, METH_VARARGS, nullptr},
     {"stream_of", py_stream_of, METH_O, nullptr},
+    {"use_of", py_use_of, METH_O, nullptr},
     {"forget_scratch", py_forget_scratch, METH_NOARGS, nullptr},
     TF_FAST(matmul) TF_FAST(matmul_set) TF_FAST(prefill_matmul) TF_FAST(matmul_act) TF_FAST(add_rmsnorm) TF_FAST(swiglu)
     TF_FAST(mx_quantize) TF_FAST(mx_dequantize) TF_FAST(mx_matmul) TF_FAST(mx_experts)

@@ -123,15 +123,16 @@ class Plan:
     """Scratch grouping pairs by expert: members, items (expert, first, count), counts [items, distinct experts]."""
 
     def __init__(self, rows: int, slots: int, experts: int, device: torch.device | str, *,
-                 prefill: bool = False) -> None:
-        pairs = rows * slots
+                 prefill: bool = False, cleared: bool = True) -> None:
+        # ``cleared``: a plan that nothing was routed into holds no items; without it ``route`` must come before every other use
+        pairs, new = rows * slots, torch.zeros if cleared else torch.empty
         self.rows, self.slots, self.experts, self.prefill = rows, slots, experts, prefill
         self.tile = PREFILL_TILE if prefill else decode_tile(pairs, experts)
-        self.members = torch.zeros((pairs,), dtype=torch.int32, device=device)
-        self.items = torch.zeros((max_items(pairs, experts, self.tile), 3), dtype=torch.int32, device=device)
-        self.counts = torch.zeros((2,), dtype=torch.int32, device=device)
-        self.rank = torch.zeros((pairs,), dtype=torch.int32, device=device)
-        self.hist = torch.zeros((-(-pairs // SMALL) * experts,), dtype=torch.int32, device=device)
+        self.members = new((pairs,), dtype=torch.int32, device=device)
+        self.items = new((max_items(pairs, experts, self.tile), 3), dtype=torch.int32, device=device)
+        self.counts = new((2,), dtype=torch.int32, device=device)
+        self.rank = new((pairs,), dtype=torch.int32, device=device)
+        self.hist = new((-(-pairs // SMALL) * experts,), dtype=torch.int32, device=device)
         self.sorted = None       # prefill form: the call's rows in member order (made on first use, before any capture)
 
 

@@ -39,14 +39,14 @@ class MoEBuffers:
     layer's output in place of 1.7e-3, 2048 rows of top-6 experts against 64 bits)."""
 
     def __init__(self, rows: int, cfg, device: torch.device | str, *, prefill: bool = False, table_experts: int | None = None,
-                 f32: bool = False) -> None:
+                 f32: bool = False, cleared: bool = True) -> None:
         slots = cfg.num_experts_per_tok + 1
         self.rows, self.slots = rows, slots
         self.logits = torch.empty((rows, cfg.num_experts + 1), dtype=torch.float32, device=device)
         self.pick = torch.empty((rows, slots), dtype=torch.int32, device=device)
         self.wts = torch.empty((rows, slots), dtype=torch.float32, device=device)
         experts = cfg.num_experts + 1 if table_experts is None else table_experts
-        self.plan = grouped.Plan(rows, slots, experts, device, prefill=prefill)
+        self.plan = grouped.Plan(rows, slots, experts, device, prefill=prefill, cleared=cleared)
         # [row, slot] in the decode form; the prefill form keeps its pairs in member order (by expert) instead
         self.act = torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=torch.bfloat16, device=device)
         self.y = torch.empty((rows, slots, cfg.hidden_size), dtype=torch.bfloat16 if prefill and not f32 else torch.float32,
@@ -166,7 +166,28 @@ class _Shape:
         self.moe_intermediate_size, self.hidden_size = m.experts.width, m.experts.dims
 
 
-_scratch: dict[tuple, MoEBuffers] = {}
+_scratch: dict[tuple, MoEBuffers] = {}                           # (a call's shape, stream) -> what eager calls use
+_captured: dict[tuple, tuple[int, MoEBuffers]] = {}              # the same -> the last capture's, and which capture that was
+
+
+def _kept(shape: tuple, stream: int, capture: int | None, make) -> MoEBuffers:
+    """Buffers for a call of ``shape``, or ``make(cleared)``.  Eager calls share them along a stream, whose calls run one after another;
+    calls on other streams have their own.  A captured call, whose graph may be replayed beside anything, uses buffers of the graph's:
+    the calls of one capture on a stream share them, and they are held until the stream is seen outside that capture."""
+
+    key = (*shape, stream)
+    owner, buf = _captured.get(key, (None, None))
+    if owner is not None and owner != capture:
+        del _captured[key]
+        buf = None
+    if capture is None:
+        buf = _scratch.get(key)
+        if buf is None:
+            buf = _scratch[key] = make(True)
+    elif buf is None:
+        buf = make(False)                                       # (clearing would be five graph nodes; run routes first)
+        _captured[key] = capture, buf
+    return buf
 
 
 def run(x: torch.Tensor, m: Routed, *, prefill: bool = False, f32: bool = False) -> torch.Tensor:
@@ -175,9 +196,8 @@ def run(x: torch.Tensor, m: Routed, *, prefill: bool = False, f32: bool = False)
 
     rows = x.shape[0]
     size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
-    key = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, prefill and f32, x.device, m.experts.count)
-    buf = _scratch.get(key)
-    if buf is None:
-        buf = _scratch[key] = MoEBuffers(size, _Shape(m), x.device, prefill=prefill, table_experts=m.experts.count, f32=f32)
+    shape = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, x.device, m.experts.count, prefill and f32)
+    buf = _kept(shape, *_lib.use_of(x), lambda cleared: MoEBuffers(size, _Shape(m), x.device, prefill=prefill, table_experts=m.experts.count,
+                                                                   f32=f32, cleared=cleared))
     moe(x.contiguous(), m.router, m.experts, buf, m.top_k, m.count, m.shared)
     return combine(buf.y[:rows], buf.wts[:rows])

@@ -4,8 +4,8 @@ import pytest
 import torch
 
 import mx_util
-from tensorfold_b200 import _lib
-from tensorfold_b200.cuda import moe, mx_experts
+from tensorfold_b200 import _lib, synthetic
+from tensorfold_b200.cuda import experts, moe, mx_experts
 from test_mx_experts_gpu import build
 
 pytestmark = pytest.mark.gpu
@@ -40,3 +40,57 @@ def test_prompt_pairs_stay_unrounded(rows):
     assert ((got.double() - ref).abs() <= bound).all()
     assert torch.equal(got, moe.combine(y, buf.wts)) and torch.equal(moe.run(x[:1], layer, prefill=True, f32=True), got[:1])
     assert _lib.device_error(x) == 0
+
+
+def affine_layer(e=12, d=384, ni=128, k=3):
+    dev = lambda i, n, kk: tuple(torch.stack([synthetic.affine_weight(n, kk, 4, 64, seed=100 * i + j)[t] for j in range(e)]).to(DEV) for t in range(3))
+    ex = experts.make([dev(1, ni, d), dev(2, ni, d)], dev(3, d, ni), 64)
+    return moe.Routed(layer_of(e=e, d=d, ni=ni, k=k).router, ex, k)
+
+
+@pytest.mark.parametrize("kind", ["mx", "affine"])
+@pytest.mark.parametrize("rows,prefill", [(5, False), (40, True)])
+def test_layers_of_one_shape_run_side_by_side(kind, rows, prefill, monkeypatch):
+    """A layer that is held up between its plan and its experts, while another of its shape runs from end to end on another stream or in
+    a graph, still gets its own plan's pairs."""
+
+    layer = layer_of() if kind == "mx" else affine_layer()
+    xs = [mx_util.rows(rows, 384, seed, DEV, std=0.5) for seed in (1, 2, 3)]
+    want = [moe.run(x, layer, prefill=prefill) for x in xs]
+    slow, quick = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs = []
+    for x in xs[1:]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = moe.run(x, layer, prefill=prefill)
+        graphs.append((graph, out))
+    select = moe.select
+
+    def held_up(*args):
+        select(*args)
+        if torch.cuda.current_stream() == slow:
+            torch.cuda._sleep(4_000_000)                       # about two milliseconds
+
+    monkeypatch.setattr(moe, "select", held_up)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(slow):
+            got = [moe.run(xs[0], layer, prefill=prefill)]
+        with torch.cuda.stream(quick):
+            got.append(moe.run(xs[1], layer, prefill=prefill))
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(graphs[1][1], want[2])
+    slow_graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(slow_graph, stream=slow):
+        out = moe.run(xs[0], layer, prefill=prefill)
+    for _ in range(3):                                         # two graphs at once, eager calls beside them
+        out.zero_(), graphs[0][1].zero_(), torch.cuda.synchronize()
+        with torch.cuda.stream(slow):
+            slow_graph.replay()
+        with torch.cuda.stream(quick):
+            graphs[0][0].replay()
+            again = moe.run(xs[2], layer, prefill=prefill)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(graphs[0][1], want[1]) and torch.equal(again, want[2])
+    assert _lib.device_error(xs[0]) == 0

@@ -235,8 +235,10 @@ __device__ __forceinline__ bool agreed(int barrier, bool ok) {
 // Fours of rows each of the c blocks of a cluster owns when they add their slices.
 __host__ __device__ __forceinline__ int quads_of(int rows, int c) { return ((rows + 3) / 4 + c - 1) / c; }
 
-// silu(gate) * up in fp32.
-__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
+// silu(gate) * up in fp32.  The fast division (2 units in the last place) gives 0 for a denominator past 2^126, which gates below -87.3 have
+// and ups may bring back into sight: both sides are quarters, so that 1 + e^-g, finite to 2^128, stays below it.  The exact division
+// takes its own subroutine: one routed row 21.0 us in place of 17.2, 391 rows of a 2 x 17408 x 5120 pair 57 in place of 47.
+__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(0.25f * g, fmaf(0.25f, expf(-g), 0.25f)) * u; }
 
 template <int NT, bool FUSED, bool GROUPED, bool PAIR = false>
 struct MxShape {

@@ -317,6 +317,7 @@ int tf_mx_unpack(const void* tiled, int n, int k, void* words, void* scales, voi
  * chain of 64-input steps, added in order, so a row's bits never depend on m.  epi and limit as in tf_qmm_act, but activations
  * are computed from the fp32 sums and rounded once.  The launches use programmatic stream serialisation and read global memory only
  * once the previous kernel is done; with pdl = 1 the weights are read before that, so they must be settled (as in tf_qmm).
+ *   out      may not share memory with x, which windows read while they store (of tf_mx_experts, neither, with bf16 rows x and out)
  *   work     tf_mx_matmul_bytes(m, n, k) bytes (0 for decode and verify windows: the kernel quantises the rows itself), 16-byte
  *            aligned, contents free; calls that may overlap need different work */
 int tf_mx_split(int n, int k);

@@ -550,6 +550,24 @@ bool whole_rows(const at::Tensor& x, int64_t k) {       // rows that the kernels
   return x.stride(1) == 1 && (x.size(0) <= 1 || (x.stride(0) * x.element_size() % 16 == 0 && x.stride(0) >= k)) && aligned(x.data_ptr(), 16);
 }
 
+// Blocks that quantise their own rows read x while others store: the two must not share a byte.  Rows that lie side by side in rows of
+// one buffer do not.
+void apart(const at::Tensor& x, const at::Tensor& out, const char* who) {
+  struct Span {
+    uintptr_t from, pitch, width, to;
+    explicit Span(const at::Tensor& t)
+        : from(reinterpret_cast<uintptr_t>(t.data_ptr())), pitch(static_cast<uintptr_t>(t.stride(0)) * t.element_size()),
+          width(static_cast<uintptr_t>(t.size(1)) * t.element_size()), to(from + (t.size(0) - 1) * pitch + width) {}
+  };
+  const Span a(x), b(out);
+  if (a.to <= b.from || b.to <= a.from) return;
+  if (x.size(0) > 1 && out.size(0) > 1 && a.pitch == b.pitch) {
+    const uintptr_t at = a.from <= b.from ? (b.from - a.from) % a.pitch : (a.pitch - (a.from - b.from) % a.pitch) % a.pitch;
+    if (at >= a.width && at + b.width <= a.pitch) return;
+  }
+  refuse("%s: out shares memory with x", who);
+}
+
 at::Tensor blocks(at::IntArrayRef sizes, int64_t last, at::ScalarType type, const at::Tensor& like) {
   at::DimVector shape(sizes.begin(), sizes.end());
   shape.back() = last;
@@ -628,6 +646,7 @@ PyObject* mx_matmul(PyObject* const* a) {
   const int m = static_cast<int>(x.size(0)), cols = epi == 2 ? n / 2 : n;
   const at::Tensor out = out_of(a[5], m, cols, f32 ? at::kFloat : at::kBFloat16, x, who);
   if (out.device() != x.device() || (m > 1 && out.stride(0) < cols)) refuse("%s: out must have rows of its own on x's device", who);
+  if (a[5] != Py_None) apart(x, out, who);
   const int64_t need = p_tf_mx_matmul_bytes(m, n, k);
   at::Tensor work;
   if (need > 0) work = empty({need}, at::kByte, x);
@@ -707,6 +726,7 @@ PyObject* mx_experts(PyObject* const* a) {
   // (the rows are strided by the C entry, so a single row needs a legal stride too)
   const bool fetchable = given.stride(1) == 1 && given.stride(0) % 8 == 0 && given.stride(0) >= k && aligned(given.data_ptr(), 16);
   const at::Tensor x = fetchable ? given : given.clone(at::MemoryFormat::Contiguous);
+  if (what != 0) apart(x, out, who);                          // (both projections: x has been read before out is written)
   const int64_t items = std::min(std::min(pairs, e.experts) + pairs / e.tile, e.items.size(0));
   const int epi = e.gated ? 2 : 1;
   if (what == 1) {

@@ -125,7 +125,8 @@ def _packed(q: MX4, who: str) -> torch.Tensor:
 
 
 def matmul(x: torch.Tensor, q: MX4, *, f32: bool = False, out: torch.Tensor | None = None, pdl: bool = False) -> torch.Tensor:
-    """x (M, k) bf16, quantised as by ``quantize``, times q.T as (M, n) bf16, or unrounded fp32 with ``f32``.
+    """x (M, k) bf16, quantised as by ``quantize``, times q.T as (M, n) bf16, or unrounded fp32 with ``f32``.  ``out`` may not share
+    memory with x.
 
     ``pdl`` launches with programmatic stream serialisation so that the weights' first bytes overlap the end of the previous
     kernel in the stream: they must not be what a kernel still in flight writes."""

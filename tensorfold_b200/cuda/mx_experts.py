@@ -58,7 +58,8 @@ def _call(what: int, x: torch.Tensor, ex: Experts, plan: grouped.Plan, out: torc
 
 
 def gate_up(x: torch.Tensor, ex: Experts, plan: grouped.Plan, out: torch.Tensor, rows: int) -> None:
-    """x [R, D] bf16 -> out [R * slots, NI] bf16, each pair's activation (rounded once from its fp32 sums)."""
+    """x [R, D] bf16 -> out [R * slots, NI] bf16, each pair's activation (rounded once from its fp32 sums).  ``out`` may not share
+    memory with x (nor act's in ``down``; ``layer`` has read x before it writes)."""
 
     _call(1, x, ex, plan, out, rows)
 

@@ -81,6 +81,15 @@ def select(logits: torch.Tensor, buf: MoEBuffers, top_k: int, experts: int) -> N
     grouped.route(buf.pick[:logits.shape[0]], buf.plan)
 
 
+def run_experts(x: torch.Tensor, ex: grouped.Experts | mx_experts.Experts, buf: MoEBuffers, rows: int) -> None:
+    """The pairs of buf's plan through their experts, affine (``experts.make``) or microscaled (``mx_experts.make``), into buf.y."""
+
+    if isinstance(ex, mx_experts.Experts):
+        mx_experts.layer(x, ex, buf.plan, buf.y.view(-1, ex.dims), rows)
+    else:
+        grouped.layer(x, ex, buf.plan, buf.act.view(-1, ex.width), buf.y.view(-1, ex.dims), rows)
+
+
 @dataclass
 class SharedExpert:
     """A shared expert of its own width, run as dense projections: ``up`` is a ``qmm.pack_pair`` weight (gate and up
@@ -102,10 +111,7 @@ def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts | mx_exp
     def routed() -> None:
         router(x, router_rows, buf.logits[:rows], prefill=buf.plan.prefill)
         select(buf.logits[:rows], buf, top_k, experts)
-        if isinstance(ex, mx_experts.Experts):
-            mx_experts.layer(x, ex, buf.plan, buf.y.view(-1, ex.dims), rows)
-        else:
-            grouped.layer(x, ex, buf.plan, buf.act.view(-1, ex.width), buf.y.view(-1, ex.dims), rows)
+        run_experts(x, ex, buf, rows)
 
     def dense() -> None:
         if isinstance(shared.up, mx.MX4):

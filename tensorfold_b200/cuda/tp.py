@@ -17,8 +17,8 @@ import torch.distributed as dist
 
 from .. import _lib
 from . import experts as grouped
-from . import moe
-from .kernels import qmm
+from . import moe, mx_experts
+from .kernels import mx, qmm
 from ..families.qwen3_5.cuda import distributed
 from ..families.qwen3_5.cuda.weights import QLinear
 
@@ -185,17 +185,17 @@ class ExpertParallelMoE:
     """One rank's share of a routed layer: the full router, the local experts and their first global id."""
 
     router: torch.Tensor            # [E (+1), D] bf16: every rank routes every row
-    experts: grouped.Experts        # local experts only
+    experts: grouped.Experts | mx_experts.Experts    # local experts only
     top_k: int
     first: int                      # global id of local expert 0
     total: int                      # experts in the whole layer
     has_shared_row: bool = False    # router carries a shared-expert gate row after the experts' (not read here)
 
-    def buffers(self, rows: int, device, *, prefill: bool = False) -> moe.MoEBuffers:
+    def buffers(self, rows: int, device, *, prefill: bool = False, f32: bool = False) -> moe.MoEBuffers:
         class _Cfg:
             num_experts_per_tok, num_experts = self.top_k, self.total
             moe_intermediate_size, hidden_size = self.experts.width, self.experts.dims
-        return moe.MoEBuffers(rows, _Cfg, device, prefill=prefill, table_experts=self.experts.count)
+        return moe.MoEBuffers(rows, _Cfg, device, prefill=prefill, table_experts=self.experts.count, f32=f32)
 
     def partial(self, x: torch.Tensor, buf: moe.MoEBuffers, out: torch.Tensor | None = None) -> torch.Tensor:
         """This rank's contribution [R, D] bf16: its experts' slots combined, the others weighted zero."""
@@ -207,7 +207,7 @@ class ExpertParallelMoE:
         moe.select_local_rows(logits, buf, self.top_k, self.total, self.first, self.experts.count)
         wts = buf.wts[:rows]
         grouped.route(buf.pick[:rows], buf.plan)
-        grouped.layer(x, self.experts, buf.plan, buf.act.view(-1, self.experts.width), buf.y.view(-1, self.experts.dims), rows)
+        moe.run_experts(x, self.experts, buf, rows)
         return moe.combine(buf.y[:rows], wts, out)
 
     def run(self, x: torch.Tensor, buf: moe.MoEBuffers, group=None, reducer: PeerReducer | None = None) -> torch.Tensor:
@@ -219,9 +219,10 @@ class ExpertParallelMoE:
 
 @dataclass
 class RowParallelLinear:
-    """A projection whose inputs are split across ranks in whole groups; ``forward`` reduces the partials."""
+    """A projection whose inputs are split across ranks in whole groups (microscaled ones: blocks, see
+    ``checkpoint.load_microscaled``); ``forward`` reduces the partials."""
 
-    q: qmm.Q4
+    q: qmm.Q4 | mx.MX4
 
     @staticmethod
     def shard(q: QLinear, rank: int, world: int) -> "RowParallelLinear":
@@ -232,7 +233,7 @@ class RowParallelLinear:
         """This rank's share of the sums: fp32, unrounded (``f32=False`` rounds the share to bf16 first: half the
         bytes on the wire, two roundings instead of one, not what the reference does)."""
 
-        return qmm.matmul(x_local, self.q, f32=f32)
+        return (mx if isinstance(self.q, mx.MX4) else qmm).matmul(x_local, self.q, f32=f32)
 
     def forward(self, x_local: torch.Tensor, group=None, *, f32: bool = True) -> torch.Tensor:
         """fp32 partials summed in rank order and rounded once (families/qwen3_5/cuda/distributed.py:249-284)."""
@@ -244,7 +245,7 @@ class RowParallelLinear:
 class ColumnParallelLinear:
     """A projection whose output rows are split across ranks; no reduction."""
 
-    q: qmm.Q4
+    q: qmm.Q4 | mx.MX4
 
     @staticmethod
     def shard(q: QLinear, rank: int, world: int, segments=None, block: int = 1) -> "ColumnParallelLinear":
@@ -252,4 +253,4 @@ class ColumnParallelLinear:
         return ColumnParallelLinear(qmm.pack(part.weight, part.scales, part.biases, part.gs, bits=part.bits))
 
     def forward(self, x: torch.Tensor, **kw) -> torch.Tensor:
-        return qmm.matmul(x, self.q, **kw)
+        return (mx if isinstance(self.q, mx.MX4) else qmm).matmul(x, self.q, **kw)

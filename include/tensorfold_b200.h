@@ -318,8 +318,9 @@ int tf_mx_unpack(const void* tiled, int n, int k, void* words, void* scales, voi
  * are computed from the fp32 sums and rounded once.  The launches use programmatic stream serialisation and read global memory only
  * once the previous kernel is done; with pdl = 1 the weights are read before that, so they must be settled (as in tf_qmm).
  *   out      may not share memory with x, which windows read while they store (of tf_mx_experts, neither, with bf16 rows x and out)
- *   work     tf_mx_matmul_bytes(m, n, k) bytes (0 for decode and verify windows: the kernel quantises the rows itself), 16-byte
- *            aligned, contents free; calls that may overlap need different work */
+ *   work     tf_mx_matmul_bytes(m, n, k) bytes, 16-byte aligned, contents free; calls that may overlap need different work.  Ask for
+ *            every m: 0 where blocks quantise the rows themselves, which depends on all three (17408 x 5120: up to 4 rows, 1024 x
+ *            5120: up to 16), and null work is refused elsewhere */
 int tf_mx_split(int n, int k);
 int64_t tf_mx_matmul_bytes(int m, int n, int k);
 int tf_mx_matmul(const void* x, int64_t ldx, int m, const void* tiled, int n, int k, void* out, int64_t ldo, int out_f32, int epi, float limit,

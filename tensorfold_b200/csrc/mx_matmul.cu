@@ -12,7 +12,8 @@
 // MMAs), to columns that belong to the stage's slot: they are free when the slot is.
 //
 // Forms (template):
-//   FUSED    up to 16 rows: the block quantises bf16 rows itself into shared memory while its weights arrive, one launch in all
+//   FUSED    few rows (`fused_pays`, 16 at most): the block quantises bf16 rows itself into shared memory while its weights arrive,
+//            one launch in all
 //   GROUPED  a tile is a plan's item (expert, first, count) x 128 columns; activations may leave quantised, as the next
 //            projection's operands
 //   PAIR     prompts: two blocks on an SM pair share 256 columns x up to 192 rows, or an item's 128 (cta_group::2), half of the rows

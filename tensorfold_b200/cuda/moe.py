@@ -39,7 +39,7 @@ class MoEBuffers:
     layer's output in place of 1.7e-3, 2048 rows of top-6 experts against 64 bits)."""
 
     def __init__(self, rows: int, cfg, device: torch.device | str, *, prefill: bool = False, table_experts: int | None = None,
-                 f32: bool = False, cleared: bool = True) -> None:
+                 f32: bool = False, microscaled: bool = False, cleared: bool = True) -> None:
         slots = cfg.num_experts_per_tok + 1
         self.rows, self.slots = rows, slots
         self.logits = torch.empty((rows, cfg.num_experts + 1), dtype=torch.float32, device=device)
@@ -47,8 +47,9 @@ class MoEBuffers:
         self.wts = torch.empty((rows, slots), dtype=torch.float32, device=device)
         experts = cfg.num_experts + 1 if table_experts is None else table_experts
         self.plan = grouped.Plan(rows, slots, experts, device, prefill=prefill, cleared=cleared)
-        # [row, slot] in the decode form; the prefill form keeps its pairs in member order (by expert) instead
-        self.act = torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=torch.bfloat16, device=device)
+        # [row, slot] in the decode form; the prefill form keeps its pairs in member order (by expert) instead.  Microscaled experts
+        # quantise their activations for the next projection, in a workspace of the call's
+        self.act = None if microscaled else torch.empty((rows, slots, cfg.moe_intermediate_size), dtype=torch.bfloat16, device=device)
         self.y = torch.empty((rows, slots, cfg.hidden_size), dtype=torch.bfloat16 if prefill and not f32 else torch.float32,
                              device=device)
 
@@ -86,8 +87,10 @@ def run_experts(x: torch.Tensor, ex: grouped.Experts | mx_experts.Experts, buf: 
 
     if isinstance(ex, mx_experts.Experts):
         mx_experts.layer(x, ex, buf.plan, buf.y.view(-1, ex.dims), rows)
-    else:
-        grouped.layer(x, ex, buf.plan, buf.act.view(-1, ex.width), buf.y.view(-1, ex.dims), rows)
+        return
+    if buf.act is None:
+        raise ValueError("experts: these buffers were made for microscaled experts")
+    grouped.layer(x, ex, buf.plan, buf.act.view(-1, ex.width), buf.y.view(-1, ex.dims), rows)
 
 
 @dataclass
@@ -202,8 +205,9 @@ def run(x: torch.Tensor, m: Routed, *, prefill: bool = False, f32: bool = False)
 
     rows = x.shape[0]
     size = 1 << max(4, (rows - 1).bit_length())                 # scratch per power of two, reused by every layer
-    shape = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, x.device, m.experts.count, prefill and f32)
+    microscaled = isinstance(m.experts, mx_experts.Experts)
+    shape = (size, m.count, m.top_k, m.experts.width, m.experts.dims, prefill, x.device, m.experts.count, prefill and f32, microscaled)
     buf = _kept(shape, *_lib.use_of(x), lambda cleared: MoEBuffers(size, _Shape(m), x.device, prefill=prefill, table_experts=m.experts.count,
-                                                                   f32=f32, cleared=cleared))
+                                                                   f32=f32, microscaled=microscaled, cleared=cleared))
     moe(x.contiguous(), m.router, m.experts, buf, m.top_k, m.count, m.shared)
     return combine(buf.y[:rows], buf.wts[:rows])

@@ -195,7 +195,8 @@ class ExpertParallelMoE:
         class _Cfg:
             num_experts_per_tok, num_experts = self.top_k, self.total
             moe_intermediate_size, hidden_size = self.experts.width, self.experts.dims
-        return moe.MoEBuffers(rows, _Cfg, device, prefill=prefill, table_experts=self.experts.count, f32=f32)
+        return moe.MoEBuffers(rows, _Cfg, device, prefill=prefill, table_experts=self.experts.count, f32=f32,
+                              microscaled=isinstance(self.experts, mx_experts.Experts))
 
     def partial(self, x: torch.Tensor, buf: moe.MoEBuffers, out: torch.Tensor | None = None) -> torch.Tensor:
         """This rank's contribution [R, D] bf16: its experts' slots combined, the others weighted zero."""

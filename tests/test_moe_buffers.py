@@ -1,5 +1,6 @@
 """Which buffers a call of ``moe.run`` uses (no GPU: nothing is launched)."""
 
+import pytest
 import torch
 
 from tensorfold_b200.cuda import moe
@@ -32,6 +33,9 @@ def test_streams_and_captures_have_buffers_of_their_own(monkeypatch):
     assert not any(buf is second for _, buf in moe._captured.values())
 
 
-def test_prompt_pairs_may_stay_unrounded():
+def test_what_buffers_hold():
+    assert moe.MoEBuffers(4, Cfg, "cpu", microscaled=True).act is None and moe.MoEBuffers(4, Cfg, "cpu").act.shape == (4, 3, 64)
+    with pytest.raises(ValueError):
+        moe.run_experts(None, None, moe.MoEBuffers(4, Cfg, "cpu", microscaled=True), 4)
     for prefill, f32, dtype in ((False, False, torch.float32), (True, False, torch.bfloat16), (True, True, torch.float32)):
         assert moe.MoEBuffers(4, Cfg, "cpu", prefill=prefill, f32=f32).y.dtype == dtype

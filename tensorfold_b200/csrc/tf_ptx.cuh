@@ -317,6 +317,24 @@ __device__ __forceinline__ uint4 transpose8(const float (&v)[8], int lane) {
   return make_uint4(p[0], p[1], p[2], p[3]);
 }
 
+// Four lanes each hold four rows of one column; afterwards each holds four columns of one row: lane l of the group gets row l.
+__device__ __forceinline__ float4 transpose4(float a, float b, float c, float d, int lane) {
+  const bool odd = lane & 1, upper = lane & 2;
+  float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? a : b, 1);
+  if (odd) a = got;
+  else b = got;
+  got = __shfl_xor_sync(0xFFFFFFFFu, odd ? c : d, 1);
+  if (odd) c = got;
+  else d = got;
+  got = __shfl_xor_sync(0xFFFFFFFFu, upper ? a : c, 2);
+  if (upper) a = got;
+  else c = got;
+  got = __shfl_xor_sync(0xFFFFFFFFu, upper ? b : d, 2);
+  if (upper) b = got;
+  else d = got;
+  return make_float4(a, b, c, d);
+}
+
 // Programmatic dependent launch: wait for the grid this one depends on (no-op without the launch attribute), and
 // let the dependent grid start its own prologue.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

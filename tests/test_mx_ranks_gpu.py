@@ -46,6 +46,21 @@ def test_row_and_column_parallel(tmp_path, rows, world):
     ckpt.close()
 
 
+def test_segments_read_on_the_device(tmp_path):
+    """A rank's share of stacked projections: a run of rows of each, joined on the device."""
+
+    codes, scales = mx_util.random_weight(96, 256, 3, DEV)
+    words, bytes_ = stored((codes, scales))
+    ckpt = saved(tmp_path, {"q.weight": words.cpu().view(torch.uint32), "q.scales": bytes_.cpu()})
+    for rank in range(2):
+        w, s = ckpt.microscaled("q", device=DEV, rank=rank, world=2, parallel="column", segments=(64, 32))
+        rows = torch.cat([torch.arange(32) + 32 * rank, torch.arange(16) + 64 + 16 * rank]).to(DEV)
+        assert w.dtype == torch.int32 and torch.equal(w, words[rows]) and torch.equal(s, bytes_[rows])
+        q = checkpoint.load_microscaled(ckpt, "q", DEV, rank=rank, world=2, parallel="column", segments=(64, 32))
+        assert (q.n, q.k) == (48, 256)
+    ckpt.close()
+
+
 @pytest.mark.parametrize("rows,prefill,f32", [(1, False, False), (9, False, False), (40, True, False), (200, True, True)])
 def test_expert_parallel(rows, prefill, f32):
     """A rank's partial is the sum over the pairs whose expert it owns, with those pairs' bits in the whole table."""

@@ -6,7 +6,8 @@ import torch
 import mx_util
 from tensorfold_b200 import _lib, synthetic
 from tensorfold_b200.cuda import experts, moe, mx_experts
-from test_mx_experts_gpu import build
+from tensorfold_b200.cuda.kernels import mx
+from test_mx_experts_gpu import build, stored
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -48,13 +49,16 @@ def affine_layer(e=12, d=384, ni=128, k=3):
     return moe.Routed(layer_of(e=e, d=d, ni=ni, k=k).router, ex, k)
 
 
-@pytest.mark.parametrize("kind", ["mx", "affine"])
+@pytest.mark.parametrize("kind", ["mx", "affine", "shared"])
 @pytest.mark.parametrize("rows,prefill", [(5, False), (40, True)])
 def test_layers_of_one_shape_run_side_by_side(kind, rows, prefill, monkeypatch):
     """A layer that is held up between its plan and its experts, while another of its shape runs from end to end on another stream or in
     a graph, still gets its own plan's pairs."""
 
-    layer = layer_of() if kind == "mx" else affine_layer()
+    layer = affine_layer() if kind == "affine" else layer_of()
+    if kind == "shared":
+        ws = [stored(mx_util.random_weight(*shape, 40, DEV)) for shape in ((256, 384), (256, 384), (384, 256))]
+        layer = moe.Routed(torch.cat([layer.router, layer.router[:1]]), layer.experts, 3, moe.SharedExpert(mx.pack_pair(*ws[:2]), mx.pack(ws[2][0], ws[2][1])))
     xs = [mx_util.rows(rows, 384, seed, DEV, std=0.5) for seed in (1, 2, 3)]
     want = [moe.run(x, layer, prefill=prefill) for x in xs]
     slow, quick = torch.cuda.Stream(), torch.cuda.Stream()

@@ -1021,7 +1021,7 @@ cudaError_t launch(MxParams& p, int64_t tiles, bool quant_out, int sms, cudaStre
     ++count;
   }
   // always: a block sets up under the previous kernel's end, and reads and writes global memory once that is done (weights and plan
-  // earlier where they are settled)
+  // earlier where they are settled; with a plan that is not, it waits before its set-up too)
   attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[count].val.programmaticStreamSerializationAllowed = 1;
   ++count;
@@ -1078,9 +1078,12 @@ int round8(int m) { return (m + 7) / 8 * 8; }
 // four MMAs read 16 KB and 128 bytes a row again; a pair halves the rows' part, but its stages pass from block to block.  A tile has a
 // start and an end besides, and slices that blocks exchange cost by the row.  Tiles in several slices stay below 128 rows: the
 // sums of taller ones do not fit the drain's registers.
-// Measured, us from graphs, as chosen / the other way: pairs 17408 x 5120 at 2048 rows 80 with / 87 without, at 700 35 with / 36,
-// at 150 15.4 without / 18.8, 10240 x 2560 at 1000 19.5 with / 20.3; exchange 5120 x 17408 at 48 rows 14.3 with / 18.8 without, 6144 x 5120
-// 8.9 with / 9.8, at 128 11.0 without / 13.5, 4096 x 4096 at 32 7.5 with / 8.1, at 128 9.1 without / 11.5.
+// Measured, us from graphs on weights that L2 does not hold, as chosen / the other way: pairs 17408 x 5120 at 2048 rows 92 with / 101 without,
+// at 700 35.2 with / 36.2, at 150 15.0 without / 18.0, 10240 x 2560 at 1000 19.8 with / 20.9; exchange 5120 x 17408 at 48 rows 14.1 with /
+// 18.1 without, 6144 x 5120 at 24 8.2 with / 9.1, at 128 10.4 without / 13.7, 4096 x 4096 at 32 7.3 with / 7.9, at 128 8.9 without / 11.2.
+// Where the model is off: 6144 x 5120 at 33 rows 8.9 without exchange / 8.5 with, at 48 9.2 / 8.9; 10240 x 2560 at 256 rows 15.0 without
+// pairs / 13.9 with; and pairs are held to eight stages, which measurements do not bear out: 248320 x 1024 (four) at 600 rows 162
+// without / 149 with.
 struct Tiling {
   int tile, cluster;
   bool pair;
@@ -1114,8 +1117,10 @@ bool fused_fits(int k, int sk) {
 
 // Whether a block should quantise its rows itself: it holds its K slice of them beside a ring of four slots, and its six idle warps
 // have few segments of 1024 inputs each.
-// Measured, us from graphs, in the block / from their own kernel: 17408 x 5120 (five segments a row) at 2 rows 10.3 / 11.9, at 4 11.5 / 11.9,
-// at 6 12.7 / 11.8; 5120 x 17408 (six) at 1 row 11.1 / 12.7, at 4 13.1 / 12.6; 4096 x 4096 (one) at 16 rows 6.5 / 6.7.
+// Measured, us from graphs on weights that L2 does not hold, in the block / from their own kernel, at 24 segments: 5120 x 17408 (six a row)
+// at 4 rows 12.2 / 12.6, 14336 x 4096 (four) at 6 8.7 / 9.1, 6144 x 5120 (three) at 8 7.6 / 7.9, 10240 x 2560 (three) at 8 6.8 / 6.7, 4096 x 8192
+// (two) at 12 8.1 / 8.4, 2048 x 8192 (two) at 12 7.6 / 7.2, the worst of nine; at 20 to 22 all nine gain, 1 to 12 %; past 24, 17408 x 5120
+// (five) at 6 12.7 / 11.8.
 constexpr int FUSED_SEGMENTS = 24;
 bool fused_pays(int m, int k, int sk) {
   if (m > MX_FUSED_ROWS || !fused_fits(k, sk)) return false;

@@ -3,7 +3,8 @@ product of quantised rows with quantised weights on the block-scaled tensor core
 
 Beside ``qmm`` (affine integers): a checkpoint's words [n, k / 8] and scale bytes [n, k / 32] become an ``MX4`` with ``pack``, and
 ``matmul`` takes any number of rows.  Rows of x are quantised to the same format inside the call, so both operands of a product
-have four bits; sums are fp32.  A row's bits never depend on the row count.
+have four bits; sums are fp32.  A row's bits never depend on the row count.  Rounding N(0, 1) rows moves a product by 0.11 of its norm,
+as much as rounding N(0, 0.02) weights does; rows with one channel in 64 eight times as large by 0.15.
 """
 
 from __future__ import annotations

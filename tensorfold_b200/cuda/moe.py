@@ -118,6 +118,8 @@ def moe(x: torch.Tensor, router_rows: torch.Tensor, ex: grouped.Experts | mx_exp
 
     def dense() -> None:
         if isinstance(shared.up, mx.MX4):
+            # two products of their own, so the activations are rounded to bf16 between them and then to four bits; the routed experts
+            # round them once.  0.5 % of the codes differ, the activations' error (0.145 of them, four bits) does not.
             act = mx.matmul_act(x, shared.up, act="swiglu", limit=shared.limit)
             mx.matmul(act, shared.down, f32=buf.y.dtype == torch.float32, out=buf.y[:rows, top_k])
         elif buf.plan.prefill:                                    # prefill arithmetic for the dense shared expert too
